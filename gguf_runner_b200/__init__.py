@@ -9,8 +9,10 @@ calls raise.
 from .binding import (  # noqa: F401
     AttnConfig,
     AttnContext,
+    Batch,
     GgrError,
     MediaAttentionPlan,
+    Pages,
     RopePositionPlan,
     Weights,
     gemma_layer_windows,

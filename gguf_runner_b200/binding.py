@@ -23,6 +23,7 @@ _LIB = None
 PTR_HOST, PTR_DEVICE = 0, 1
 DTYPE_F32, DTYPE_BF16 = 0, 1
 KV_F32, KV_BF16, KV_Q8_ROW, KV_Q8_BLOCK32, KV_TURBO = 0, 1, 2, 3, 4
+KV_Q8_HEAD = 5  # pages only
 ROPE_NEOX, ROPE_ADJACENT = 0, 1
 ROPE_SEQUENTIAL, ROPE_INTERLEAVED = 0, 1
 SCALE_SCORE, SCALE_Q_PRESCALED = 0, 1
@@ -33,6 +34,8 @@ IMPL_AUTO, IMPL_SIMT, IMPL_MMA, IMPL_TCGEN05 = 0, 1, 2, 3
 W_F32, W_BF16, W_Q8_0, W_Q4_K, W_Q6_K = 0, 1, 2, 3, 4
 
 KV_FORMATS = {"f32": KV_F32, "bf16": KV_BF16, "q8_row": KV_Q8_ROW, "q8_block32": KV_Q8_BLOCK32, "turbo": KV_TURBO}
+PAGE_FORMATS = {"bf16": KV_BF16, "q8_head": KV_Q8_HEAD}
+DTYPES = {"f32": DTYPE_F32, "bf16": DTYPE_BF16}
 
 
 class GgrError(RuntimeError):
@@ -80,6 +83,8 @@ EXPORTED_SYMBOLS = [
     "ggr_weights_upload", "ggr_weights_free", "ggr_proj_matmul", "ggr_attn_layer_decode", "ggr_attn_layer_prefill",
     "ggr_rope_plan_new", "ggr_rope_plan_free", "ggr_rope_plan_append_text", "ggr_rope_plan_append_grid",
     "ggr_rope_plan_len", "ggr_rope_plan_next_text", "ggr_rope_plan_at", "ggr_rope_plan_export",
+    "ggr_pages_create", "ggr_pages_destroy", "ggr_pages_device_ptrs", "ggr_batch_create", "ggr_batch_destroy", "ggr_batch_set",
+    "ggr_paged_append", "ggr_paged_read", "ggr_paged_attention", "ggr_packed_attention",
     "ggr_rope_axis", "ggr_media_plan_validate", "ggr_media_chunk_end", "ggr_gemma_layer_windows",
 ]
 
@@ -156,6 +161,18 @@ def lib() -> C.CDLL:
     L.ggr_attn_kernel_time.argtypes = [vp, i32, C.POINTER(C.c_double), C.POINTER(i64), i32]
     L.ggr_attn_kv_device_ptrs.argtypes = [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp),
                                           C.POINTER(C.c_uint64)]
+    L.ggr_pages_create.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, C.POINTER(vp)]
+    L.ggr_pages_destroy.argtypes = [vp]
+    L.ggr_pages_destroy.restype = None
+    L.ggr_pages_device_ptrs.argtypes = [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(C.c_uint64)]
+    L.ggr_batch_create.argtypes = [vp, vp, i32, i32, i32, i32, C.POINTER(vp)]
+    L.ggr_batch_destroy.argtypes = [vp]
+    L.ggr_batch_destroy.restype = None
+    L.ggr_batch_set.argtypes = [vp, i32, vp, vp, vp, i32]
+    L.ggr_paged_append.argtypes = [vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp]
+    L.ggr_paged_read.argtypes = [vp, vp, i32, i32, vp, i64, vp, i64]
+    L.ggr_paged_attention.argtypes = [vp, vp, i32, vp, i64, vp, i64]
+    L.ggr_packed_attention.argtypes = [vp, vp, i32, vp, i64, vp, i64, vp, i64, vp, i64]
     L.ggr_rope_plan_new.restype = vp
     L.ggr_rope_plan_free.argtypes = [vp]
     L.ggr_rope_plan_free.restype = None
@@ -296,6 +313,105 @@ def _ptr(x, want_dtype=None):
     if want_dtype is not None and a.dtype != want_dtype:
         raise ValueError(f"buffer dtype {a.dtype} != {want_dtype}")
     return C.c_void_p(a.ctypes.data), PTR_HOST
+
+
+class Pages:
+    """A pool of cache pages for every layer of a context: K and V [layer][page][KV head][position][head_dim] in bf16, or int8
+    with f32 scales [layer][page][KV head][position] (`q8_head`). Without tensors the library allocates (and clears) the pool;
+    with them (k, v, and the scales of an int8 pool) it uses the caller's, which the object keeps alive."""
+
+    def __init__(self, ctx: "AttnContext", n_pages: int, page_size: int, kv_format: str = "bf16", k=None, v=None, k_scale=None,
+                 v_scale=None):
+        if kv_format not in PAGE_FORMATS:
+            raise ValueError(f"page format {kv_format!r} is not one of {sorted(PAGE_FORMATS)}")
+        cfg = ctx.config
+        self._L, self.ctx, self.n_pages, self.page_size, self.kv_format = lib(), ctx, n_pages, page_size, kv_format
+        self.arrays = (k, v, k_scale, v_scale)
+        rows = cfg.n_layers * n_pages * cfg.n_kv_heads * page_size
+        q8 = kv_format == "q8_head"
+        ptrs = []
+        for name, x, n, dtype in (("k", k, rows * cfg.head_dim, "int8" if q8 else "bfloat16"),
+                                  ("v", v, rows * cfg.head_dim, "int8" if q8 else "bfloat16"),
+                                  ("k_scale", k_scale, rows, "float32"), ("v_scale", v_scale, rows, "float32")):
+            if x is not None:
+                ctx._check_tensor(name, x, dtype)
+                if not x.is_contiguous() or x.numel() != n:
+                    raise ValueError(f"{name}: a page pool of this shape has {n} contiguous elements")
+            ptrs.append(None if x is None else C.c_void_p(x.data_ptr()))
+        h = C.c_void_p()
+        ctx._follow_torch_stream(k)
+        ctx._check(self._L.ggr_pages_create(ctx._h, n_pages, page_size, PAGE_FORMATS[kv_format], *ptrs, C.byref(h)))
+        self._h = h
+
+    def device_ptrs(self):
+        """Device addresses (k, v, k_scale, v_scale) and the byte size of the K (or V) array."""
+        k, v, ks, vs, nb = C.c_void_p(), C.c_void_p(), C.c_void_p(), C.c_void_p(), C.c_uint64()
+        self.ctx._check(self._L.ggr_pages_device_ptrs(self._h, C.byref(k), C.byref(v), C.byref(ks), C.byref(vs), C.byref(nb)))
+        return k.value, v.value, ks.value, vs.value, nb.value
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._L.ggr_pages_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Batch:
+    """Plan of a step over several sequences: `set` takes the new-token counts, the lengths and the page table, the
+    `paged_*` calls (with `pages=None`: `packed_attention`) of the context then work by it, layer after layer. `dtype` is that
+    of the rows, "bf16" or "f32"."""
+
+    def __init__(self, ctx: "AttnContext", pages: Optional[Pages], dtype: str, max_seqs: int, max_tokens: int, max_pages: int = 0):
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
+        self._L, self.ctx, self.pages, self.dtype = lib(), ctx, pages, dtype
+        self.max_tokens, self.n_tokens, self.n_rows = max_tokens, 0, 0
+        self.torch_dtype = "float32" if dtype == "f32" else "bfloat16"
+        h = C.c_void_p()
+        ctx._check(self._L.ggr_batch_create(ctx._h, None if pages is None else pages._h, DTYPES[dtype], max_seqs, max_tokens, max_pages,
+                                            C.byref(h)))
+        self._h = h
+
+    def set(self, q_len, kv_len=None, page_table=None):
+        """page_table: a row of page ids per sequence (a list of lists, or a 2-D array padded with anything)."""
+        q = np.ascontiguousarray(q_len, dtype=np.int32).reshape(-1)
+        kv = q if kv_len is None else np.ascontiguousarray(kv_len, dtype=np.int32).reshape(-1)
+        if q.shape != kv.shape:
+            raise ValueError("q_len and kv_len have different lengths")
+        if page_table is None:
+            table = np.empty((q.size, 0), np.int32)
+        elif isinstance(page_table, np.ndarray):
+            table = np.ascontiguousarray(page_table, dtype=np.int32)
+        else:
+            rows = [np.asarray(r, dtype=np.int32).reshape(-1) for r in page_table]
+            table = np.zeros((len(rows), max((r.size for r in rows), default=0)), np.int32)
+            for i, r in enumerate(rows):
+                if self.pages is not None and i < kv.size and r.size * self.pages.page_size < kv[i]:
+                    raise ValueError(f"sequence {i} has {kv[i]} tokens and {r.size} pages")
+                table[i, :r.size] = r
+        if table.ndim != 2 or table.shape[0] != q.size:
+            raise ValueError("the page table has one row per sequence")
+        self.ctx._follow_torch_stream_of_device()
+        self.n_tokens = self.n_rows = 0
+        self.ctx._check(self._L.ggr_batch_set(self._h, q.size, q.ctypes.data, kv.ctypes.data, table.ctypes.data if table.size else None,
+                                              table.shape[1]))
+        self.n_tokens, self.n_rows = int(q.sum()), int(kv.sum())
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._L.ggr_batch_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class AttnContext:
@@ -613,6 +729,88 @@ class AttnContext:
         return out
 
     # ---- cache access ------------------------------------------------------------------
+    # ---- batches over pages, packed prompts --------------------------------------------
+    def _check_tensor(self, name, x, dtype):
+        if not _is_torch(x) or not x.is_cuda or x.device.index != self.config.device:
+            raise ValueError(f"{name} must be a CUDA tensor on device {self.config.device}")
+        if str(x.dtype) != "torch." + dtype:
+            raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
+
+    def _follow_torch_stream_of_device(self):
+        import torch
+        handle = torch.cuda.current_stream(self.config.device).cuda_stream or 1
+        if handle != self._stream:
+            self.set_stream(handle)
+
+    def _rows(self, name, x, dtype, n, dim):
+        """Address and row stride of `n` rows (a [rows][dim] tensor whose elements of a row lie together)."""
+        self._check_tensor(name, x, dtype)
+        if x.dim() != 2 or x.shape[0] < n or x.shape[1] != dim or (dim > 1 and x.stride(1) != 1):
+            raise ValueError(f"{name} must have at least {n} rows of {dim} elements, each row contiguous")
+        return x.data_ptr(), (x.stride(0) if x.shape[0] > 1 else dim)
+
+    def _row_out(self, out, like, n, dim, dtype):
+        if out is None:
+            import torch
+            return torch.empty((n, dim), dtype=getattr(torch, dtype), device=like.device)
+        return out
+
+    def paged_append(self, batch: Batch, layer: int, k, v, q=None, q_out=None):
+        """Rows of k and v into the pages of the batch's new tokens. With q: RoPE on q and k first; returns rotated q."""
+        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
+        kp, ks = self._rows("k", k, dt, n, c.kv_dim)
+        vp, vs = self._rows("v", v, dt, n, c.kv_dim)
+        qp, qs, op = None, 0, None
+        if q is not None:
+            q_out = self._row_out(q_out, q, n, c.q_dim, dt)
+            qp, qs = self._rows("q", q, dt, n, c.q_dim)
+            op, os_ = self._rows("q_out", q_out, dt, n, c.q_dim)
+            if os_ != c.q_dim:
+                raise ValueError("q_out must be dense")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        self._follow_torch_stream(k)
+        self._check(self._L.ggr_paged_append(self._h, batch._h, layer, 0 if q is None else 1, qp, qs, kp, ks, vp, vs, op))
+        return q_out
+
+    def paged_read(self, batch: Batch, layer: int, dtype: str = "bf16", k_out=None, v_out=None):
+        """All cached rows of all sequences of the batch, dequantised: (k, v), each [sum of kv_len][kv_dim]."""
+        import torch
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
+        name, c, n = "float32" if dtype == "f32" else "bfloat16", self.config, batch.n_rows
+        k_out, v_out = (torch.empty((n, c.kv_dim), dtype=getattr(torch, name), device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
+        kp, ks = self._rows("k_out", k_out, name, n, c.kv_dim)
+        vp, vs = self._rows("v_out", v_out, name, n, c.kv_dim)
+        self._follow_torch_stream(k_out)
+        self._check(self._L.ggr_paged_read(self._h, batch._h, layer, DTYPES[dtype], kp, ks, vp, vs))
+        return k_out, v_out
+
+    def paged_attention(self, batch: Batch, layer: int, q, out=None):
+        """Attention of the batch's new tokens (rotated q) over their sequences' pages."""
+        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
+        out = self._row_out(out, q, n, c.q_dim, dt)
+        qp, qs = self._rows("q", q, dt, n, c.q_dim)
+        op, os_ = self._rows("out", out, dt, n, c.q_dim)
+        self._follow_torch_stream(q)
+        self._check(self._L.ggr_paged_attention(self._h, batch._h, layer, qp, qs, op, os_))
+        return out
+
+    def packed_attention(self, batch: Batch, layer: int, q, k, v, out=None):
+        """Causal attention of whole prompts from their rotated q, k and v rows (a batch without pages)."""
+        import torch
+        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
+        if torch.cuda.is_current_stream_capturing():
+            n = batch.max_tokens  # replays may find a longer plan
+        out = self._row_out(out, q, n, c.q_dim, dt)
+        qp, qs = self._rows("q", q, dt, n, c.q_dim)
+        kp, ks = self._rows("k", k, dt, n, c.kv_dim)
+        vp, vs = self._rows("v", v, dt, n, c.kv_dim)
+        op, os_ = self._rows("out", out, dt, n, c.q_dim)
+        self._follow_torch_stream(q)
+        self._check(self._L.ggr_packed_attention(self._h, batch._h, layer, qp, qs, kp, ks, vp, vs, op, os_))
+        return out
+
     def kv_read_row(self, layer: int, pos: int, seq: int = 0):
         k = np.empty(self.config.kv_dim, dtype=np.float32)
         v = np.empty(self.config.kv_dim, dtype=np.float32)

@@ -19,6 +19,7 @@
 #include "attn_turbo.cuh"
 #include "attn_turbo_mma.cuh"
 #include "common.cuh"
+#include "path_view.h"
 #include "prefill_split.cuh"
 #include "prefill_tc.cuh"
 #include "prefill_tc_wide.cuh"
@@ -2995,3 +2996,49 @@ extern "C" int ggr_attn_layer_prefill(ggr_attn_ctx* c, int32_t layer, int32_t se
     }
     return GGR_OK;
 }
+
+// ---- what the other translation units see of a context (path_view.h) ------------------------------
+
+namespace ggr {
+
+PathView path_view(const ggr_attn_ctx* c) {
+    PathView v{};
+    v.device = c->cfg.device;
+    v.n_layers = c->cfg.n_layers;
+    v.Hq = c->cfg.n_heads;
+    v.Hkv = c->cfg.n_kv_heads;
+    v.D = c->D;
+    v.G = c->G;
+    v.rope_dim = c->rope_dim;
+    v.sm_count = c->sm_count;
+    v.smem_optin = c->smem_optin;
+    v.stream = c->stream;
+    v.score_scale = c->cfg.scale_mode == GGR_SCALE_SCORE ? c->attn_scale : 1.0f;
+    v.position_plan = c->has_plan != 0;
+    v.image_blocks = c->cfg.image_mode == GGR_IMAGE_BIDIRECTIONAL && !c->blocks.empty();
+    v.sharded = c->cfg.shard_mode != GGR_SHARD_NONE;
+    v.d_err = c->d_err;
+    v.windows = &c->windows;
+    return v;
+}
+RopeParams path_rope(const ggr_attn_ctx* c, int layer) { return rope_params(c, layer); }
+int path_fail(ggr_attn_ctx* c, int status, const std::string& msg) { return fail(c, status, msg); }
+void path_create_error(const std::string& msg) { g_create_err = msg; }
+bool path_capturing(ggr_attn_ctx* c) { return capturing(c); }
+void path_launched(ggr_attn_ctx* c) { c->launches++; }
+cudaEvent_t path_timer_start(ggr_attn_ctx* c, int kind) {
+    LaunchTimer t(c, kind);
+    const cudaEvent_t stop = t.stop;
+    t.stop = nullptr;
+    return stop;
+}
+void path_timer_stop(ggr_attn_ctx* c, cudaEvent_t stop) {
+    if (stop) cudaEventRecord(stop, c->stream);
+}
+bool path_has_fixups(const ggr_attn_ctx* c, int layer) { return (size_t)layer < c->fixups.size() && c->fixups[layer].any(); }
+int path_fixups(ggr_attn_ctx* c, int layer, int n, const void** q, const void** k, const void** v, int* in_bf16) {
+    if (use_turbo_prep(c)) return fail(c, GGR_ERR_UNSUPPORTED, "bias and QK-norm of a TurboQuant context are applied by its own append only");
+    return apply_fixups(c, layer, n, q, k, v, in_bf16, false);
+}
+
+}  // namespace ggr

@@ -1,0 +1,767 @@
+// Paged KV cache, batch plans, and attention over pages and over packed prompts: the host side of
+// include/ggr_attn.h's ggr_pages, ggr_batch, ggr_paged_* and ggr_packed_attention.
+//
+// A plan is made once per step (ggr_batch_set) and used by every layer: the lengths and page tables are cut on the host into
+// work items of equal size, which the kernels read from device memory. Captured launches therefore follow the plan: a graph of
+// a token step is replayed with the lengths that the last ggr_batch_set gave.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <memory>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "../../include/ggr_attn.h"
+#include "paged.cuh"
+#include "paged_mma.cuh"
+#include "path_view.h"
+
+using namespace ggr;
+
+static_assert(kKvQ8Head == GGR_KV_Q8_HEAD, "page format");
+
+struct ggr_pages {
+    ggr_attn_ctx* ctx;
+    int device, n_layers, page_size;
+    PageView v{};
+    void* owned[4] = {nullptr, nullptr, nullptr, nullptr};
+    CUtensorMap tmK16, tmV16;  // 16 rows of a page, one 64- or 128-byte block of columns
+};
+
+namespace {
+
+constexpr int kMaxLists = 4;  // distinct windows of a model's layers
+enum Kind { kSplitK = 0, kRows = 1, kKinds = 2 };
+
+struct Guard {
+    int prev = -1;
+    explicit Guard(int dev) {
+        cudaGetDevice(&prev);
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~Guard() {
+        int cur = -1;
+        cudaGetDevice(&cur);
+        if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+    }
+};
+
+#define PAGED_TRY(c, expr)                                                                              \
+    do {                                                                                                \
+        cudaError_t e_ = (expr);                                                                        \
+        if (e_ != cudaSuccess)                                                                          \
+            return path_fail(c, GGR_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_));      \
+    } while (0)
+
+int elem_bytes(int dtype) { return dtype == GGR_DTYPE_F32 ? 4 : 2; }
+
+// dims (x: elements, y, z), strides in bytes of y and z; box (bx, by, bz); the block of columns decides the swizzle
+bool make_map3(CUtensorMap* map, bool bytes, const void* base, uint64_t dx, uint64_t dy, uint64_t dz, uint64_t sy, uint64_t sz, uint32_t bx, uint32_t by,
+               uint32_t bz) {
+    PFN_tmapEncodeTiled enc = tmap_encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {dx, dy, dz}, strides[2] = {sy, sz};
+    const cuuint32_t box[3] = {bx, by, bz}, estr[3] = {1, 1, 1};
+    const uint32_t row = bx * (bytes ? 1 : 2);
+    return enc(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+struct ggr_batch {
+    ggr_attn_ctx* ctx;
+    ggr_pages* pages;  // null: packed prompts
+    int device, dtype, max_seqs, max_tokens, max_pages;
+    int Hq, Hkv, D, G, sm_count, smem_optin, n_layers;
+    std::vector<int> list_of;   // layer -> list
+    std::vector<int> windows;   // list -> window
+    size_t item_cap[kKinds] = {};
+    size_t part_tiles = 0;      // partial states (of 16 rows, per KV head) that the scratch holds
+    // device image of the plan: fixed places, so that captured launches keep their pointers
+    unsigned char* d_plan = nullptr;
+    unsigned char* h_plan[2] = {nullptr, nullptr};
+    cudaEvent_t up[2] = {nullptr, nullptr};
+    bool up_used[2] = {false, false};
+    int turn = 0;
+    size_t at_counts = 0, at_pos = 0, at_slot = 0, at_entries = 0, at_table = 0, at_items[kMaxLists][kKinds] = {}, bytes = 0;
+    float* d_part = nullptr;
+    unsigned* d_tickets = nullptr;
+    __nv_bfloat16* d_planes = nullptr;  // packed f32 rows: [k, v][2 planes][max_tokens][Hkv * D]
+    // the plan in force
+    bool set = false;
+    int n_seqs = 0, n_tokens = 0, n_entries = 0, n_rows = 0;
+    int n_items[kMaxLists][kKinds] = {};
+    std::vector<PagedItem> scratch;
+    std::vector<int> page_owner;  // stamp of the sequence whose new rows a page receives
+    int stamp = 0;
+
+    const int* counts(int list, int kind) const { return reinterpret_cast<const int*>(d_plan + at_counts) + (list * kKinds + kind) * 4; }
+    const int* table() const { return reinterpret_cast<const int*>(d_plan + at_table); }
+    const PagedItem* items(int list, int kind) const { return reinterpret_cast<const PagedItem*>(d_plan + at_items[list][kind]); }
+};
+
+namespace {
+
+// ---- planning --------------------------------------------------------------------------------------
+
+struct Tile {
+    int seq, row0, rows, key0, key1;
+};
+
+// Size of the pieces that row tiles are cut into along their keys, in 16-key tiles. One CTA per SM streams a piece at its
+// share of the memory's rate and spends some microseconds on its start and its merge whatever its size, so pieces are made as
+// large as still gives every SM one, or (ragged batches) several. Modelled for a handful of counts per SM, smallest time taken.
+int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile_bytes, double sm_rate, int min_tiles, size_t max_pieces, int* longest_out) {
+    int64_t total = 0;
+    int longest = 1;
+    for (const Tile& t : tiles) {
+        const int n = (t.key1 - t.key0 + 15) / 16;
+        total += n;
+        longest = std::max(longest, n);
+    }
+    *longest_out = longest;
+    int best = longest;
+    double best_cost = -1.0;
+    auto consider = [&](int piece) {
+        piece = std::max(piece, std::max(min_tiles, (longest + kPagedSplitMax - 1) / kPagedSplitMax));
+        piece = std::min(piece, longest);
+        int64_t pieces = 0, cut = 0;
+        for (const Tile& t : tiles) {
+            const int n = (t.key1 - t.key0 + 15) / 16, k = (n + piece - 1) / piece;
+            pieces += k;
+            if (k > 1) cut += k;
+        }
+        if ((size_t)cut > max_pieces) return;
+        const double ctas = (double)pieces * Hkv;
+        const double rate = std::min(sm_rate, 6.6e12 / std::min(ctas, (double)slots));
+        const double t0 = 3e-6, one = t0 + piece * tile_bytes / rate;
+        double cost = ctas <= slots ? one : (total * Hkv * tile_bytes / rate + ctas * t0) / slots + 0.5 * one;
+        if (cut) cost += 2.5e-6;
+        if (best_cost < 0.0 || cost < best_cost) {
+            best_cost = cost;
+            best = piece;
+        }
+    };
+    consider(longest);
+    for (int w = 1; w <= 12; ++w) {
+        // the smallest piece that gives at most w CTAs per SM
+        int lo = 1, hi = longest;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            int64_t pieces = 0;
+            for (const Tile& t : tiles) pieces += ((t.key1 - t.key0 + 15) / 16 + mid - 1) / mid;
+            if (pieces * Hkv <= (int64_t)w * slots)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        consider(lo);
+        if (lo <= min_tiles) break;
+    }
+    return best;
+}
+
+int first_key(int pos, int window) { return window > 0 ? std::max(0, pos + 1 - window) : 0; }
+
+}  // namespace
+
+extern "C" int ggr_pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v, float* k_scale, float* v_scale,
+                                ggr_pages** out) {
+    if (!c) return GGR_ERR_INVALID;
+    if (!out) return path_fail(c, GGR_ERR_INVALID, "null argument");
+    *out = nullptr;
+    const PathView p = path_view(c);
+    if (n_pages <= 0) return path_fail(c, GGR_ERR_INVALID, "a page pool needs at least one page");
+    if (page_size < kPageRowsMin || page_size > 256 || (page_size & (page_size - 1)))
+        return path_fail(c, GGR_ERR_INVALID, "page_size must be 16, 32, 64, 128 or 256");
+    if (kv_format != GGR_KV_BF16 && kv_format != GGR_KV_Q8_HEAD)
+        return path_fail(c, GGR_ERR_UNSUPPORTED, "pages are built in GGR_KV_BF16 and GGR_KV_Q8_HEAD");
+    if (p.D != 64 && p.D != 128 && p.D != 256) return path_fail(c, GGR_ERR_UNSUPPORTED, "pages are built for head_dim 64, 128 and 256");
+    if (p.sharded) return path_fail(c, GGR_ERR_UNSUPPORTED, "a context that holds a shard of the positions has no pages");
+    if ((int64_t)n_pages * page_size >= ((int64_t)1 << 31) || (int64_t)p.n_layers * n_pages * p.Hkv >= ((int64_t)1 << 31))
+        return path_fail(c, GGR_ERR_RANGE, "the page pool has more rows than a 32-bit index names");
+    const bool q8 = kv_format == GGR_KV_Q8_HEAD, given = k || v || k_scale || v_scale;
+    if (given && (!k || !v || (q8 && (!k_scale || !v_scale)) || (!q8 && (k_scale || v_scale))))
+        return path_fail(c, GGR_ERR_INVALID, "give all arrays of the page pool or none");
+    for (const void* x : {(const void*)k, (const void*)v, (const void*)k_scale, (const void*)v_scale})
+        if ((uintptr_t)x % 128) return path_fail(c, GGR_ERR_INVALID, "the arrays of a page pool must start on a 128-byte boundary");
+    Guard guard(p.device);
+    std::unique_ptr<ggr_pages> pg(new (std::nothrow) ggr_pages());
+    if (!pg) return path_fail(c, GGR_ERR_ALLOC, "out of host memory");
+    pg->ctx = c;
+    pg->device = p.device;
+    pg->n_layers = p.n_layers;
+    pg->page_size = page_size;
+    PageView& view = pg->v;
+    view.fmt = kv_format;
+    view.D = p.D;
+    view.Hkv = p.Hkv;
+    view.n_pages = n_pages;
+    while ((1 << view.page_log2) < page_size) ++view.page_log2;
+    const size_t rows = (size_t)p.n_layers * n_pages * p.Hkv * page_size, bytes = rows * p.D * (q8 ? 1 : 2);
+    if (given) {
+        view.k = static_cast<unsigned char*>(k);
+        view.v = static_cast<unsigned char*>(v);
+        view.ks = k_scale;
+        view.vs = v_scale;
+    } else {
+        for (int i = 0; i < (q8 ? 4 : 2); ++i) {
+            const size_t n = i < 2 ? bytes : rows * sizeof(float);
+            if (cudaMalloc(&pg->owned[i], n) != cudaSuccess || cudaMemsetAsync(pg->owned[i], 0, n, p.stream) != cudaSuccess) {
+                cudaGetLastError();
+                for (void* x : pg->owned) cudaFree(x);
+                return path_fail(c, GGR_ERR_ALLOC, "unable to allocate the page pool (" + std::to_string(2 * bytes) + " bytes)");
+            }
+        }
+        view.k = static_cast<unsigned char*>(pg->owned[0]);
+        view.v = static_cast<unsigned char*>(pg->owned[1]);
+        view.ks = static_cast<float*>(pg->owned[2]);
+        view.vs = static_cast<float*>(pg->owned[3]);
+    }
+    const uint64_t row_bytes = (uint64_t)p.D * (q8 ? 1 : 2), groups = (uint64_t)p.n_layers * n_pages * p.Hkv;
+    const uint32_t box = (uint32_t)(row_bytes < 128 ? row_bytes : 128) / (q8 ? 1 : 2);
+    for (int i = 0; i < 2; ++i)
+        if (!make_map3(i ? &pg->tmV16 : &pg->tmK16, q8, i ? view.v : view.k, p.D, page_size, groups, row_bytes, row_bytes * page_size, box, 16, 1)) {
+            for (void* x : pg->owned) cudaFree(x);
+            return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pool");
+        }
+    *out = pg.release();
+    return GGR_OK;
+}
+
+extern "C" void ggr_pages_destroy(ggr_pages* pages) {
+    if (!pages) return;
+    Guard guard(pages->device);
+    for (void* x : pages->owned) cudaFree(x);  // (cudaFree waits for the work that uses it)
+    delete pages;
+}
+
+extern "C" int ggr_pages_device_ptrs(const ggr_pages* pages, void** k, void** v, float** k_scale, float** v_scale, uint64_t* array_bytes) {
+    if (!pages) return GGR_ERR_INVALID;
+    if (k) *k = pages->v.k;
+    if (v) *v = pages->v.v;
+    if (k_scale) *k_scale = pages->v.ks;
+    if (v_scale) *v_scale = pages->v.vs;
+    if (array_bytes)
+        *array_bytes = (uint64_t)pages->n_layers * pages->v.n_pages * pages->v.Hkv * pages->page_size * pages->v.D * (pages->v.fmt == GGR_KV_Q8_HEAD ? 1 : 2);
+    return GGR_OK;
+}
+
+extern "C" void ggr_batch_destroy(ggr_batch* b) {
+    if (!b) return;
+    Guard guard(b->device);
+    for (int i = 0; i < 2; ++i) {
+        if (b->up_used[i]) cudaEventSynchronize(b->up[i]);
+        if (b->up[i]) cudaEventDestroy(b->up[i]);
+        if (b->h_plan[i]) cudaFreeHost(b->h_plan[i]);
+    }
+    cudaFree(b->d_plan);
+    cudaFree(b->d_part);
+    cudaFree(b->d_tickets);
+    cudaFree(b->d_planes);
+    delete b;
+}
+
+extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens, int32_t max_pages, ggr_batch** out) {
+    if (!c) return GGR_ERR_INVALID;
+    if (!out) return path_fail(c, GGR_ERR_INVALID, "null argument");
+    *out = nullptr;
+    const PathView p = path_view(c);
+    if (pages && pages->ctx != c) return path_fail(c, GGR_ERR_INVALID, "the pages belong to another context");
+    if (dtype != GGR_DTYPE_F32 && dtype != GGR_DTYPE_BF16) return path_fail(c, GGR_ERR_INVALID, "unknown dtype");
+    if (max_seqs <= 0 || max_tokens <= 0 || max_pages < (pages ? 1 : 0)) return path_fail(c, GGR_ERR_INVALID, "a batch plan needs room for a sequence, a token and a page");
+    if (p.D != 64 && p.D != 128 && p.D != 256) return path_fail(c, GGR_ERR_UNSUPPORTED, "batch plans are built for head_dim 64, 128 and 256");
+    if (p.sharded) return path_fail(c, GGR_ERR_UNSUPPORTED, "a context that holds a shard of the positions has no batch plans");
+    if ((int64_t)max_tokens * p.Hq * p.D >= ((int64_t)1 << 40)) return path_fail(c, GGR_ERR_RANGE, "max_tokens is out of range");
+    Guard guard(p.device);
+    std::unique_ptr<ggr_batch, void (*)(ggr_batch*)> b(new (std::nothrow) ggr_batch(), ggr_batch_destroy);
+    if (!b) return path_fail(c, GGR_ERR_ALLOC, "out of host memory");
+    b->ctx = c;
+    b->pages = pages;
+    b->device = p.device;
+    b->dtype = dtype;
+    b->max_seqs = max_seqs;
+    b->max_tokens = max_tokens;
+    b->max_pages = max_pages;
+    b->Hq = p.Hq;
+    b->Hkv = p.Hkv;
+    b->D = p.D;
+    b->G = p.G;
+    b->sm_count = p.sm_count;
+    b->smem_optin = p.smem_optin;
+    b->n_layers = p.n_layers;
+    for (int l = 0; l < p.n_layers; ++l) {
+        const int w = p.windows->empty() ? 0 : (*p.windows)[l];
+        size_t i = 0;
+        while (i < b->windows.size() && b->windows[i] != w) ++i;
+        if (i == b->windows.size()) b->windows.push_back(w);
+        b->list_of.push_back((int)i);
+    }
+    if (b->windows.size() > kMaxLists) return path_fail(c, GGR_ERR_UNSUPPORTED, "more than four distinct windows");
+    // items: row tiles of the longest plan, and the pieces that cutting them may add
+    const size_t rows = (size_t)max_tokens * p.G, lists = b->windows.size();
+    b->part_tiles = (size_t)(8 * p.sm_count + p.Hkv - 1) / p.Hkv + 16;
+    b->item_cap[kSplitK] = (rows + 15) / 16 + max_seqs + b->part_tiles;
+    b->item_cap[kRows] = (rows + 127) / 128 + max_seqs;
+    size_t at = 0;
+    auto place = [&](size_t n) {
+        const size_t here = at;
+        at = (at + n + 255) / 256 * 256;
+        return here;
+    };
+    b->at_counts = place(lists * kKinds * 4 * sizeof(int));
+    b->at_pos = place((size_t)max_tokens * sizeof(int));
+    b->at_slot = place((size_t)max_tokens * sizeof(int));
+    b->at_entries = place((size_t)max_pages * sizeof(int2));
+    b->at_table = place((size_t)max_pages * sizeof(int));
+    for (size_t l = 0; l < lists; ++l)
+        for (int k = 0; k < kKinds; ++k) b->at_items[l][k] = place(b->item_cap[k] * sizeof(PagedItem));
+    b->bytes = at;
+    const size_t state = 16 * (size_t)(p.D + 2) * sizeof(float) * p.Hkv;
+    bool ok = cudaMalloc((void**)&b->d_plan, b->bytes) == cudaSuccess && cudaMalloc((void**)&b->d_part, b->part_tiles * state) == cudaSuccess &&
+              cudaMalloc((void**)&b->d_tickets, b->part_tiles * p.Hkv * sizeof(unsigned)) == cudaSuccess;
+    if (ok && !pages && dtype == GGR_DTYPE_F32)
+        ok = cudaMalloc((void**)&b->d_planes, (size_t)4 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
+    for (int i = 0; ok && i < 2; ++i)
+        ok = cudaHostAlloc((void**)&b->h_plan[i], b->bytes, cudaHostAllocDefault) == cudaSuccess &&
+             cudaEventCreateWithFlags(&b->up[i], cudaEventDisableTiming) == cudaSuccess;
+    if (!ok) {
+        cudaGetLastError();
+        return path_fail(c, GGR_ERR_ALLOC, "unable to allocate the batch plan");
+    }
+    if (cudaMemsetAsync(b->d_plan, 0, b->bytes, p.stream) != cudaSuccess ||
+        cudaMemsetAsync(b->d_tickets, 0, b->part_tiles * p.Hkv * sizeof(unsigned), p.stream) != cudaSuccess)
+        return path_fail(c, GGR_ERR_CUDA, "unable to clear the batch plan");
+    if (pages) b->page_owner.assign(pages->v.n_pages, 0);
+    *out = b.release();
+    return GGR_OK;
+}
+
+extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table, int32_t table_stride) {
+    if (!b) return GGR_ERR_INVALID;
+    ggr_attn_ctx* c = b->ctx;
+    const PathView p = path_view(c);
+    if (n_seqs < 0 || n_seqs > b->max_seqs) return path_fail(c, GGR_ERR_RANGE, "more sequences than the batch plan holds");
+    if (n_seqs && (!q_len || !kv_len)) return path_fail(c, GGR_ERR_INVALID, "null argument");
+    const int ps = b->pages ? b->pages->page_size : 0;
+    int64_t tokens = 0, entries = 0, rows = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        if (q_len[i] < 0 || kv_len[i] < q_len[i]) return path_fail(c, GGR_ERR_INVALID, "kv_len counts the new tokens: it must be at least q_len, and q_len not negative");
+        if (!b->pages && kv_len[i] != q_len[i]) return path_fail(c, GGR_ERR_INVALID, "packed prompts have no cached keys: kv_len must equal q_len");
+        tokens += q_len[i];
+        rows += kv_len[i];
+        if (b->pages) {
+            const int n = (int)(((int64_t)kv_len[i] + ps - 1) / ps);
+            if (n > table_stride) return path_fail(c, GGR_ERR_RANGE, "a sequence has more pages than a row of the page table");
+            entries += n;
+        }
+    }
+    if (tokens > b->max_tokens) return path_fail(c, GGR_ERR_RANGE, "more new tokens than the batch plan holds");
+    if (entries > b->max_pages) return path_fail(c, GGR_ERR_RANGE, "more pages than the batch plan holds");
+    if (rows >= ((int64_t)1 << 31)) return path_fail(c, GGR_ERR_RANGE, "more rows than a 32-bit index names");
+    if (entries && !page_table) return path_fail(c, GGR_ERR_INVALID, "null page table");
+    if (b->pages) {
+        // a page takes new rows of one sequence only: two would write the same place
+        if (b->stamp > (1 << 30)) {
+            std::fill(b->page_owner.begin(), b->page_owner.end(), 0);
+            b->stamp = 0;
+        }
+        const int stamp0 = b->stamp;
+        b->stamp += n_seqs;
+        for (int i = 0; i < n_seqs; ++i) {
+            const int32_t* row = page_table + (int64_t)i * table_stride;
+            const int n = (kv_len[i] + ps - 1) / ps;
+            for (int j = 0; j < n; ++j) {
+                if (row[j] < 0 || row[j] >= b->pages->v.n_pages) return path_fail(c, GGR_ERR_RANGE, "page table entry outside the pool");
+                if ((int64_t)(j + 1) * ps > kv_len[i] - q_len[i] && q_len[i] > 0) {
+                    int& owner = b->page_owner[row[j]];
+                    if (owner > stamp0) return path_fail(c, GGR_ERR_INVALID, "a page would receive new rows twice");
+                    owner = stamp0 + 1 + i;
+                }
+            }
+        }
+    }
+    Guard guard(b->device);
+    if (path_capturing(c)) return path_fail(c, GGR_ERR_INVALID, "a batch plan cannot be set while its stream is captured");
+    const int turn = b->turn;
+    unsigned char* h = b->h_plan[turn];
+    if (b->up_used[turn]) PAGED_TRY(c, cudaEventSynchronize(b->up[turn]));
+    b->set = false;
+    int* tok_pos = reinterpret_cast<int*>(h + b->at_pos);
+    int* tok_slot = reinterpret_cast<int*>(h + b->at_slot);
+    int2* entry = reinterpret_cast<int2*>(h + b->at_entries);
+    int* table = reinterpret_cast<int*>(h + b->at_table);
+    struct Seq {
+        int tok0, src;
+    };
+    std::vector<Seq> seqs(n_seqs);
+    {
+        int tok = 0, e = 0, dense = 0;
+        for (int i = 0; i < n_seqs; ++i) {
+            seqs[i] = {tok, b->pages ? e : tok};
+            const int first = kv_len[i] - q_len[i];
+            const int32_t* row = b->pages ? page_table + (int64_t)i * table_stride : nullptr;
+            for (int t = 0; t < q_len[i]; ++t, ++tok) {
+                tok_pos[tok] = first + t;
+                tok_slot[tok] = row ? row[(first + t) / ps] * ps + (first + t) % ps : 0;
+            }
+            if (row)
+                for (int j = 0; j * (int64_t)ps < kv_len[i]; ++j, ++e) {
+                    table[e] = row[j];
+                    entry[e] = make_int2(dense + j * ps, std::min(ps, kv_len[i] - j * ps));
+                }
+            dense += kv_len[i];
+        }
+    }
+    const bool f32 = b->dtype == GGR_DTYPE_F32, q8 = b->pages && b->pages->v.fmt == GGR_KV_Q8_HEAD;
+    const double tile_bytes = 16.0 * 2 * b->D * (q8 ? 1 : 2);
+    for (size_t l = 0; l < b->windows.size(); ++l) {
+        const int window = b->windows[l];
+        std::vector<Tile> tiles[kKinds];
+        for (int i = 0; i < n_seqs; ++i) {
+            const int first = kv_len[i] - q_len[i], n_rows = q_len[i] * b->G;
+            const int kind = !b->pages || n_rows > 64 ? kRows : kSplitK, step = kind == kRows ? 128 : 16;
+            for (int r = 0; r < n_rows; r += step) {
+                const int m = std::min(step, n_rows - r);
+                const int lo = first_key(first + r / b->G, window), hi = first + (r + m - 1) / b->G + 1;
+                tiles[kind].push_back({i, r, m, lo & ~15, hi});
+            }
+        }
+        int* counts = reinterpret_cast<int*>(h + b->at_counts) + l * kKinds * 4;
+        for (int k = 0; k < kKinds; ++k) {
+            PagedItem* items = reinterpret_cast<PagedItem*>(h + b->at_items[l][k]);
+            int n = 0, part = 0, ticket = 0, longest = 1;
+            const int piece = k == kSplitK && !tiles[k].empty()
+                                  ? choose_piece(tiles[k], b->Hkv, b->sm_count, tile_bytes, q8 || f32 ? 40e9 : 65e9, b->D == 256 ? 4 : 8, b->part_tiles, &longest)
+                                  : 1 << 27;
+            std::stable_sort(tiles[k].begin(), tiles[k].end(), [](const Tile& x, const Tile& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
+            for (const Tile& t : tiles[k]) {
+                const int n16 = (t.key1 - t.key0 + 15) / 16, cuts = std::max(1, (n16 + piece - 1) / piece), each = (n16 + cuts - 1) / cuts;
+                PagedItem it{};
+                it.tok0 = seqs[t.seq].tok0;
+                it.pos0 = kv_len[t.seq] - q_len[t.seq];
+                it.n_tok = q_len[t.seq];
+                it.row0 = t.row0;
+                it.rows = t.rows;
+                it.src = seqs[t.seq].src;
+                it.part = -1;
+                it.n_split = (n16 + each - 1) / each;
+                if (it.n_split > 1) {
+                    it.part = part;
+                    it.ticket = ticket++;
+                    part += it.n_split;
+                }
+                for (int s = 0; s < it.n_split; ++s) {
+                    it.split = s;
+                    it.key0 = t.key0 + s * each * 16;
+                    it.key1 = std::min(t.key1, it.key0 + each * 16);
+                    items[n++] = it;
+                }
+            }
+            counts[k * 4] = n;
+            counts[k * 4 + 1] = (int)entries;
+            counts[k * 4 + 2] = (int)tokens;
+            b->n_items[l][k] = n;
+        }
+    }
+    auto copy = [&](size_t at, size_t n) -> cudaError_t {
+        return n ? cudaMemcpyAsync(b->d_plan + at, h + at, n, cudaMemcpyHostToDevice, p.stream) : cudaSuccess;
+    };
+    PAGED_TRY(c, copy(b->at_counts, b->windows.size() * kKinds * 4 * sizeof(int)));
+    PAGED_TRY(c, copy(b->at_pos, tokens * sizeof(int)));
+    PAGED_TRY(c, copy(b->at_slot, tokens * sizeof(int)));
+    PAGED_TRY(c, copy(b->at_entries, entries * sizeof(int2)));
+    PAGED_TRY(c, copy(b->at_table, entries * sizeof(int)));
+    for (size_t l = 0; l < b->windows.size(); ++l)
+        for (int k = 0; k < kKinds; ++k) PAGED_TRY(c, copy(b->at_items[l][k], b->n_items[l][k] * sizeof(PagedItem)));
+    PAGED_TRY(c, cudaEventRecord(b->up[turn], p.stream));
+    b->up_used[turn] = true;
+    b->turn = turn ^ 1;
+    b->n_seqs = n_seqs;
+    b->n_tokens = (int)tokens;
+    b->n_entries = (int)entries;
+    b->n_rows = (int)rows;
+    b->set = true;
+    return GGR_OK;
+}
+
+namespace {
+
+int check_call(ggr_attn_ctx* c, ggr_batch* b, int layer, bool wants_pages) {
+    if (!b || b->ctx != c) return path_fail(c, GGR_ERR_INVALID, "the batch plan belongs to another context");
+    if (!b->set) return path_fail(c, GGR_ERR_INVALID, "the batch plan has not been set");
+    if (layer < 0 || layer >= b->n_layers) return path_fail(c, GGR_ERR_RANGE, "layer outside the cache");
+    if (wants_pages && !b->pages) return path_fail(c, GGR_ERR_INVALID, "the batch plan has no pages");
+    if (!wants_pages && b->pages) return path_fail(c, GGR_ERR_INVALID, "packed prompts need a batch plan without pages");
+    return GGR_OK;
+}
+
+// rows of `dim` elements at `stride`: vector loads and tensor maps need whole 16-byte pieces
+int check_rows(ggr_attn_ctx* c, const char* name, const void* x, int64_t* stride, int dim, int es) {
+    if (!x) return path_fail(c, GGR_ERR_INVALID, std::string("null ") + name);
+    if (*stride == 0) *stride = dim;
+    if (*stride < dim) return path_fail(c, GGR_ERR_INVALID, std::string(name) + ": rows overlap");
+    if ((uintptr_t)x % 16 || (*stride * es) % 16) return path_fail(c, GGR_ERR_INVALID, std::string(name) + ": rows must start on 16-byte boundaries");
+    if (*stride * es >= ((int64_t)1 << 39)) return path_fail(c, GGR_ERR_RANGE, std::string(name) + ": row stride out of range");
+    return GGR_OK;
+}
+
+template <int D, int FMT, bool F32>
+int launch_attention(ggr_attn_ctx* c, const PathView& p, const ggr_batch* b, int list, const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnArgs a, bool capturing) {
+    // a captured launch has to serve whatever plan its replays find: enough CTAs for any, items dealt in turn
+    const int most = (2 * b->sm_count + b->Hkv - 1) / b->Hkv;
+    for (int k = 0; k < kKinds; ++k) {
+        const int n = b->n_items[list][k];
+        if (!n && !capturing) continue;
+        a.plan.counts = b->counts(list, k);
+        a.plan.items = b->items(list, k);
+        const dim3 grid(capturing ? most : n, b->Hkv);
+        if (k == kSplitK) {
+            if constexpr (FMT == KV_F32) continue;
+            else {
+                using S = PagedSplitKShape<D, FMT, F32>;
+                static KernelSmemSetup setup;
+                PAGED_TRY(c, setup.ensure(paged_splitk_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
+                PathTimer t(c, 0);
+                paged_splitk_kernel<D, FMT, F32><<<grid, S::W * 32, S::SMEM, p.stream>>>(tk, tv, a);
+            }
+        } else {
+            using S = PagedRowsShape<D, FMT, F32>;
+            static KernelSmemSetup setup;
+            PAGED_TRY(c, setup.ensure(paged_rows_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
+            PathTimer t(c, 0);
+            paged_rows_kernel<D, FMT, F32><<<grid, 288, S::SMEM, p.stream>>>(tk, tv, a);
+        }
+        PAGED_TRY(c, cudaGetLastError());
+        path_launched(c);
+    }
+    return GGR_OK;
+}
+
+template <int FMT, bool F32>
+int launch_by_dim(ggr_attn_ctx* c, const PathView& p, const ggr_batch* b, int list, const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnArgs& a, bool cap) {
+    switch (b->D) {
+        case 64: return launch_attention<64, FMT, F32>(c, p, b, list, tk, tv, a, cap);
+        case 128: return launch_attention<128, FMT, F32>(c, p, b, list, tk, tv, a, cap);
+        default: return launch_attention<256, FMT, F32>(c, p, b, list, tk, tv, a, cap);
+    }
+}
+
+PagedAttnArgs attention_args(const PathView& p, const ggr_batch* b, int layer) {
+    PagedAttnArgs a{};
+    a.plan.table = b->table();
+    a.layer = layer;
+    a.Hq = b->Hq;
+    a.G = b->G;
+    a.window = b->windows[b->list_of[layer]];
+    a.c = p.score_scale * kLog2e;
+    a.part = b->d_part;
+    a.tickets = b->d_tickets;
+    a.err = p.d_err;
+    a.pages.Hkv = b->Hkv;
+    a.pages.D = b->D;
+    return a;
+}
+
+}  // namespace
+
+extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t rotate, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                const void* v, int64_t v_stride, void* q_out) {
+    if (!c) return GGR_ERR_INVALID;
+    int rc = check_call(c, b, layer, true);
+    if (rc) return rc;
+    const PathView p = path_view(c);
+    const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D, kv_dim = b->Hkv * b->D;
+    if ((rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v", v, &v_stride, kv_dim, es))) return rc;
+    if (!rotate && (q || q_out)) return path_fail(c, GGR_ERR_INVALID, "q is taken only to be rotated");
+    int64_t qo_stride = q_dim;
+    if (rotate) {
+        if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "q_out", q_out, &qo_stride, q_dim, es))) return rc;
+        if (p.position_plan) return path_fail(c, GGR_ERR_UNSUPPORTED, "a position plan belongs to one generation: batches rotate by cache position");
+        if (q == q_out && (p.rope_dim != b->D || q_stride != qo_stride))
+            return path_fail(c, GGR_ERR_INVALID, "q_out may be q itself only for dense rows whose heads are rotated as a whole");
+    }
+    Guard guard(p.device);
+    const bool capturing = path_capturing(c);
+    if (!b->n_tokens && !capturing) return GGR_OK;
+    int in_bf16 = b->dtype == GGR_DTYPE_BF16;
+    if (rotate && path_has_fixups(c, layer)) {
+        if (q_stride != q_dim || k_stride != kv_dim || v_stride != kv_dim) return path_fail(c, GGR_ERR_UNSUPPORTED, "bias and QK-norm need dense rows");
+        if (capturing) return path_fail(c, GGR_ERR_UNSUPPORTED, "bias and QK-norm of a batch are not captured: their scratch follows the batch");
+        if ((rc = path_fixups(c, layer, b->n_tokens, &q, &k, &v, &in_bf16))) return rc;
+    }
+    AppendArgs a{};
+    a.pages = b->pages->v;
+    a.rope = path_rope(c, layer);
+    a.counts = b->counts(0, 0);
+    a.tok_pos = reinterpret_cast<const int*>(b->d_plan + b->at_pos);
+    a.tok_slot = reinterpret_cast<const int*>(b->d_plan + b->at_slot);
+    a.layer = layer;
+    a.rotate = rotate != 0;
+    a.write_q = rotate != 0;
+    a.in_bf16 = in_bf16;
+    a.q_bf16 = b->dtype == GGR_DTYPE_BF16;
+    a.Hq = b->Hq;
+    a.heads = (rotate ? b->Hq : 0) + 2 * b->Hkv;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.qo_stride = qo_stride;
+    const int n = capturing ? b->max_tokens : b->n_tokens;
+    a.tokens_per_cta = std::min(4, std::max(1, n / (8 * b->sm_count)));
+    const int grid = (n + a.tokens_per_cta - 1) / a.tokens_per_cta;
+    const size_t smem = rotate ? (size_t)2 * a.tokens_per_cta * a.rope.rope_half * sizeof(float) : 0;
+    {
+        PathTimer t(c, 1);
+        if (in_bf16)
+            paged_append_kernel<true><<<grid, 256, smem, p.stream>>>(a);
+        else
+            paged_append_kernel<false><<<grid, 256, smem, p.stream>>>(a);
+    }
+    PAGED_TRY(c, cudaGetLastError());
+    path_launched(c);
+    return GGR_OK;
+}
+
+namespace {
+
+template <int FMT, int D>
+void launch_read(const ReadArgs& a, bool bf16, int grid, cudaStream_t stream) {
+    if (bf16)
+        paged_read_kernel<FMT, D, true><<<grid, 256, 0, stream>>>(a);
+    else
+        paged_read_kernel<FMT, D, false><<<grid, 256, 0, stream>>>(a);
+}
+
+}  // namespace
+
+extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride) {
+    if (!c) return GGR_ERR_INVALID;
+    int rc = check_call(c, b, layer, true);
+    if (rc) return rc;
+    if (out_dtype != GGR_DTYPE_F32 && out_dtype != GGR_DTYPE_BF16) return path_fail(c, GGR_ERR_INVALID, "unknown dtype");
+    const int kv_dim = b->Hkv * b->D, es = elem_bytes(out_dtype);
+    if ((rc = check_rows(c, "k_out", k_out, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v_out", v_out, &v_stride, kv_dim, es))) return rc;
+    const PathView p = path_view(c);
+    Guard guard(p.device);
+    const bool capturing = path_capturing(c);
+    if (!b->n_entries && !capturing) return GGR_OK;
+    ReadArgs a{};
+    a.pages = b->pages->v;
+    a.counts = b->counts(0, 0);
+    a.table = b->table();
+    a.entries = reinterpret_cast<const int2*>(b->d_plan + b->at_entries);
+    a.layer = layer;
+    a.k_out = k_out;
+    a.v_out = v_out;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    const int64_t blocks = (int64_t)(capturing ? b->max_pages : b->n_entries) * (b->pages->page_size / 16) * b->Hkv;
+    const int grid = (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)8 * b->sm_count);
+    const bool bf16 = out_dtype == GGR_DTYPE_BF16;
+    {
+        PathTimer t(c, 1);
+        if (b->pages->v.fmt == GGR_KV_BF16) {
+            switch (b->D) {
+                case 64: launch_read<KV_BF16, 64>(a, bf16, grid, p.stream); break;
+                case 128: launch_read<KV_BF16, 128>(a, bf16, grid, p.stream); break;
+                default: launch_read<KV_BF16, 256>(a, bf16, grid, p.stream);
+            }
+        } else {
+            switch (b->D) {
+                case 64: launch_read<kKvQ8Head, 64>(a, bf16, grid, p.stream); break;
+                case 128: launch_read<kKvQ8Head, 128>(a, bf16, grid, p.stream); break;
+                default: launch_read<kKvQ8Head, 256>(a, bf16, grid, p.stream);
+            }
+        }
+    }
+    PAGED_TRY(c, cudaGetLastError());
+    path_launched(c);
+    return GGR_OK;
+}
+
+extern "C" int ggr_paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, void* out, int64_t out_stride) {
+    if (!c) return GGR_ERR_INVALID;
+    int rc = check_call(c, b, layer, true);
+    if (rc) return rc;
+    const PathView p = path_view(c);
+    const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D;
+    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es))) return rc;
+    if (p.image_blocks) return path_fail(c, GGR_ERR_UNSUPPORTED, "bidirectional blocks belong to one generation: batches attend causally");
+    Guard guard(p.device);
+    const bool capturing = path_capturing(c);
+    if (!b->n_tokens && !capturing) return GGR_OK;
+    PagedAttnArgs a = attention_args(p, b, layer);
+    a.paged = 1;
+    a.pages = b->pages->v;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.o_stride = out_stride;
+    const int list = b->list_of[layer];
+    const CUtensorMap &tk = b->pages->tmK16, &tv = b->pages->tmV16;
+    const bool f32 = b->dtype == GGR_DTYPE_F32;
+    if (b->pages->v.fmt == GGR_KV_BF16)
+        return f32 ? launch_by_dim<KV_BF16, true>(c, p, b, list, tk, tv, a, capturing) : launch_by_dim<KV_BF16, false>(c, p, b, list, tk, tv, a, capturing);
+    return f32 ? launch_by_dim<kKvQ8Head, true>(c, p, b, list, tk, tv, a, capturing) : launch_by_dim<kKvQ8Head, false>(c, p, b, list, tk, tv, a, capturing);
+}
+
+extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                    int64_t v_stride, void* out, int64_t out_stride) {
+    if (!c) return GGR_ERR_INVALID;
+    int rc = check_call(c, b, layer, false);
+    if (rc) return rc;
+    const PathView p = path_view(c);
+    const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D, kv_dim = b->Hkv * b->D;
+    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) ||
+        (rc = check_rows(c, "v", v, &v_stride, kv_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es)))
+        return rc;
+    if (p.image_blocks) return path_fail(c, GGR_ERR_UNSUPPORTED, "bidirectional blocks belong to one generation: batches attend causally");
+    Guard guard(p.device);
+    const bool capturing = path_capturing(c);
+    if (!b->n_tokens && !capturing) return GGR_OK;
+    const int rows = capturing ? b->max_tokens : b->n_tokens;
+    const bool f32 = b->dtype == GGR_DTYPE_F32;
+    PagedAttnArgs a = attention_args(p, b, layer);
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.o_stride = out_stride;
+    a.pk = k;
+    a.pv = v;
+    a.pk_stride = k_stride;
+    a.pv_stride = v_stride;
+    CUtensorMap tk, tv;
+    const int list = b->list_of[layer];
+    if (f32) {
+        const int64_t plane = (int64_t)b->max_tokens * kv_dim;
+        __nv_bfloat16 *kp = b->d_planes, *vp = b->d_planes + 2 * plane;
+        a.plane_rows = b->max_tokens;
+        const uint64_t sy = (uint64_t)b->D * 2, sz = (uint64_t)kv_dim * 2;
+        if (!make_map3(&tk, false, kp, b->D, b->Hkv, (uint64_t)2 * b->max_tokens, sy, sz, 64, 1, 16) ||
+            !make_map3(&tv, false, vp, b->D, b->Hkv, (uint64_t)2 * b->max_tokens, sy, sz, 64, 1, 16))
+            return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
+        {
+            PathTimer t(c, 1);
+            paged_planes_kernel<<<dim3((unsigned)(((int64_t)rows * kv_dim / 4 + 255) / 256), 2), 256, 0, p.stream>>>(
+                static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, rows, kv_dim, kp, vp, plane);
+        }
+        PAGED_TRY(c, cudaGetLastError());
+        path_launched(c);
+        return launch_by_dim<KV_F32, true>(c, p, b, list, tk, tv, a, capturing);
+    }
+    if (!make_map3(&tk, false, k, b->D, b->Hkv, rows, (uint64_t)b->D * 2, (uint64_t)k_stride * 2, 64, 1, 16) ||
+        !make_map3(&tv, false, v, b->D, b->Hkv, rows, (uint64_t)b->D * 2, (uint64_t)v_stride * 2, 64, 1, 16))
+        return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
+    return launch_by_dim<KV_BF16, false>(c, p, b, list, tk, tv, a, capturing);
+}

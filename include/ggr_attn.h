@@ -47,6 +47,8 @@ enum { GGR_DTYPE_F32 = 0, GGR_DTYPE_BF16 = 1 };
  * 2-bit codes of the rotated head plus one sign bit of the projected residual per element, sigma and residual
  * norm per (row, kv head); head_dim 64, 128 or 256 */
 enum { GGR_KV_F32 = 0, GGR_KV_BF16 = 1, GGR_KV_Q8_ROW = 2, GGR_KV_Q8_BLOCK32 = 3, GGR_KV_TURBO = 4 };
+/* pages only (ggr_pages_create): int8 codes with one f32 scale per (position, KV head) */
+enum { GGR_KV_Q8_HEAD = 5 };
 enum { GGR_ROPE_NEOX = 0, GGR_ROPE_ADJACENT = 1 };
 enum { GGR_ROPE_SEQUENTIAL = 0, GGR_ROPE_INTERLEAVED = 1 };
 enum { GGR_SCALE_SCORE = 0, GGR_SCALE_Q_PRESCALED = 1 };
@@ -370,6 +372,82 @@ int ggr_attn_layer_decode(ggr_attn_ctx* ctx, int32_t layer, const int32_t* pos, 
 int ggr_attn_layer_prefill(ggr_attn_ctx* ctx, int32_t layer, int32_t seq, int32_t base_pos, int32_t m, const float* xb,
                            const ggr_weights* wq, const ggr_weights* wk, const ggr_weights* wv, const ggr_weights* wo,
                            float* xb2, int32_t ptr_kind);
+
+/*
+ * Batches over a paged cache, and packed prompts (no counterpart in the reference, which holds one sequence per RunState): for
+ * hosts that serve many conversations from one pool of cache pages. A step brings new tokens of several sequences, single
+ * tokens and chunks of prompts alike; the rows of all of them lie behind each other, sequence after sequence.
+ *
+ *   ggr_batch_set        lengths and page table of the step, once for all layers
+ *   per layer: ggr_paged_append (RoPE, rows into their pages), ggr_paged_attention
+ *
+ * The context gives the shape, the RoPE and scale settings, the layer windows, the stream and the error text; its own dense
+ * cache is not touched (seq_len 1 keeps it small). head_dim 64, 128 or 256, any number of query heads per KV head. Rows are
+ * device memory in the plan's dtype (GGR_DTYPE_BF16: tensor-core arithmetic of bf16 operands; GGR_DTYPE_F32: 32-bit
+ * precision), 16-byte aligned, with a row stride in elements (0 = dense; a multiple of 16 bytes), so that q, k and v may be
+ * slices of one projection. Outputs have the same dtype. Calls only enqueue work on the context's stream.
+ */
+typedef struct ggr_pages ggr_pages;
+typedef struct ggr_batch ggr_batch;
+/*
+ * A pool of n_pages pages of page_size (16, 32, 64, 128 or 256) positions for every layer: K and V arrays
+ * [layer][page][KV head][position][head_dim] in GGR_KV_BF16 or GGR_KV_Q8_HEAD, and for the latter the scales
+ * [layer][page][KV head][position]. A head with m = max |x| is stored as codes round(x * (127 / m)) (half away from zero) and
+ * scale m / 127, every step in f32; m below 1e-36 as zeros with scale 1; a head with a value that is not finite reads back as
+ * NaN. k, v, k_scale, v_scale: device arrays of the caller's (128-byte aligned, kept until the pool is destroyed), or all
+ * null, in which case the library allocates and clears them. A page id names the same page in every layer.
+ */
+int ggr_pages_create(ggr_attn_ctx* ctx, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v,
+                     float* k_scale, float* v_scale, ggr_pages** out);
+/* After the batch plans that use the pool. */
+void ggr_pages_destroy(ggr_pages* pages);
+int ggr_pages_device_ptrs(const ggr_pages* pages, void** k, void** v, float** k_scale, float** v_scale,
+                          uint64_t* array_bytes);
+/*
+ * A batch plan with room for max_seqs sequences, max_tokens new tokens and max_pages page table entries in all. pages null:
+ * a plan for ggr_packed_attention (max_pages 0). A plan owns the scratch of its launches: launches of one plan have to be
+ * ordered (one stream, or events between), different plans are independent. Destroy a plan before its context; work that
+ * uses it is waited for.
+ */
+int ggr_batch_create(ggr_attn_ctx* ctx, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens,
+                     int32_t max_pages, ggr_batch** out);
+void ggr_batch_destroy(ggr_batch* batch);
+/*
+ * The step: sequence i has q_len[i] new tokens (0 is allowed), the last of its kv_len[i] tokens; entry j of row i of
+ * page_table (host, n_seqs rows of table_stride entries) is the page of its positions [j * page_size, (j + 1) * page_size),
+ * j < ceil(kv_len / page_size); entries behind that are not read. Pages may be shared between sequences (a common prefix),
+ * but a page that receives new rows receives them from one sequence (else GGR_ERR_INVALID). A plan without pages has kv_len =
+ * q_len and no table. A layer with a window w sees the last w positions, the current one included; pages before that may be
+ * reused: their entries only have to name a page. The call copies its arrays and enqueues one upload; it does not belong into a
+ * stream capture, but captured launches of the plan follow it when they are replayed behind it.
+ */
+int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
+                  int32_t table_stride);
+/*
+ * Stores the new tokens' rows of k and v in their pages. rotate: RoPE by cache position on q and k first (and the layer's
+ * bias / QK-norm fixups, dense rows only, before that), rotated (and, in GGR_SCALE_Q_PRESCALED mode, scaled) q to q_out
+ * [tokens][q_dim], which may be q itself when heads are rotated as a whole. rotate 0: k is stored as it is, q and q_out are
+ * null.
+ */
+int ggr_paged_append(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t rotate, const void* q, int64_t q_stride,
+                     const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out);
+/* All kv_len rows of all sequences, sequence after sequence, dequantised into k_out and v_out [rows][kv_dim] (out_dtype, row
+ * strides in elements). */
+int ggr_paged_read(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride,
+                   void* v_out, int64_t v_stride);
+/*
+ * out[t] = attention of new token t (rotated q) over the visible cached rows of its sequence, its own and those of the
+ * chunk's tokens before it included. What a token does not see (later tokens, other sequences, rows that were never written)
+ * does not touch its result, whatever it holds.
+ */
+int ggr_paged_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, void* out,
+                        int64_t out_stride);
+/*
+ * Causal attention of whole prompts straight from their rotated q, k and v rows, no cache involved. A captured launch has to
+ * be given buffers of max_tokens rows: replays may find a longer plan.
+ */
+int ggr_packed_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride);
 
 /* Number of kernels this context has launched since it was created. */
 int64_t ggr_attn_launch_count(const ggr_attn_ctx* ctx);

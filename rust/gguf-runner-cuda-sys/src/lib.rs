@@ -99,6 +99,18 @@ pub struct GgrWeights {
     _private: [u8; 0],
 }
 
+#[repr(C)]
+pub struct GgrPages {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct GgrBatch {
+    _private: [u8; 0],
+}
+
+pub const GGR_KV_Q8_HEAD: i32 = 5;
+
 pub const GGR_W_F32: i32 = 0;
 pub const GGR_W_BF16: i32 = 1;
 pub const GGR_W_Q8_0: i32 = 2;
@@ -174,6 +186,24 @@ extern "C" {
     pub fn ggr_weights_upload(device: i32, wtype: i32, rows: i32, cols: i32, host_data: *const c_void,
         out: *mut *mut GgrWeights) -> i32;
     pub fn ggr_weights_free(w: *mut GgrWeights);
+    pub fn ggr_pages_create(ctx: *mut GgrAttnCtx, n_pages: i32, page_size: i32, kv_format: i32, k: *mut c_void,
+        v: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, out: *mut *mut GgrPages) -> i32;
+    pub fn ggr_pages_destroy(pages: *mut GgrPages);
+    pub fn ggr_pages_device_ptrs(pages: *const GgrPages, k: *mut *mut c_void, v: *mut *mut c_void,
+        k_scale: *mut *mut f32, v_scale: *mut *mut f32, array_bytes: *mut u64) -> i32;
+    pub fn ggr_batch_create(ctx: *mut GgrAttnCtx, pages: *mut GgrPages, dtype: i32, max_seqs: i32, max_tokens: i32,
+        max_pages: i32, out: *mut *mut GgrBatch) -> i32;
+    pub fn ggr_batch_destroy(batch: *mut GgrBatch);
+    pub fn ggr_batch_set(batch: *mut GgrBatch, n_seqs: i32, q_len: *const i32, kv_len: *const i32,
+        page_table: *const i32, table_stride: i32) -> i32;
+    pub fn ggr_paged_append(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, rotate: i32, q: *const c_void,
+        q_stride: i64, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, q_out: *mut c_void) -> i32;
+    pub fn ggr_paged_read(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, out_dtype: i32, k_out: *mut c_void,
+        k_stride: i64, v_out: *mut c_void, v_stride: i64) -> i32;
+    pub fn ggr_paged_attention(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, q: *const c_void, q_stride: i64,
+        out: *mut c_void, out_stride: i64) -> i32;
+    pub fn ggr_packed_attention(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, q: *const c_void, q_stride: i64,
+        k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, out: *mut c_void, out_stride: i64) -> i32;
     pub fn ggr_proj_matmul(ctx: *mut GgrAttnCtx, w: *const GgrWeights, x: *const f32, n: i32, xout: *mut f32,
         ptr_kind: i32) -> i32;
     pub fn ggr_attn_layer_decode(ctx: *mut GgrAttnCtx, layer: i32, pos: *const i32, b: i32, xb: *const f32,
