@@ -788,7 +788,10 @@ class AttnContext:
 
     def paged_attention(self, batch: Batch, layer: int, q, out=None):
         """Attention of the batch's new tokens (rotated q) over their sequences' pages."""
+        import torch
         c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
+        if torch.cuda.is_current_stream_capturing():
+            n = batch.max_tokens  # replays may find a longer plan
         out = self._row_out(out, q, n, c.q_dim, dt)
         qp, qs = self._rows("q", q, dt, n, c.q_dim)
         op, os_ = self._rows("out", out, dt, n, c.q_dim)

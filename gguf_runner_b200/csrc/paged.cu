@@ -18,6 +18,7 @@
 #include "../../include/ggr_attn.h"
 #include "paged.cuh"
 #include "paged_mma.cuh"
+#include "paged_tc.cuh"
 #include "path_view.h"
 
 using namespace ggr;
@@ -29,13 +30,18 @@ struct ggr_pages {
     int device, n_layers, page_size;
     PageView v{};
     void* owned[4] = {nullptr, nullptr, nullptr, nullptr};
-    CUtensorMap tmK16, tmV16;  // 16 rows of a page, one 64- or 128-byte block of columns
+    CUtensorMap tmK16, tmV16;    // 16 rows of a page, one 64- or 128-byte block of columns
+    CUtensorMap tmK128, tmV128;  // bf16: min(page_size, 128) rows
 };
 
 namespace {
 
+// Packed rows (new tokens times query heads of a KV head) of a sequence above which it goes to the tcgen05 kernel, and above
+// which (32-bit precision, head_dim 256) to the kernel whose warps share the keys.
+constexpr int kTcMinRows = 64, kRowsMinRows = 64;
 constexpr int kMaxLists = 4;  // distinct windows of a model's layers
-enum Kind { kSplitK = 0, kRows = 1, kKinds = 2 };
+// lists of a plan: items of the three attention kernels, and the pairs of query tiles whose pieces are merged
+enum Kind { kSplitK = 0, kRows = 1, kTc = 2, kMerge = 3, kKinds = 4 };
 
 struct Guard {
     int prev = -1;
@@ -83,6 +89,19 @@ struct ggr_batch {
     std::vector<int> windows;   // list -> window
     size_t item_cap[kKinds] = {};
     size_t part_tiles = 0;      // partial states (of 16 rows, per KV head) that the scratch holds
+    bool tc = false;            // the tcgen05 kernel takes this shape and dtype
+    int tc_tokens = 0;          // tokens of one of its query tiles
+    size_t tc_parts = 0;        // its partial states
+    float* d_tc_part = nullptr;
+    int* d_sched = nullptr;
+    // 8-bit pages on their way to the tcgen05 kernel: dense bf16 rows, and which pages go there
+    __nv_bfloat16* d_dense = nullptr;
+    float* d_dense_scales = nullptr;
+    size_t dense_rows = 0;
+    CUtensorMap tmKd, tmVd;
+    size_t at_dense_entries = 0, at_dense_table = 0;
+    int n_dense = 0;
+    unsigned captured = 0;       // kinds of kernels that captured launches of this plan hold
     // device image of the plan: fixed places, so that captured launches keep their pointers
     unsigned char* d_plan = nullptr;
     unsigned char* h_plan[2] = {nullptr, nullptr};
@@ -102,6 +121,7 @@ struct ggr_batch {
     int stamp = 0;
 
     const int* counts(int list, int kind) const { return reinterpret_cast<const int*>(d_plan + at_counts) + (list * kKinds + kind) * 4; }
+    const int* dense_counts() const { return reinterpret_cast<const int*>(d_plan + at_counts) + windows.size() * kKinds * 4; }
     const int* table() const { return reinterpret_cast<const int*>(d_plan + at_table); }
     const PagedItem* items(int list, int kind) const { return reinterpret_cast<const PagedItem*>(d_plan + at_items[list][kind]); }
 };
@@ -164,6 +184,38 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
         consider(lo);
         if (lo <= min_tiles) break;
     }
+    return best;
+}
+
+// The same for the tcgen05 kernel, in 128-key tiles of a pair of query tiles: `tiles` of every pair, of all KV heads. A step over
+// a tile takes 0.75 us, an item 3 us besides (its start, its epilogue), and cutting at all costs the merge.
+int choose_tc_piece(const std::vector<int>& tiles, int sm_count, size_t max_pieces) {
+    int64_t total = 0;
+    int longest = 1;
+    for (int n : tiles) {
+        total += n;
+        longest = std::max(longest, n);
+    }
+    int best = longest;
+    double best_cost = -1.0;
+    auto consider = [&](int piece) {
+        int64_t items = 0, cut = 0;
+        for (int n : tiles) {
+            const int k = (n + piece - 1) / piece;
+            items += k;
+            if (k > 1) cut += k;
+        }
+        if ((size_t)cut > max_pieces) return;
+        const double t0 = 3.0, t = 0.75, one = t0 + piece * t;
+        double cost = items <= sm_count ? one : std::max(one, (total * t + items * t0) / sm_count + 0.5 * one);
+        if (cut) cost += 4.0;
+        if (best_cost < 0.0 || cost < best_cost) {
+            best_cost = cost;
+            best = piece;
+        }
+    };
+    consider(longest);
+    for (int k = 2; k <= 32 && longest / k >= 3; ++k) consider((longest + k - 1) / k);
     return best;
 }
 
@@ -231,6 +283,13 @@ extern "C" int ggr_pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_s
             for (void* x : pg->owned) cudaFree(x);
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pool");
         }
+    if (!q8 && p.D <= 128)
+        for (int i = 0; i < 2; ++i)
+            if (!make_map3(i ? &pg->tmV128 : &pg->tmK128, false, i ? view.v : view.k, p.D, page_size, groups, row_bytes, row_bytes * page_size, 64,
+                           std::min(page_size, 128), 1)) {
+                for (void* x : pg->owned) cudaFree(x);
+                return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pool");
+            }
     *out = pg.release();
     return GGR_OK;
 }
@@ -265,6 +324,10 @@ extern "C" void ggr_batch_destroy(ggr_batch* b) {
     cudaFree(b->d_part);
     cudaFree(b->d_tickets);
     cudaFree(b->d_planes);
+    cudaFree(b->d_tc_part);
+    cudaFree(b->d_sched);
+    cudaFree(b->d_dense);
+    cudaFree(b->d_dense_scales);
     delete b;
 }
 
@@ -309,17 +372,29 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     b->part_tiles = (size_t)(8 * p.sm_count + p.Hkv - 1) / p.Hkv + 16;
     b->item_cap[kSplitK] = (rows + 15) / 16 + max_seqs + b->part_tiles;
     b->item_cap[kRows] = (rows + 127) / 128 + max_seqs;
+    b->tc = dtype == GGR_DTYPE_BF16 && p.D <= 128 && p.G <= 128;
+    if (b->tc) {
+        b->tc_tokens = 128 / p.G;
+        const size_t pairs = (((size_t)max_tokens + 2 * b->tc_tokens - 1) / (2 * b->tc_tokens) + max_seqs) * p.Hkv;
+        b->tc_parts = 2 * (size_t)p.sm_count;
+        b->item_cap[kTc] = pairs + b->tc_parts;
+        b->item_cap[kMerge] = b->tc_parts;
+    }
     size_t at = 0;
     auto place = [&](size_t n) {
         const size_t here = at;
         at = (at + n + 255) / 256 * 256;
         return here;
     };
-    b->at_counts = place(lists * kKinds * 4 * sizeof(int));
+    b->at_counts = place((lists * kKinds + 1) * 4 * sizeof(int));
     b->at_pos = place((size_t)max_tokens * sizeof(int));
     b->at_slot = place((size_t)max_tokens * sizeof(int));
     b->at_entries = place((size_t)max_pages * sizeof(int2));
     b->at_table = place((size_t)max_pages * sizeof(int));
+    if (b->tc && pages && pages->v.fmt == GGR_KV_Q8_HEAD) {
+        b->at_dense_entries = place((size_t)max_pages * sizeof(int2));
+        b->at_dense_table = place((size_t)max_pages * sizeof(int));
+    }
     for (size_t l = 0; l < lists; ++l)
         for (int k = 0; k < kKinds; ++k) b->at_items[l][k] = place(b->item_cap[k] * sizeof(PagedItem));
     b->bytes = at;
@@ -328,6 +403,9 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
               cudaMalloc((void**)&b->d_tickets, b->part_tiles * p.Hkv * sizeof(unsigned)) == cudaSuccess;
     if (ok && !pages && dtype == GGR_DTYPE_F32)
         ok = cudaMalloc((void**)&b->d_planes, (size_t)4 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
+    if (ok && b->tc)
+        ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 256 * (p.D + 2) * sizeof(float)) == cudaSuccess &&
+             cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
     for (int i = 0; ok && i < 2; ++i)
         ok = cudaHostAlloc((void**)&b->h_plan[i], b->bytes, cudaHostAllocDefault) == cudaSuccess &&
              cudaEventCreateWithFlags(&b->up[i], cudaEventDisableTiming) == cudaSuccess;
@@ -336,7 +414,8 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
         return path_fail(c, GGR_ERR_ALLOC, "unable to allocate the batch plan");
     }
     if (cudaMemsetAsync(b->d_plan, 0, b->bytes, p.stream) != cudaSuccess ||
-        cudaMemsetAsync(b->d_tickets, 0, b->part_tiles * p.Hkv * sizeof(unsigned), p.stream) != cudaSuccess)
+        cudaMemsetAsync(b->d_tickets, 0, b->part_tiles * p.Hkv * sizeof(unsigned), p.stream) != cudaSuccess ||
+        (b->tc && cudaMemsetAsync(b->d_sched, 0, 2 * sizeof(int), p.stream) != cudaSuccess))
         return path_fail(c, GGR_ERR_CUDA, "unable to clear the batch plan");
     if (pages) b->page_owner.assign(pages->v.n_pages, 0);
     *out = b.release();
@@ -420,21 +499,93 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
         }
     }
     const bool f32 = b->dtype == GGR_DTYPE_F32, q8 = b->pages && b->pages->v.fmt == GGR_KV_Q8_HEAD;
+    // kernel of every sequence; captured launches hold certain kernels, and a plan that has any keeps to those
+    std::vector<int> kind(n_seqs, kSplitK), lin(n_seqs, 0);
+    auto allowed = [&](int k) { return !b->captured || (b->captured >> k & 1); };
+    int64_t dense = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        const int64_t n_rows = (int64_t)q_len[i] * b->G;
+        int k = b->tc && n_rows > kTcMinRows ? kTc : (!b->pages || n_rows > kRowsMinRows ? kRows : kSplitK);
+        if (!b->pages && f32) k = kRows;
+        if (!allowed(k)) k = allowed(kRows) ? kRows : (allowed(kSplitK) ? kSplitK : kTc);
+        kind[i] = k;
+        if (k == kTc && q8 && q_len[i] > 0) {
+            lin[i] = (int)dense;
+            dense += ((int64_t)kv_len[i] + ps - 1) / ps * ps;
+        } else if (k == kTc && !b->pages) {
+            lin[i] = seqs[i].tok0;
+        }
+    }
+    if (dense > (int64_t)b->dense_rows) {
+        if (!b->captured || !b->d_dense) {
+            const size_t row = (size_t)b->Hkv * b->D;
+            if (b->d_dense) {
+                PAGED_TRY(c, cudaStreamSynchronize(p.stream));
+                cudaFree(b->d_dense);
+                cudaFree(b->d_dense_scales);
+            }
+            b->d_dense = nullptr;
+            b->d_dense_scales = nullptr;
+            b->dense_rows = 0;
+            const size_t want = (size_t)std::max<int64_t>(dense, 4096);
+            if (want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__nv_bfloat16)) == cudaSuccess &&
+                cudaMalloc((void**)&b->d_dense_scales, 2 * (want + 128) * b->Hkv * sizeof(float)) == cudaSuccess) {
+                if (!make_map3(&b->tmKd, false, b->d_dense, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128) ||
+                    !make_map3(&b->tmVd, false, b->d_dense + want * row, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128))
+                    return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the dequantised rows");
+                b->dense_rows = want;
+            } else {
+                cudaGetLastError();
+                cudaFree(b->d_dense);
+                b->d_dense = nullptr;
+            }
+        }
+        // where the rows do not fit (no memory, or captured launches hold the smaller buffer) the warp-level kernel reads the pages
+        if (dense > (int64_t)b->dense_rows)
+            for (int i = 0; i < n_seqs; ++i)
+                if (kind[i] == kTc) {
+                    if (!allowed(kRows) && !allowed(kSplitK)) return path_fail(c, GGR_ERR_RANGE, "the captured launches of this plan hold less room for dequantised pages");
+                    kind[i] = allowed(kRows) ? kRows : kSplitK;
+                }
+    }
+    int n_dense = 0;
+    if (q8 && b->tc) {
+        int2* de = reinterpret_cast<int2*>(h + b->at_dense_entries);
+        int* dt = reinterpret_cast<int*>(h + b->at_dense_table);
+        const int widest = *std::min_element(b->windows.begin(), b->windows.end()) == 0 ? 0 : *std::max_element(b->windows.begin(), b->windows.end());
+        for (int i = 0; i < n_seqs; ++i) {
+            if (kind[i] != kTc || q_len[i] == 0) continue;
+            for (int j = first_key(kv_len[i] - q_len[i], widest) / ps; j * (int64_t)ps < kv_len[i]; ++j, ++n_dense) {
+                dt[n_dense] = table[seqs[i].src + j];
+                de[n_dense] = make_int2(lin[i] + j * ps, std::min(ps, kv_len[i] - j * ps));
+            }
+        }
+        reinterpret_cast<int*>(h + b->at_counts)[b->windows.size() * kKinds * 4 + 1] = n_dense;
+    }
     const double tile_bytes = 16.0 * 2 * b->D * (q8 ? 1 : 2);
     for (size_t l = 0; l < b->windows.size(); ++l) {
         const int window = b->windows[l];
         std::vector<Tile> tiles[kKinds];
+        std::vector<int> pair_tiles;
         for (int i = 0; i < n_seqs; ++i) {
             const int first = kv_len[i] - q_len[i], n_rows = q_len[i] * b->G;
-            const int kind = !b->pages || n_rows > 64 ? kRows : kSplitK, step = kind == kRows ? 128 : 16;
+            if (kind[i] == kTc) {
+                for (int t = 0; t < q_len[i]; t += 2 * b->tc_tokens) {
+                    const int lo = first_key(first + t, window) & ~127, hi = std::min(first + t + 2 * b->tc_tokens, kv_len[i]);
+                    tiles[kTc].push_back({i, t, 0, lo, hi});
+                    for (int k = 0; k < b->Hkv; ++k) pair_tiles.push_back((hi - lo + 127) / 128);
+                }
+                continue;
+            }
+            const int step = kind[i] == kRows ? 128 : 16;
             for (int r = 0; r < n_rows; r += step) {
                 const int m = std::min(step, n_rows - r);
                 const int lo = first_key(first + r / b->G, window), hi = first + (r + m - 1) / b->G + 1;
-                tiles[kind].push_back({i, r, m, lo & ~15, hi});
+                tiles[kind[i]].push_back({i, r, m, lo & ~15, hi});
             }
         }
         int* counts = reinterpret_cast<int*>(h + b->at_counts) + l * kKinds * 4;
-        for (int k = 0; k < kKinds; ++k) {
+        for (int k = 0; k < kTc; ++k) {
             PagedItem* items = reinterpret_cast<PagedItem*>(h + b->at_items[l][k]);
             int n = 0, part = 0, ticket = 0, longest = 1;
             const int piece = k == kSplitK && !tiles[k].empty()
@@ -465,15 +616,55 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
                 }
             }
             counts[k * 4] = n;
+            b->n_items[l][k] = n;
+        }
+        {
+            PagedItem* merge = reinterpret_cast<PagedItem*>(h + b->at_items[l][kMerge]);
+            const int piece = pair_tiles.empty() ? 1 : choose_tc_piece(pair_tiles, b->sm_count, b->tc_parts);
+            int n = 0, n_merge = 0, part = 0;
+            b->scratch.clear();
+            for (const Tile& t : tiles[kTc]) {
+                const int nt = (t.key1 - t.key0 + 127) / 128, cuts = std::max(1, (nt + piece - 1) / piece), each = (nt + cuts - 1) / cuts;
+                PagedItem it{};
+                it.tok0 = seqs[t.seq].tok0;
+                it.pos0 = kv_len[t.seq] - q_len[t.seq];
+                it.n_tok = q_len[t.seq];
+                it.row0 = t.row0;
+                it.src = seqs[t.seq].src;
+                it.lin = lin[t.seq];
+                it.n_split = (nt + each - 1) / each;
+                for (it.kvh = 0; it.kvh < b->Hkv; ++it.kvh) {
+                    it.part = -1;
+                    if (it.n_split > 1) {
+                        it.part = part;
+                        part += it.n_split;
+                    }
+                    for (int s = 0; s < it.n_split; ++s) {
+                        it.split = s;
+                        it.key0 = t.key0 + s * each * 128;
+                        it.key1 = std::min(t.key1, it.key0 + each * 128);
+                        b->scratch.push_back(it);
+                        if (s == 0 && it.n_split > 1) merge[n_merge++] = it;
+                    }
+                }
+            }
+            std::stable_sort(b->scratch.begin(), b->scratch.end(), [](const PagedItem& x, const PagedItem& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
+            n = (int)b->scratch.size();
+            if (n) memcpy(h + b->at_items[l][kTc], b->scratch.data(), n * sizeof(PagedItem));
+            counts[kTc * 4] = b->n_items[l][kTc] = n;
+            counts[kMerge * 4] = b->n_items[l][kMerge] = n_merge;
+        }
+        for (int k = 0; k < kKinds; ++k) {
             counts[k * 4 + 1] = (int)entries;
             counts[k * 4 + 2] = (int)tokens;
-            b->n_items[l][k] = n;
         }
     }
     auto copy = [&](size_t at, size_t n) -> cudaError_t {
         return n ? cudaMemcpyAsync(b->d_plan + at, h + at, n, cudaMemcpyHostToDevice, p.stream) : cudaSuccess;
     };
-    PAGED_TRY(c, copy(b->at_counts, b->windows.size() * kKinds * 4 * sizeof(int)));
+    PAGED_TRY(c, copy(b->at_counts, (b->windows.size() * kKinds + 1) * 4 * sizeof(int)));
+    PAGED_TRY(c, copy(b->at_dense_entries, n_dense * sizeof(int2)));
+    PAGED_TRY(c, copy(b->at_dense_table, n_dense * sizeof(int)));
     PAGED_TRY(c, copy(b->at_pos, tokens * sizeof(int)));
     PAGED_TRY(c, copy(b->at_slot, tokens * sizeof(int)));
     PAGED_TRY(c, copy(b->at_entries, entries * sizeof(int2)));
@@ -487,6 +678,7 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
     b->n_tokens = (int)tokens;
     b->n_entries = (int)entries;
     b->n_rows = (int)rows;
+    b->n_dense = n_dense;
     b->set = true;
     return GGR_OK;
 }
@@ -512,13 +704,94 @@ int check_rows(ggr_attn_ctx* c, const char* name, const void* x, int64_t* stride
     return GGR_OK;
 }
 
+// Tensor maps of a launch: 16-row tiles for the warp-level kernels, 128-row tiles and query tiles for the tcgen05 kernel.
+struct Maps {
+    const CUtensorMap *k16, *v16, *k128, *v128;
+};
+
+template <int FMT, int D>
+void launch_read(const ReadArgs& a, bool bf16, int grid, cudaStream_t stream) {
+    if (bf16)
+        paged_read_kernel<FMT, D, kReadBf16><<<grid, 256, 0, stream>>>(a);
+    else
+        paged_read_kernel<FMT, D, kReadF32><<<grid, 256, 0, stream>>>(a);
+}
+
+int read_grid(const ggr_batch* b, int64_t entries) {
+    const int64_t blocks = entries * (b->pages->page_size / 16) * b->Hkv;
+    return (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)8 * b->sm_count);
+}
+
+template <int D, int FMT>
+int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& args, int rows, bool capturing) {
+    if constexpr (D <= 128) {
+        constexpr bool q8 = FMT == kKvQ8Head;
+        const int64_t scale_rows = (int64_t)b->dense_rows + 128;  // (whole tiles are read)
+        if constexpr (q8) {
+            ReadArgs r{};
+            r.pages = b->pages->v;
+            r.counts = b->dense_counts();
+            r.table = reinterpret_cast<const int*>(b->d_plan + b->at_dense_table);
+            r.entries = reinterpret_cast<const int2*>(b->d_plan + b->at_dense_entries);
+            r.layer = args.layer;
+            r.k_out = b->d_dense;
+            r.v_out = b->d_dense + b->dense_rows * b->Hkv * b->D;
+            r.k_stride = r.v_stride = (int64_t)b->Hkv * b->D;
+            r.ks_out = b->d_dense_scales;
+            r.vs_out = b->d_dense_scales + b->Hkv * scale_rows;
+            r.scale_rows = scale_rows;
+            {
+                PathTimer t(c, 1);
+                paged_read_kernel<kKvQ8Head, D, kReadCodes><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
+            }
+            PAGED_TRY(c, cudaGetLastError());
+            path_launched(c);
+        }
+        PagedTcArgs t{};
+        t.a = args;
+        t.a.plan.counts = b->counts(list, kTc);
+        t.a.plan.items = b->items(list, kTc);
+        t.tiles_tokens = b->tc_tokens;
+        t.box_rows = b->pages ? std::min(b->pages->page_size, 128) : 128;
+        t.linear = !b->pages || q8;
+        t.dense_ks = b->d_dense_scales;
+        t.dense_vs = b->d_dense_scales + b->Hkv * scale_rows;
+        t.dense_rows = scale_rows;
+        t.sched = b->d_sched;
+        t.part = b->d_tc_part;
+        CUtensorMap tq;
+        if (!make_map3(&tq, false, args.q, D, b->Hq, rows, (uint64_t)D * 2, (uint64_t)args.q_stride * 2, 64, b->G, b->tc_tokens))
+            return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the query rows");
+        static KernelSmemSetup setup;
+        PAGED_TRY(c, setup.ensure(paged_tc_kernel<D, q8>, p.device, p.smem_optin, (int)kPtSmem<D>));
+        {
+            PathTimer timer(c, 0);
+            paged_tc_kernel<D, q8><<<capturing ? b->sm_count : std::min(b->sm_count, b->n_items[list][kTc]), kPtThreads, kPtSmem<D>, p.stream>>>(
+                tq, q8 ? b->tmKd : *m.k128, q8 ? b->tmVd : *m.v128, t);
+        }
+        PAGED_TRY(c, cudaGetLastError());
+        path_launched(c);
+        if (!capturing && !b->n_items[list][kMerge]) return GGR_OK;
+        t.a.plan.counts = b->counts(list, kMerge);
+        t.a.plan.items = b->items(list, kMerge);
+        const int pairs = capturing ? (int)b->tc_parts / 2 : b->n_items[list][kMerge];
+        {
+            PathTimer timer(c, 2);
+            PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(std::min(pairs * 32, 8 * b->sm_count)), 256, 0, p.stream, t));
+        }
+        path_launched(c);
+    }
+    return GGR_OK;
+}
+
 template <int D, int FMT, bool F32>
-int launch_attention(ggr_attn_ctx* c, const PathView& p, const ggr_batch* b, int list, const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnArgs a, bool capturing) {
+int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, PagedAttnArgs a, int rows, bool capturing) {
+    if (capturing && !b->n_tokens) return path_fail(c, GGR_ERR_INVALID, "a captured launch needs a plan with tokens: it holds the kernels of that plan");
     // a captured launch has to serve whatever plan its replays find: enough CTAs for any, items dealt in turn
     const int most = (2 * b->sm_count + b->Hkv - 1) / b->Hkv;
-    for (int k = 0; k < kKinds; ++k) {
+    for (int k = 0; k < kTc; ++k) {
         const int n = b->n_items[list][k];
-        if (!n && !capturing) continue;
+        if (!n) continue;
         a.plan.counts = b->counts(list, k);
         a.plan.items = b->items(list, k);
         const dim3 grid(capturing ? most : n, b->Hkv);
@@ -529,27 +802,35 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, const ggr_batch* b, int
                 static KernelSmemSetup setup;
                 PAGED_TRY(c, setup.ensure(paged_splitk_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
                 PathTimer t(c, 0);
-                paged_splitk_kernel<D, FMT, F32><<<grid, S::W * 32, S::SMEM, p.stream>>>(tk, tv, a);
+                paged_splitk_kernel<D, FMT, F32><<<grid, S::W * 32, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
             }
         } else {
             using S = PagedRowsShape<D, FMT, F32>;
             static KernelSmemSetup setup;
             PAGED_TRY(c, setup.ensure(paged_rows_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
             PathTimer t(c, 0);
-            paged_rows_kernel<D, FMT, F32><<<grid, 288, S::SMEM, p.stream>>>(tk, tv, a);
+            paged_rows_kernel<D, FMT, F32><<<grid, 288, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
         }
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
+        if (capturing) b->captured |= 1u << k;
+    }
+    if constexpr (!F32 && D <= 128) {
+        if (b->n_items[list][kTc]) {
+            const int rc = launch_tc<D, FMT>(c, p, b, list, m, a, rows, capturing);
+            if (rc) return rc;
+            if (capturing) b->captured |= 1u << kTc;
+        }
     }
     return GGR_OK;
 }
 
 template <int FMT, bool F32>
-int launch_by_dim(ggr_attn_ctx* c, const PathView& p, const ggr_batch* b, int list, const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnArgs& a, bool cap) {
+int launch_by_dim(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& a, int rows, bool cap) {
     switch (b->D) {
-        case 64: return launch_attention<64, FMT, F32>(c, p, b, list, tk, tv, a, cap);
-        case 128: return launch_attention<128, FMT, F32>(c, p, b, list, tk, tv, a, cap);
-        default: return launch_attention<256, FMT, F32>(c, p, b, list, tk, tv, a, cap);
+        case 64: return launch_attention<64, FMT, F32>(c, p, b, list, m, a, rows, cap);
+        case 128: return launch_attention<128, FMT, F32>(c, p, b, list, m, a, rows, cap);
+        default: return launch_attention<256, FMT, F32>(c, p, b, list, m, a, rows, cap);
     }
 }
 
@@ -633,18 +914,6 @@ extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, in
     return GGR_OK;
 }
 
-namespace {
-
-template <int FMT, int D>
-void launch_read(const ReadArgs& a, bool bf16, int grid, cudaStream_t stream) {
-    if (bf16)
-        paged_read_kernel<FMT, D, true><<<grid, 256, 0, stream>>>(a);
-    else
-        paged_read_kernel<FMT, D, false><<<grid, 256, 0, stream>>>(a);
-}
-
-}  // namespace
-
 extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride) {
     if (!c) return GGR_ERR_INVALID;
     int rc = check_call(c, b, layer, true);
@@ -666,8 +935,7 @@ extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int3
     a.v_out = v_out;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    const int64_t blocks = (int64_t)(capturing ? b->max_pages : b->n_entries) * (b->pages->page_size / 16) * b->Hkv;
-    const int grid = (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)8 * b->sm_count);
+    const int grid = read_grid(b, capturing ? b->max_pages : b->n_entries);
     const bool bf16 = out_dtype == GGR_DTYPE_BF16;
     {
         PathTimer t(c, 1);
@@ -709,11 +977,12 @@ extern "C" int ggr_paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer,
     a.q_stride = q_stride;
     a.o_stride = out_stride;
     const int list = b->list_of[layer];
-    const CUtensorMap &tk = b->pages->tmK16, &tv = b->pages->tmV16;
+    const Maps m{&b->pages->tmK16, &b->pages->tmV16, &b->pages->tmK128, &b->pages->tmV128};
     const bool f32 = b->dtype == GGR_DTYPE_F32;
+    const int rows = capturing ? b->max_tokens : b->n_tokens;
     if (b->pages->v.fmt == GGR_KV_BF16)
-        return f32 ? launch_by_dim<KV_BF16, true>(c, p, b, list, tk, tv, a, capturing) : launch_by_dim<KV_BF16, false>(c, p, b, list, tk, tv, a, capturing);
-    return f32 ? launch_by_dim<kKvQ8Head, true>(c, p, b, list, tk, tv, a, capturing) : launch_by_dim<kKvQ8Head, false>(c, p, b, list, tk, tv, a, capturing);
+        return f32 ? launch_by_dim<KV_BF16, true>(c, p, b, list, m, a, rows, capturing) : launch_by_dim<KV_BF16, false>(c, p, b, list, m, a, rows, capturing);
+    return f32 ? launch_by_dim<kKvQ8Head, true>(c, p, b, list, m, a, rows, capturing) : launch_by_dim<kKvQ8Head, false>(c, p, b, list, m, a, rows, capturing);
 }
 
 extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
@@ -741,7 +1010,8 @@ extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer
     a.pv = v;
     a.pk_stride = k_stride;
     a.pv_stride = v_stride;
-    CUtensorMap tk, tv;
+    CUtensorMap tk, tv, tk128, tv128;
+    const Maps m{&tk, &tv, &tk128, &tv128};
     const int list = b->list_of[layer];
     if (f32) {
         const int64_t plane = (int64_t)b->max_tokens * kv_dim;
@@ -758,10 +1028,13 @@ extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer
         }
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
-        return launch_by_dim<KV_F32, true>(c, p, b, list, tk, tv, a, capturing);
+        return launch_by_dim<KV_F32, true>(c, p, b, list, m, a, rows, capturing);
     }
-    if (!make_map3(&tk, false, k, b->D, b->Hkv, rows, (uint64_t)b->D * 2, (uint64_t)k_stride * 2, 64, 1, 16) ||
-        !make_map3(&tv, false, v, b->D, b->Hkv, rows, (uint64_t)b->D * 2, (uint64_t)v_stride * 2, 64, 1, 16))
+    const uint64_t sy = (uint64_t)b->D * 2;
+    if (!make_map3(&tk, false, k, b->D, b->Hkv, rows, sy, (uint64_t)k_stride * 2, 64, 1, 16) ||
+        !make_map3(&tv, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, 16) ||
+        !make_map3(&tk128, false, k, b->D, b->Hkv, rows, sy, (uint64_t)k_stride * 2, 64, 1, 128) ||
+        !make_map3(&tv128, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, 128))
         return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
-    return launch_by_dim<KV_BF16, false>(c, p, b, list, tk, tv, a, capturing);
+    return launch_by_dim<KV_BF16, false>(c, p, b, list, m, a, rows, capturing);
 }

@@ -41,6 +41,9 @@ struct PagedItem {
     int part;   // key splits: first partial state of the row tile (in tiles), else -1
     int split, n_split;
     int ticket;
+    int kvh;    // tcgen05 kernel only: its items are dealt over all KV heads; row0 is then a token, not a packed row
+    int lin;    // and the dense row of the sequence's first key where tiles come from dense rows
+    int unused[2];
 };
 
 // What a launch reads from the plan on the device.
@@ -209,12 +212,17 @@ struct ReadArgs {
     void* k_out;
     void* v_out;
     int64_t k_stride, v_stride;  // elements between dense rows
+    float* ks_out;               // kReadCodes: scales [KV head][scale_rows]
+    float* vs_out;
+    int64_t scale_rows;
 };
+
+enum ReadOut { kReadF32 = 0, kReadBf16 = 1, kReadCodes = 2 };  // kReadCodes: the codes themselves in bf16, their scales apart
 
 // Rows of all sequences out of their pages: a warp-wide task is 16 elements of one row, a CTA takes blocks of 16 rows of one
 // KV head of K and of V. The page ids of four blocks are fetched before the rows of any, and the rows of four before the
 // first is stored: a block alone is two dependent loads.
-template <int FMT, int D, bool OUT_BF16>
+template <int FMT, int D, int OUT>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
     constexpr int per_row = D / 16, rows_per_pass = 128 / per_row;  // 128 threads for K, 128 for V
     constexpr int passes = (16 + rows_per_pass - 1) / rows_per_pass;
@@ -273,10 +281,11 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
                 } else {
                     const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) x[q] = (float)(int8_t)(w[q >> 2] >> (8 * (q & 3))) * scale[i];
+                    for (int q = 0; q < 16; ++q) x[q] = (float)(int8_t)(w[q >> 2] >> (8 * (q & 3))) * (OUT == kReadCodes ? 1.0f : scale[i]);
+                    if (OUT == kReadCodes && e == 0) (is_v ? a.vs_out : a.ks_out)[head[u] * a.scale_rows + dense[u] + r] = scale[i];
                 }
                 const int64_t to = (int64_t)(dense[u] + r) * stride + (int64_t)head[u] * D + e;
-                if constexpr (OUT_BF16) {
+                if constexpr (OUT != kReadF32) {
                     uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to);
                     if constexpr (FMT == KV_BF16) {
                         o[0] = raw[i][0];

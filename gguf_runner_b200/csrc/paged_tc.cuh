@@ -1,0 +1,642 @@
+// Attention of chunks and of packed prompts in bf16 on the 5th-generation tensor cores, head_dim 64 and 128.
+//
+// The pipeline is that of the dense prefill kernel (prefill_tc.cuh): a persistent CTA per SM, a producer warp, one MMA issuer,
+// two softmax warpgroups with a 128-row query tile each that take turns on the tensor core, S and O in tensor memory, P
+// written over S. What differs is where rows come from:
+//  - A query tile holds 128 / G tokens times the G query heads of one KV head (one 3-D copy: element, head, token), so that a
+//    key tile is read once for all heads that share it and a chunk of few tokens still fills the tensor core's 128 rows.
+//  - A 128-key tile is gathered from its pages, a copy per page (half a page of 256) and 64-column block, issued by the lanes
+//    of the producer warp side by side; each lane looks its page up one tile ahead.
+//  - Items (two query tiles and a stretch of keys) are cut on the host, longest first, and handed out through a counter. Pieces
+//    of a pair of tiles leave un-normalised rows, which paged_tc_merge_kernel weighs in the order of the keys.
+//  - Codes of 8-bit pages come as dense rows of bf16 (paged_read_kernel, which every code survives; 17 us of 480 for 2048
+//    tokens behind 14336, 40/8 heads of 128), and their scales stay apart: the softmax multiplies scores by those of K and
+//    weights by those of V, so that 8-bit rows cost no rounding of their own. A lane fetches four of a tile's 128 scales one
+//    tile ahead, and the warp reads them back from its output staging area.
+// Values that nobody in the item sees (behind the sequence's end, before its window) may be anything, and 0 * NaN is NaN: the
+// producer clears them in the first and last tile, before the MMA issuer hears of the tile. Rows that come out not finite are
+// computed again by paged_row_again.
+#pragma once
+
+#include "paged_mma.cuh"
+
+namespace ggr {
+
+struct PagedTcArgs {
+    PagedAttnArgs a;
+    int tiles_tokens;  // tokens of a query tile: 128 / G
+    int box_rows;      // paged: rows of one copy, min(page_size, 128)
+    int linear;        // K and V tiles come from dense rows (packed prompts, or the codes of 8-bit pages)
+    const float* dense_ks;  // 8-bit pages: scales of the dense rows [KV head][dense_rows]
+    const float* dense_vs;
+    int64_t dense_rows;
+    int* sched;        // [0] items handed out beyond the first wave, [1] CTAs that have left
+    float* part;       // states of pieces: [256][D], then [256] (m, l)
+};
+
+constexpr int kPtThreads = 384, kPtCtrlRegs = 88, kPtSoftmaxRegs = 208;
+static_assert(tc::RegSplitOk<kPtCtrlRegs, kPtSoftmaxRegs>::value, "setmaxnreg split would never complete");
+constexpr int kPtExpPolyMask = 0x5;  // groups of four scores of which one pair takes its exponentials from the FMA pipe
+template <int D>
+constexpr int kPtState = 256 * (D + 2);
+template <int D>
+constexpr size_t kPtSmem = (size_t)6 * (D / 64) * 128 * 128 + 8 * 4096 + 1024;
+
+// The key tiles of an item that each query tile walks.
+struct PtRange {
+    int lo0, hi0, lo1, hi1, lo, hi;
+    __device__ __forceinline__ int lo_of(int t) const { return t ? lo1 : lo0; }
+    __device__ __forceinline__ int hi_of(int t) const { return t ? hi1 : hi0; }
+    __device__ __forceinline__ bool active(int t, int j) const { return j >= lo_of(t) && j < hi_of(t); }
+};
+__device__ __forceinline__ PtRange pt_range(const PagedTcArgs& p, const PagedItem& w) {
+    PtRange r;
+    int lo_t[2], hi_t[2];
+    const int s_lo = w.key0 >> 7, s_hi = (w.key1 + 127) >> 7;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = w.row0 + t * p.tiles_tokens, last = min(first + p.tiles_tokens, w.n_tok) - 1;
+        lo_t[t] = hi_t[t] = 0;
+        if (first > last) continue;
+        lo_t[t] = max(s_lo, paged_first_key(w.pos0 + first, p.a.window) >> 7);
+        hi_t[t] = max(lo_t[t], min(s_hi, (w.pos0 + last + 128) >> 7));
+    }
+    r.lo0 = lo_t[0], r.hi0 = hi_t[0], r.lo1 = lo_t[1], r.hi1 = hi_t[1];
+    const bool act0 = r.hi0 > r.lo0, act1 = r.hi1 > r.lo1;
+    r.lo = act0 ? r.lo0 : r.lo1;
+    r.hi = act0 ? r.hi0 : r.hi1;
+    if (act0 && act1) {
+        r.lo = min(r.lo0, r.lo1);
+        r.hi = max(r.hi0, r.hi1);
+    }
+    return r;
+}
+
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void lds_f32x4(uint32_t at, uint64_t& lo, uint64_t& hi) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(at));
+}
+
+// SCALED: rows are codes, with scales beside them.
+template <int D, bool SCALED>
+__global__ void __launch_bounds__(kPtThreads, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const __grid_constant__ PagedTcArgs p) {
+    using namespace tc;
+    constexpr int NBLK = D / 64;
+    constexpr uint32_t BLK = 128 * 128, TILE = NBLK * BLK, O_COL0 = 256;
+
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t bars[25];
+    __shared__ uint32_t s_tmem_base;
+    __shared__ int s_abort;
+    __shared__ __align__(16) PagedItem s_item[2];
+    __shared__ int s_live[2];
+
+    const PagedAttnArgs& a = p.a;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sQ = smem_base, sK = sQ + 2 * TILE, sV = sK + 2 * TILE, sOut = sV + 2 * TILE;
+
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t q_full = bar0, q_empty = bar0 + 8u, raw = bar0 + 8u * 24;
+    auto k_full = [&](int s) { return bar0 + 8u * (2 + s); };
+    auto k_empty = [&](int s) { return bar0 + 8u * (4 + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (6 + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (8 + s); };
+    auto s_full = [&](int t) { return bar0 + 8u * (10 + t); };
+    auto p_half = [&](int t, int half) { return bar0 + 8u * (12 + 2 * t + half); };
+    auto o_final = [&](int t) { return bar0 + 8u * (16 + t); };
+    auto o_free = [&](int t) { return bar0 + 8u * (18 + t); };
+    auto item_full = [&](int s) { return bar0 + 8u * (20 + s); };
+    auto item_empty = [&](int s) { return bar0 + 8u * (22 + s); };
+
+    if (tid == 0) {
+        s_abort = 0;
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(raw, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(k_full(s), 1);
+            mbar_init(k_empty(s), 1);
+            mbar_init(v_full(s), 1);
+            mbar_init(v_empty(s), 1);
+            mbar_init(s_full(s), 1);
+            mbar_init(p_half(s, 0), 128);
+            mbar_init(p_half(s, 1), 128);
+            mbar_init(o_final(s), 1);
+            mbar_init(o_free(s), 128);
+            mbar_init(item_full(s), 1);
+            mbar_init(item_empty(s), 9);  // lane 0 of the eight softmax warps and of the MMA issuer
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&s_tmem_base), 512);
+        tmem_relinquish();
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = s_tmem_base;
+    volatile int* abortp = &s_abort;
+    volatile int* livep = s_live;
+
+    if (warp >= 8) {
+        reg_release<kPtCtrlRegs>();
+        if (warp == 8) {
+            // ---------------- scheduler + TMA producer: the whole warp, a lane per copy ----------------
+            const int n_items = a.plan.counts[0];
+            const int boxes = p.linear ? 1 : 128 / p.box_rows, copies = boxes * NBLK;
+            const int box = lane / NBLK, blk = lane % NBLK, box_key = p.linear ? 0 : box * p.box_rows;
+            const uint32_t box_at = blk * BLK + box_key * 128, box_bytes = p.linear ? BLK : p.box_rows * 128;
+            const uint32_t q_bytes = (uint32_t)p.tiles_tokens * a.G * 128 * NBLK;
+            const int page_log2 = a.pages.page_log2;
+            int g = 0;  // K / V tiles requested so far (ring position)
+            uint32_t raws = 0;
+            for (int it = 0;; ++it) {
+                const int slot = it & 1;
+                if (!mbar_wait_warp(item_empty(slot), ((it >> 1) & 1) ^ 1, abortp)) break;
+                int r = 0;
+                if (lane == 0) r = it == 0 ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.sched, 1);
+                r = __shfl_sync(0xffffffffu, r, 0);
+                const bool live = r < n_items;
+                if (live && lane < (int)(sizeof(PagedItem) / 4))
+                    reinterpret_cast<int*>(&s_item[slot])[lane] = reinterpret_cast<const int*>(a.plan.items + r)[lane];
+                if (lane == 0) s_live[slot] = live;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(item_full(slot));
+                if (!live) break;
+                const PagedItem w = s_item[slot];
+                const PtRange rg = pt_range(p, w);
+                const bool act0 = rg.hi0 > rg.lo0, act1 = rg.hi1 > rg.lo1;
+                if (!mbar_wait_warp(q_empty, (it & 1) ^ 1, abortp)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(q_full, ((act0 ? 1 : 0) + (act1 ? 1 : 0)) * q_bytes);
+                    for (int t = 0; t < 2; ++t) {
+                        if (!(t == 0 ? act0 : act1)) continue;
+                        for (int b = 0; b < NBLK; ++b)
+                            tma_load_3d(sQ + t * TILE + b * BLK, &tmQ, b * 64, w.kvh * a.G, w.tok0 + w.row0 + t * p.tiles_tokens, q_full);
+                    }
+                }
+                // values outside [any_lo, any_hi) are seen by no row of the item; pages end with the sequence
+                const int any_lo = paged_first_key(w.pos0 + w.row0, a.window);
+                const int any_hi = w.pos0 + min(w.row0 + 2 * p.tiles_tokens, w.n_tok), kv_end = w.pos0 + w.n_tok;
+                auto page_of = [&](int j) {
+                    const int key = j * 128 + box_key;
+                    return !p.linear && lane < copies && key < kv_end && j < rg.hi ? a.plan.table[w.src + (key >> page_log2)] : 0;
+                };
+                int page = page_of(rg.lo);
+                bool ok = true;
+                for (int j = rg.lo; j < rg.hi; ++j, ++g) {
+                    const int s = g & 1, key = j * 128 + box_key;
+                    const uint32_t ph = ((g >> 1) & 1) ^ 1;
+                    const bool mine = lane < copies && (p.linear || key < kv_end);
+                    const uint32_t bytes = box_bytes * __popc(__ballot_sync(0xffffffffu, mine));
+                    const int y = p.linear ? w.kvh : key & ((1 << page_log2) - 1);
+                    const int z = p.linear ? w.lin + key : (a.layer * a.pages.n_pages + page) * a.pages.Hkv + w.kvh;
+                    page = page_of(j + 1);
+                    if (!(ok = mbar_wait_warp(k_empty(s), ph, abortp))) break;
+                    if (lane == 0) mbar_expect_tx(k_full(s), bytes);
+                    __syncwarp();
+                    if (mine) tma_load_3d(sK + s * TILE + box_at, &tmK, blk * 64, y, z, k_full(s));
+                    if (!(ok = mbar_wait_warp(v_empty(s), ph, abortp))) break;
+                    const bool edge = j * 128 < any_lo || (j + 1) * 128 > any_hi;
+                    const uint32_t vbar = edge ? raw : v_full(s);
+                    if (lane == 0) mbar_expect_tx(vbar, bytes);
+                    __syncwarp();
+                    if (mine) tma_load_3d(sV + s * TILE + box_at, &tmV, blk * 64, y, z, vbar);
+                    if (edge) {
+                        if (!(ok = mbar_wait_warp(raw, raws & 1u, abortp))) break;
+                        ++raws;
+                        for (int i = lane; i < 128 * NBLK * 8; i += 32) {
+                            const int row = (i >> 3) & 127, k = j * 128 + row;
+                            if (k >= any_lo && k < any_hi) continue;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sV + s * TILE + (i >> 10) * BLK + row * 128 + (i & 7) * 16), "r"(0u)
+                                         : "memory");
+                        }
+                        fence_smem_to_async_proxy();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_full(s));
+                    }
+                }
+                if (!ok) break;
+            }
+        } else if (warp == 9) {
+            // ---------------- MMA issuer ----------------
+            constexpr uint32_t IDESC_QK = idesc_bf16(128, 0), IDESC_PV = idesc_bf16(D, 1);
+            const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024), dV = smem_desc(sV, BLK, 1024);
+            const uint32_t tm = __shfl_sync(0xffffffffu, s_tmem_base, 0);
+            auto issue_qk = [&](int t, int s) {
+                const uint64_t a0 = dQ + (uint64_t)((t * TILE) >> 4), b0 = dK + (uint64_t)((s * TILE) >> 4);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint32_t off = ((ks >> 2) * BLK + (ks & 3) * 32) >> 4;
+                    mma_ss_e(tm + t * 128, a0 + off, b0 + off, IDESC_QK, ks > 0 ? 1u : 0u);
+                }
+            };
+            auto issue_pv_half = [&](int t, int s, int half, bool accumulate) {
+                const uint64_t b0 = dV + (uint64_t)((s * TILE) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const int ks = half * 4 + kk;
+                    mma_ts_e(tm + O_COL0 + t * D, tm + t * 128 + ks * 8, b0 + (uint64_t)((ks * 16 * 128) >> 4), IDESC_PV, (accumulate || ks > 0) ? 1u : 0u);
+                }
+            };
+            int g = 0, c0 = 0, c1 = 0;
+            bool ok = true;
+            for (int it = 0; ok; ++it) {
+                const int slot = it & 1;
+                if (!(ok = mbar_wait_warp(item_full(slot), (it >> 1) & 1, abortp))) break;
+                const int live = __shfl_sync(0xffffffffu, livep[slot], 0);
+                PtRange w = pt_range(p, s_item[slot]);
+                w.lo0 = __shfl_sync(0xffffffffu, w.lo0, 0);
+                w.hi0 = __shfl_sync(0xffffffffu, w.hi0, 0);
+                w.lo1 = __shfl_sync(0xffffffffu, w.lo1, 0);
+                w.hi1 = __shfl_sync(0xffffffffu, w.hi1, 0);
+                w.lo = __shfl_sync(0xffffffffu, w.lo, 0);
+                w.hi = __shfl_sync(0xffffffffu, w.hi, 0);
+                if (lane == 0) mbar_arrive(item_empty(slot));
+                if (!live) break;
+                const int lo = w.lo, hi = w.hi;
+                // every item moves o_free and o_final of both tiles on by one phase
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (w.hi_of(t) <= w.lo_of(t)) {
+                        if (!(ok = mbar_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
+                        if (lane == 0) mbar_arrive(o_final(t));
+                    }
+                if (!ok) break;
+                if (!(ok = mbar_wait_warp(q_full, it & 1, abortp))) break;
+                if (hi == lo) {
+                    mma_commit_e(q_empty);
+                    continue;
+                }
+                if (!(ok = mbar_wait_warp(k_full(g & 1), (g >> 1) & 1, abortp))) break;
+                fence_after_sync();
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (w.active(t, lo)) {
+                        issue_qk(t, g & 1);
+                        mma_commit_e(s_full(t));
+                    }
+                mma_commit_e(k_empty(g & 1));
+                if (hi - lo == 1) mma_commit_e(q_empty);
+                for (int j = lo; j < hi; ++j, ++g) {
+                    const int s = g & 1;
+                    const bool has_next = j + 1 < hi;
+                    if (!(ok = mbar_wait_warp(v_full(s), (g >> 1) & 1, abortp))) break;
+                    bool next_k_ready = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int lo_t = w.lo_of(t), hi_t = w.hi_of(t), c_t = t ? c1 : c0;
+                        if (j >= lo_t && j < hi_t) {
+                            const uint32_t ph = (c_t + j - lo_t) & 1;
+                            if (!(ok = mbar_wait_warp(p_half(t, 0), ph, abortp))) break;
+                            if (j == lo_t && !(ok = mbar_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
+                            fence_after_sync();
+                            issue_pv_half(t, s, 0, j > lo_t);
+                            if (!(ok = mbar_wait_warp(p_half(t, 1), ph, abortp))) break;
+                            fence_after_sync();
+                            issue_pv_half(t, s, 1, true);
+                            if (j == hi_t - 1) mma_commit_e(o_final(t));
+                        }
+                        if (has_next && j + 1 >= lo_t && j + 1 < hi_t) {
+                            if (!next_k_ready) {
+                                if (!(ok = mbar_wait_warp(k_full(s ^ 1), ((g + 1) >> 1) & 1, abortp))) break;
+                                fence_after_sync();
+                                next_k_ready = true;
+                            }
+                            issue_qk(t, s ^ 1);
+                            mma_commit_e(s_full(t));
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit_e(v_empty(s));
+                    if (has_next) {
+                        mma_commit_e(k_empty(s ^ 1));
+                        if (j + 2 == hi) mma_commit_e(q_empty);
+                    }
+                }
+                c0 += w.hi0 - w.lo0;
+                c1 += w.hi1 - w.lo1;
+            }
+        }
+    } else {
+        // ---------------- softmax warps: one thread per query row ----------------
+        reg_acquire<kPtSoftmaxRegs>();
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int tile_tok = row / a.G, head = row - tile_tok * a.G;  // token of the tile and head of the group
+        const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lane_addr + t * 128, tO = tmem + lane_addr + O_COL0 + t * D;
+        const float c = a.c, thr = 8.0f / c;
+        bool ok = true;
+        int cs = 0;
+        for (int it = 0; ok; ++it) {
+            const int slot = it & 1;
+            if (!(ok = mbar_wait(item_full(slot), (it >> 1) & 1, abortp))) break;
+            const int live = livep[slot];
+            const PagedItem w = s_item[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(item_empty(slot));
+            if (!live) break;
+            const PtRange rg = pt_range(p, w);
+            const int lo_t = rg.lo_of(t), hi_t = rg.hi_of(t), n_t = hi_t - lo_t;
+            const int tok = w.row0 + t * p.tiles_tokens + tile_tok;
+            const bool valid = tile_tok < p.tiles_tokens && tok < w.n_tok;
+            int vs = 0, ve = 0;
+            if (valid) {
+                ve = w.pos0 + tok + 1;
+                vs = paged_first_key(w.pos0 + tok, a.window);
+            }
+            float m_used = -INFINITY, l = 0.0f;
+            const uint32_t scales = sOut + (uint32_t)warp * 4096u;  // 128 of K, 128 of V
+            float4 next_ks, next_vs;
+            auto fetch_scales = [&](int j) {
+                const int key = j * 128 + lane * 4;
+                const int64_t at = (int64_t)w.kvh * p.dense_rows + w.lin + key;
+                const int any_lo = paged_first_key(w.pos0 + w.row0, a.window), any_hi = w.pos0 + min(w.row0 + 2 * p.tiles_tokens, w.n_tok);
+                next_ks = __ldg(reinterpret_cast<const float4*>(p.dense_ks + at));
+                next_vs = __ldg(reinterpret_cast<const float4*>(p.dense_vs + at));
+                // a weight of zero times what lies beside the item's keys must stay zero
+                if (key < any_lo || key >= any_hi) next_vs.x = 0.0f;
+                if (key + 1 < any_lo || key + 1 >= any_hi) next_vs.y = 0.0f;
+                if (key + 2 < any_lo || key + 2 >= any_hi) next_vs.z = 0.0f;
+                if (key + 3 < any_lo || key + 3 >= any_hi) next_vs.w = 0.0f;
+            };
+            if (SCALED && lo_t < hi_t) fetch_scales(lo_t);
+            for (int j = lo_t; j < hi_t; ++j) {
+                const int k = j - lo_t;
+                if constexpr (SCALED) {
+                    __syncwarp();
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales + lane * 16), "f"(next_ks.x), "f"(next_ks.y), "f"(next_ks.z),
+                                 "f"(next_ks.w) : "memory");
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales + 512 + lane * 16), "f"(next_vs.x), "f"(next_vs.y), "f"(next_vs.z),
+                                 "f"(next_vs.w) : "memory");
+                    __syncwarp();
+                    if (j + 1 < hi_t) fetch_scales(j + 1);
+                }
+                if (!(ok = mbar_wait(s_full(t), (cs + k) & 1, abortp))) break;
+                fence_after_sync();
+                uint32_t sr[4][32];
+#pragma unroll
+                for (int cidx = 0; cidx < 4; ++cidx) tmem_ld32(tS + cidx * 32, sr[cidx]);
+                tmem_wait_ld();
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int cidx = 0; cidx < 4; ++cidx)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            uint64_t k01, k23;
+                            lds_f32x4(scales + (cidx * 32 + i) * 4, k01, k23);
+                            float x0, x1, x2, x3;
+                            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1])), k01), x0, x1);
+                            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3])), k23), x2, x3);
+                            sr[cidx][i] = __float_as_uint(x0);
+                            sr[cidx][i + 1] = __float_as_uint(x1);
+                            sr[cidx][i + 2] = __float_as_uint(x2);
+                            sr[cidx][i + 3] = __float_as_uint(x3);
+                        }
+                }
+                const int key0 = j * 128;
+                const bool cut = key0 < vs || key0 + 128 > ve, any_cut = __any_sync(0xffffffffu, cut);
+                if (cut) {
+#pragma unroll
+                    for (int cidx = 0; cidx < 4; ++cidx)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int key = key0 + cidx * 32 + i;
+                            if (key < vs || key >= ve) sr[cidx][i] = 0xff800000u;  // -inf
+                        }
+                }
+                float mxa = -INFINITY, mxb = -INFINITY, mxc = -INFINITY, mxd = -INFINITY;
+#pragma unroll
+                for (int cidx = 0; cidx < 4; ++cidx)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        mxa = max3(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
+                        mxb = max3(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
+                        mxc = max3(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
+                        mxd = max3(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
+                    }
+                const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+                const bool need = mx > m_used + thr;
+                float alpha = 1.0f;
+                if (need) {
+                    alpha = ex2((m_used - mx) * c);
+                    m_used = mx;
+                }
+                if (k > 0 && __any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+                    for (int cidx = 0; cidx < D / 32; ++cidx) {
+                        uint32_t orow[32];
+                        tmem_ld32(tO + cidx * 32, orow);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) orow[i] = __float_as_uint(__uint_as_float(orow[i]) * alpha);
+                        tmem_st32(tO + cidx * 32, orow);
+                    }
+                }
+                l *= alpha;
+                const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
+                const float neg = -mref * c;
+                const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
+                uint64_t sum_a = 0ull, sum_b = 0ull;
+#pragma unroll
+                for (int cidx = 0; cidx < 4; ++cidx) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const uint64_t ta = fma_f32x2(pack_f32x2(__uint_as_float(sr[cidx][2 * i]), __uint_as_float(sr[cidx][2 * i + 1])), c2, neg2);
+                        const uint64_t tb = fma_f32x2(pack_f32x2(__uint_as_float(sr[cidx][2 * i + 2]), __uint_as_float(sr[cidx][2 * i + 3])), c2, neg2);
+                        float x0, x1, p2, p3;
+                        unpack_f32x2(ta, x0, x1);
+                        float p0 = ex2(x0), p1 = ex2(x1);
+                        if (kPtExpPolyMask & (1 << ((i >> 1) & 3))) {
+                            ex2_poly_x2(tb, p2, p3);
+                        } else {
+                            float x2, x3;
+                            unpack_f32x2(tb, x2, x3);
+                            p2 = ex2(x2);
+                            p3 = ex2(x3);
+                        }
+                        sum_a = add_f32x2(sum_a, pack_f32x2(p0, p1));
+                        sum_b = add_f32x2(sum_b, pack_f32x2(p2, p3));
+                        if constexpr (SCALED) {
+                            uint64_t v01, v23;
+                            lds_f32x4(scales + 512 + (cidx * 32 + 2 * i) * 4, v01, v23);
+                            unpack_f32x2(mul_f32x2(pack_f32x2(p0, p1), v01), p0, p1);
+                            unpack_f32x2(mul_f32x2(pack_f32x2(p2, p3), v23), p2, p3);
+                        }
+                        pk[i] = pack_bf16x2(p0, p1);
+                        pk[i + 1] = pack_bf16x2(p2, p3);
+                    }
+                    if (any_cut) {
+                        // the polynomial gives 2^-125 for a hidden key, which a large value there would show: exactly zero instead
+                        const int lo = min(max(vs - key0 - cidx * 32, 0), 32), hi = min(max(ve - key0 - cidx * 32, 0), 32);
+                        const uint32_t seen = hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            pk[i] &= ((seen >> (2 * i)) & 1u ? 0xffffu : 0u) | ((seen >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+                    }
+                    tmem_st16(tS + cidx * 16, pk);
+                    if (cidx == 1) {
+                        tmem_wait_st();
+                        fence_before_sync();
+                        mbar_arrive(p_half(t, 0));
+                    }
+                }
+                {
+                    float s0, s1;
+                    unpack_f32x2(add_f32x2(sum_a, sum_b), s0, s1);
+                    l += s0 + s1;
+                }
+                tmem_wait_st();
+                fence_before_sync();
+                mbar_arrive(p_half(t, 1));
+            }
+            if (!ok) break;
+            cs += n_t;
+            if (!(ok = mbar_wait(o_final(t), it & 1, abortp))) break;
+            fence_after_sync();
+            const bool split = w.part >= 0;
+            float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPtState<D>;
+            if (split) __stcg(reinterpret_cast<float2*>(state + 256 * D) + t * 128 + row, make_float2(n_t > 0 ? m_used : -INFINITY, n_t > 0 ? l : 0.0f));
+            bool bad = false;
+            if (n_t > 0) {
+                // rows leave through a per-warp staging area of 32 rows x 128 bytes, 16-byte pieces XORed by the row, and are
+                // stored as whole 128-byte lines: 64 bf16 columns at a time, or 32 columns of a piece's f32 state
+                const float inv = 1.0f / l;
+                const uint32_t stage = sOut + (uint32_t)warp * 4096u;
+                const int sub_row = lane >> 3, piece = lane & 7;
+                const int64_t my_at = valid ? (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D : -1;
+#pragma unroll 1
+                for (int cidx = 0; cidx < D / 32; ++cidx) {
+                    uint32_t orow[32];
+                    tmem_ld32(tO + cidx * 32, orow);
+                    tmem_wait_ld();
+                    if (split) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128u + (uint32_t)(((i >> 2) ^ (lane & 7)) << 4)),
+                                         "r"(orow[i]), "r"(orow[i + 1]), "r"(orow[i + 2]), "r"(orow[i + 3]) : "memory");
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const float x = __uint_as_float(orow[i + 2 * q]) * inv, y = __uint_as_float(orow[i + 2 * q + 1]) * inv;
+                                bad |= !isfinite(x) | !isfinite(y);
+                                h[q] = pack_bf16x2(x, y);
+                            }
+                            const int pc = (cidx & 1) * 4 + (i >> 3);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128u + (uint32_t)((pc ^ (lane & 7)) << 4)), "r"(h[0]),
+                                         "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        }
+                        if (!(cidx & 1)) continue;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k4 = 0; k4 < 8; ++k4) {
+                        const int rr = k4 * 4 + sub_row;
+                        uint4 x;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                     : "r"(stage + rr * 128u + (uint32_t)((piece ^ (rr & 7)) << 4)));
+                        const int64_t at = __shfl_sync(0xffffffffu, my_at, rr);
+                        if (at < 0) continue;
+                        if (split)
+                            __stcg(reinterpret_cast<uint4*>(state + (int64_t)(t * 128 + (warp & 3) * 32 + rr) * D + cidx * 32 + piece * 4), x);
+                        else
+                            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + (cidx >> 1) * 64 + piece * 8) = x;
+                    }
+                    __syncwarp();
+                }
+                fence_before_sync();
+            }
+            mbar_arrive(o_free(t));
+            unsigned again = __ballot_sync(0xffffffffu, bad && valid);
+            while (again) {
+                const int rr = __ffs(again) - 1;
+                again &= again - 1;
+                const int tk = __shfl_sync(0xffffffffu, tok, rr), hd = __shfl_sync(0xffffffffu, head, rr);
+                paged_row_again<D, false>(a, w, w.kvh, tk * a.G + hd, lane);
+            }
+        }
+    }
+
+    // ---------------- common tail ----------------
+    if (s_abort) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // let copies in flight land
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (tid == 0) {
+        if (s_abort && a.err) atomicExch(a.err, 1);
+        // the last CTA to leave rewinds the work counter for the next launch
+        __threadfence();
+        if (atomicAdd(p.sched + 1, 1) == (int)gridDim.x - 1) {
+            p.sched[0] = 0;
+            p.sched[1] = 0;
+            __threadfence();
+        }
+    }
+}
+
+// Weighs the pieces of every pair of query tiles that was cut: a warp per row, pieces in the order of their keys. The list holds
+// the first piece of each pair.
+template <int D>
+__global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_constant__ PagedTcArgs p) {
+    grid_wait();
+    const PagedAttnArgs& a = p.a;
+    constexpr int V = D / 32;  // elements of a lane
+    const int lane = threadIdx.x & 31;
+    const int n = a.plan.counts[0] * 256;
+    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
+        const PagedItem& w = a.plan.items[i >> 8];
+        const int r = i & 255, t = r >> 7, tile_tok = (r & 127) / a.G, head = (r & 127) - tile_tok * a.G;
+        const int tok = w.row0 + t * p.tiles_tokens + tile_tok;
+        if (tile_tok >= p.tiles_tokens || tok >= w.n_tok) continue;
+        const float* state = p.part + (int64_t)w.part * kPtState<D>;
+        float top = -INFINITY;
+        for (int s = lane; s < w.n_split; s += 32)
+            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(state + (int64_t)s * kPtState<D> + 256 * D) + r).x);
+        top = warp_max(top);
+        float o[V] = {}, l = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < w.n_split; ++s) {
+            const float* st = state + (int64_t)s * kPtState<D>;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(st + 256 * D) + r);
+            if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing seen: no rows were left either
+            const float f = tc::ex2((ml.x - top) * a.c);
+            l = fmaf(f, ml.y, l);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                const float2 x = __ldcg(reinterpret_cast<const float2*>(st + (int64_t)r * D + e * 64) + lane);
+                o[2 * e] = fmaf(f, x.x, o[2 * e]);
+                o[2 * e + 1] = fmaf(f, x.y, o[2 * e + 1]);
+            }
+        }
+        const float inv = 1.0f / l;
+        bool bad = false;
+        uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D);
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+            const float x = o[2 * e] * inv, y = o[2 * e + 1] * inv;
+            bad |= !isfinite(x) | !isfinite(y);
+            out[e * 32 + lane] = pack_bf16x2(x, y);
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+            __syncwarp();
+            paged_row_again<D, false>(a, w, w.kvh, tok * a.G + head, lane);
+        }
+    }
+}
+
+}  // namespace ggr

@@ -418,8 +418,10 @@ void ggr_batch_destroy(ggr_batch* batch);
  * j < ceil(kv_len / page_size); entries behind that are not read. Pages may be shared between sequences (a common prefix),
  * but a page that receives new rows receives them from one sequence (else GGR_ERR_INVALID). A plan without pages has kv_len =
  * q_len and no table. A layer with a window w sees the last w positions, the current one included; pages before that may be
- * reused: their entries only have to name a page. The call copies its arrays and enqueues one upload; it does not belong into a
- * stream capture, but captured launches of the plan follow it when they are replayed behind it.
+ * reused: their entries only have to name a page. The call copies its arrays and enqueues their upload; it does not belong into a
+ * stream capture, but captured launches of the plan follow it when they are replayed behind it. A captured call has to be
+ * given buffers of max_tokens rows, as replays may find a longer step; it holds the kernels of the step it was captured with,
+ * and the plan keeps to those from then on: token steps that are replayed are best given a plan of their own.
  */
 int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
                   int32_t table_stride);
@@ -443,8 +445,7 @@ int ggr_paged_read(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t o
 int ggr_paged_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, void* out,
                         int64_t out_stride);
 /*
- * Causal attention of whole prompts straight from their rotated q, k and v rows, no cache involved. A captured launch has to
- * be given buffers of max_tokens rows: replays may find a longer plan.
+ * Causal attention of whole prompts straight from their rotated q, k and v rows, no cache involved.
  */
 int ggr_packed_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride);
