@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <functional>
 #include <memory>
 #include <new>
 #include <string>
@@ -111,12 +112,13 @@ struct ggr_batch {
     size_t at_counts = 0, at_pos = 0, at_slot = 0, at_entries = 0, at_table = 0, at_items[kMaxLists][kKinds] = {}, bytes = 0;
     float* d_part = nullptr;
     unsigned* d_tickets = nullptr;
-    __nv_bfloat16* d_planes = nullptr;  // packed f32 rows: [k, v][2 planes][max_tokens][Hkv * D]
+    __nv_bfloat16* d_planes = nullptr;  // packed f32 rows: [k, v][3 planes][max_tokens][Hkv * D]
     // the plan in force
     bool set = false;
     int n_seqs = 0, n_tokens = 0, n_entries = 0, n_rows = 0;
     int n_items[kMaxLists][kKinds] = {};
     std::vector<PagedItem> scratch;
+    int rows_step = 128;
     std::vector<int> page_owner;  // stamp of the sequence whose new rows a page receives
     int stamp = 0;
 
@@ -187,36 +189,51 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
     return best;
 }
 
-// The same for the tcgen05 kernel, in 128-key tiles of a pair of query tiles: `tiles` of every pair, of all KV heads. A step over
-// a tile takes 0.75 us, an item 3 us besides (its start, its epilogue), and cutting at all costs the merge.
-int choose_tc_piece(const std::vector<int>& tiles, int sm_count, size_t max_pieces) {
-    int64_t total = 0;
-    int longest = 1;
-    for (int n : tiles) {
-        total += n;
-        longest = std::max(longest, n);
-    }
-    int best = longest;
+// The same for the tcgen05 kernel. `tiles`: 128-key tiles of every pair of query tiles, longest first, of which each stands for Hkv
+// items. Items are taken longest first by whichever SM is free, so that only the last ones matter: those after the last whole
+// wave are cut, so far that the SMs end together. A step over a tile takes `t` us, an item 3 us besides (its start, its
+// epilogue), a piece's rows one more, and the merge 4. Returns how many pairs stay whole; *piece: the size of the others' pieces.
+int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, double t, int* piece) {
+    const int n = (int)tiles.size();
+    int best_whole = n;
     double best_cost = -1.0;
-    auto consider = [&](int piece) {
-        int64_t items = 0, cut = 0;
-        for (int n : tiles) {
-            const int k = (n + piece - 1) / piece;
-            items += k;
-            if (k > 1) cut += k;
+    std::vector<double> ends;
+    auto consider = [&](int whole, int size) {
+        size_t cut = 0;
+        for (int i = whole; i < n; ++i) cut += (tiles[i] + size - 1) / size * Hkv;
+        if (cut > max_pieces) return;
+        // (a heap of the times at which the SMs are free)
+        ends.assign(sm_count, 0.0);
+        double last = 0.0;
+        auto add = [&](double d) {
+            std::pop_heap(ends.begin(), ends.end(), std::greater<double>());
+            last = std::max(last, ends.back() += d);
+            std::push_heap(ends.begin(), ends.end(), std::greater<double>());
+        };
+        for (int i = 0; i < whole; ++i)
+            for (int h = 0; h < Hkv; ++h) add(3.0 + tiles[i] * t);
+        for (int i = whole; i < n; ++i) {
+            const int k = (tiles[i] + size - 1) / size;
+            for (int h = 0; h < Hkv * k; ++h) add(4.0 + (double)((tiles[i] + k - 1) / k) * t);
         }
-        if ((size_t)cut > max_pieces) return;
-        const double t0 = 3.0, t = 0.75, one = t0 + piece * t;
-        double cost = items <= sm_count ? one : std::max(one, (total * t + items * t0) / sm_count + 0.5 * one);
-        if (cut) cost += 4.0;
+        const double cost = last + (whole < n ? 4.0 : 0.0);
         if (best_cost < 0.0 || cost < best_cost) {
             best_cost = cost;
-            best = piece;
+            best_whole = whole;
+            *piece = size;
         }
     };
-    consider(longest);
-    for (int k = 2; k <= 32 && longest / k >= 3; ++k) consider((longest + k - 1) / k);
-    return best;
+    *piece = 1;
+    if (!n || (int64_t)n * Hkv > 8 * sm_count) return n;
+    consider(n, 1);
+    const int waves = (int)((int64_t)n * Hkv / sm_count);
+    for (int w = waves; w >= std::max(0, waves - 1); --w) {
+        const int whole = (int)((int64_t)w * sm_count / Hkv);
+        if (whole >= n) continue;
+        for (int k : {2, 3, 4, 5, 6, 8, 12, 16})
+            if (tiles[whole] / k >= 2) consider(whole, (tiles[whole] + k - 1) / k);
+    }
+    return best_whole;
 }
 
 int first_key(int pos, int window) { return window > 0 ? std::max(0, pos + 1 - window) : 0; }
@@ -370,8 +387,10 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     // items: row tiles of the longest plan, and the pieces that cutting them may add
     const size_t rows = (size_t)max_tokens * p.G, lists = b->windows.size();
     b->part_tiles = (size_t)(8 * p.sm_count + p.Hkv - 1) / p.Hkv + 16;
-    b->item_cap[kSplitK] = (rows + 15) / 16 + max_seqs + b->part_tiles;
-    b->item_cap[kRows] = (rows + 127) / 128 + max_seqs;
+    const size_t step = dtype == GGR_DTYPE_F32 ? 8 : 16;
+    b->rows_step = dtype == GGR_DTYPE_F32 && p.D == 256 ? 64 : 128;
+    b->item_cap[kSplitK] = (rows + step - 1) / step + max_seqs + b->part_tiles;
+    b->item_cap[kRows] = (rows + b->rows_step - 1) / b->rows_step + max_seqs;
     b->tc = dtype == GGR_DTYPE_BF16 && p.D <= 128 && p.G <= 128;
     if (b->tc) {
         b->tc_tokens = 128 / p.G;
@@ -402,7 +421,7 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     bool ok = cudaMalloc((void**)&b->d_plan, b->bytes) == cudaSuccess && cudaMalloc((void**)&b->d_part, b->part_tiles * state) == cudaSuccess &&
               cudaMalloc((void**)&b->d_tickets, b->part_tiles * p.Hkv * sizeof(unsigned)) == cudaSuccess;
     if (ok && !pages && dtype == GGR_DTYPE_F32)
-        ok = cudaMalloc((void**)&b->d_planes, (size_t)4 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
+        ok = cudaMalloc((void**)&b->d_planes, (size_t)6 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
     if (ok && b->tc)
         ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 256 * (p.D + 2) * sizeof(float)) == cudaSuccess &&
              cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
@@ -573,11 +592,10 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
                 for (int t = 0; t < q_len[i]; t += 2 * b->tc_tokens) {
                     const int lo = first_key(first + t, window) & ~127, hi = std::min(first + t + 2 * b->tc_tokens, kv_len[i]);
                     tiles[kTc].push_back({i, t, 0, lo, hi});
-                    for (int k = 0; k < b->Hkv; ++k) pair_tiles.push_back((hi - lo + 127) / 128);
                 }
                 continue;
             }
-            const int step = kind[i] == kRows ? 128 : 16;
+            const int step = kind[i] == kRows ? b->rows_step : (f32 ? 8 : 16);  // rows of a tile of the kernel
             for (int r = 0; r < n_rows; r += step) {
                 const int m = std::min(step, n_rows - r);
                 const int lo = first_key(first + r / b->G, window), hi = first + (r + m - 1) / b->G + 1;
@@ -589,7 +607,7 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
             PagedItem* items = reinterpret_cast<PagedItem*>(h + b->at_items[l][k]);
             int n = 0, part = 0, ticket = 0, longest = 1;
             const int piece = k == kSplitK && !tiles[k].empty()
-                                  ? choose_piece(tiles[k], b->Hkv, b->sm_count, tile_bytes, q8 || f32 ? 40e9 : 65e9, b->D == 256 ? 4 : 8, b->part_tiles, &longest)
+                                  ? choose_piece(tiles[k], b->Hkv, b->sm_count, tile_bytes, q8 || f32 ? 40e9 : 65e9, paged_splitk_warps(b->D, q8 ? kKvQ8Head : KV_BF16, f32), b->part_tiles, &longest)
                                   : 1 << 27;
             std::stable_sort(tiles[k].begin(), tiles[k].end(), [](const Tile& x, const Tile& y) { return x.key1 - x.key0 > y.key1 - y.key0; });
             for (const Tile& t : tiles[k]) {
@@ -620,11 +638,15 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
         }
         {
             PagedItem* merge = reinterpret_cast<PagedItem*>(h + b->at_items[l][kMerge]);
-            const int piece = pair_tiles.empty() ? 1 : choose_tc_piece(pair_tiles, b->sm_count, b->tc_parts);
-            int n = 0, n_merge = 0, part = 0;
+            auto n_tiles = [](const Tile& t) { return (t.key1 - t.key0 + 127) / 128; };
+            std::stable_sort(tiles[kTc].begin(), tiles[kTc].end(), [&](const Tile& x, const Tile& y) { return n_tiles(x) > n_tiles(y); });
+            for (const Tile& t : tiles[kTc]) pair_tiles.push_back(n_tiles(t));
+            int n = 0, n_merge = 0, part = 0, piece = 1;
+            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, q8 ? 4.0 : 2.4, &piece);
             b->scratch.clear();
             for (const Tile& t : tiles[kTc]) {
-                const int nt = (t.key1 - t.key0 + 127) / 128, cuts = std::max(1, (nt + piece - 1) / piece), each = (nt + cuts - 1) / cuts;
+                const bool cut = &t - tiles[kTc].data() >= whole;
+                const int nt = n_tiles(t), cuts = cut ? (nt + piece - 1) / piece : 1, each = (nt + cuts - 1) / cuts;
                 PagedItem it{};
                 it.tok0 = seqs[t.seq].tok0;
                 it.pos0 = kv_len[t.seq] - q_len[t.seq];
@@ -809,7 +831,7 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
             static KernelSmemSetup setup;
             PAGED_TRY(c, setup.ensure(paged_rows_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
             PathTimer t(c, 0);
-            paged_rows_kernel<D, FMT, F32><<<grid, 288, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
+            paged_rows_kernel<D, FMT, F32><<<grid, S::THREADS, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
         }
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
@@ -1015,16 +1037,16 @@ extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer
     const int list = b->list_of[layer];
     if (f32) {
         const int64_t plane = (int64_t)b->max_tokens * kv_dim;
-        __nv_bfloat16 *kp = b->d_planes, *vp = b->d_planes + 2 * plane;
+        __nv_bfloat16 *kp = b->d_planes, *vp = b->d_planes + 3 * plane;
         a.plane_rows = b->max_tokens;
         const uint64_t sy = (uint64_t)b->D * 2, sz = (uint64_t)kv_dim * 2;
-        if (!make_map3(&tk, false, kp, b->D, b->Hkv, (uint64_t)2 * b->max_tokens, sy, sz, 64, 1, 16) ||
-            !make_map3(&tv, false, vp, b->D, b->Hkv, (uint64_t)2 * b->max_tokens, sy, sz, 64, 1, 16))
+        if (!make_map3(&tk, false, kp, b->D, b->Hkv, (uint64_t)3 * b->max_tokens, sy, sz, 64, 1, 16) ||
+            !make_map3(&tv, false, vp, b->D, b->Hkv, (uint64_t)3 * b->max_tokens, sy, sz, 64, 1, 16))
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
         {
             PathTimer t(c, 1);
             paged_planes_kernel<<<dim3((unsigned)(((int64_t)rows * kv_dim / 4 + 255) / 256), 2), 256, 0, p.stream>>>(
-                static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, rows, kv_dim, kp, vp, plane);
+                static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, b->counts(0, 0), kv_dim, kp, vp, plane);
         }
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);

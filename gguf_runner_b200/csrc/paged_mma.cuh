@@ -9,9 +9,16 @@
 //    tile. Bound by the bytes of the cache: for a few tokens times G heads every cache byte is read once.
 //  - paged_rows_kernel: eight warps with 16 rows each walk the same keys through one ring, which a ninth warp fills.
 //
-// Precision. bf16 rows: q and codes are exact operands, softmax weights (times the scale of an 8-bit row) are rounded once to
-// bf16. f32 rows: q and the weights go in as two bf16 parts (the 2^-17 left out is below what the sums lose), f32 keys and
-// values as two bf16 planes, products of two low parts left out.
+// Precision. bf16 rows: q is an exact operand, softmax weights are rounded once to bf16. f32 rows: q and the weights go in as
+// three bf16 parts (24 bits), f32 keys and values as three bf16 planes, of which the products up to the weight of 2^-16 are
+// taken (six of nine; the others are below an f32 rounding). Two parts (16 bits) were measured first: 3.9e-6 from 64 bits
+// (2-norm) instead of 2e-7.
+// 8-bit pages: f16 operands, in which a code is exact and costs two instructions per pair instead of four in bf16. A row of q is
+// brought to [1, 2) by a power of two; a weight (at most 4, the reference maximum being at most two powers of two behind) times
+// the scale of V is taken relative to the largest such scale so far and times 2^13, so that f16 reaches 2^-38 of the largest
+// term. bf16 rows: one f16 part (11 bits); f32 rows: two (22 bits).
+// In split-K form f32 tiles have eight rows, and the other eight of the tensor core's sixteen hold the second part: one or two
+// instructions per product instead of two or three, and both halves of a row lie in one lane.
 //
 // Keys that only some rows of a tile see get weight 0, and 0 times an infinity or NaN in a value would spoil the other rows:
 // a row whose result is not finite is computed again, key by key, by paged_row_again. Rows of a tile that nobody sees
@@ -27,7 +34,7 @@ namespace ggr {
 constexpr int kPagedSplitMax = 128;  // pieces of one row tile
 
 struct PagedAttnArgs {
-    PageView pages;          // fmt also for packed rows: KV_BF16 (one plane), KV_F32 (two bf16 planes)
+    PageView pages;          // fmt also for packed rows: KV_BF16 (one plane), KV_F32 (three bf16 planes)
     PlanView plan;
     int paged;               // 0: keys are rows of packed k / v
     int layer, Hq, G, window;
@@ -91,27 +98,32 @@ __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const Paged
     }
 }
 
-// FMT: KV_BF16, kKvQ8Head, or KV_F32 = two bf16 planes. F32: rows in two bf16 parts.
-template <int D, int FMT, bool F32>
+// FMT: KV_BF16, kKvQ8Head, or KV_F32 = three bf16 planes. F32: rows in several parts; PACK: the first two of them in one
+// fragment of eight rows, the third in another.
+template <int D, int FMT, bool F32, bool PACK, bool QSMEM>
 struct PagedMma {
+    static_assert(F32 || !PACK, "bf16 rows have one part");
     static constexpr bool Q8 = FMT == kKvQ8Head, PLANES = FMT == KV_F32;
-    static constexpr int NP = F32 ? 2 : 1;
+    static constexpr int NP = !F32 ? 1 : (Q8 ? 2 : 3) - (PACK ? 1 : 0);  // fragments per product
+    static constexpr int PL = PLANES ? 3 : 1;
+    static constexpr int ROWS = PACK ? 8 : 16;
     static constexpr int ROW = Q8 ? D : 2 * D;                    // bytes of a cache row
     static constexpr int BOX = ROW < 128 ? ROW : 128;             // bytes of a row in one swizzled block
     static constexpr int NBLK = ROW / BOX;
     static constexpr uint32_t BLK = 16 * BOX;
     static constexpr uint32_t MAT = NBLK * BLK;                   // 16 rows of K or V
-    static constexpr uint32_t TILE = (PLANES ? 4 : 2) * MAT;      // K [K low] V [V low]
-    static constexpr uint32_t V0 = (PLANES ? 2 : 1) * MAT;
-    static constexpr uint32_t TX = TILE + (Q8 ? 128 : 0);
+    static constexpr uint32_t TILE = 2 * PL * MAT;                // planes of K, planes of V
+    static constexpr uint32_t V0 = PL * MAT;
     static constexpr int KS = D / 16, NT = D / 8;
-    static constexpr bool QSMEM = D == 256;                       // q fragments in shared memory: 128 registers of o leave no room
-    static constexpr uint32_t QBYTES = QSMEM ? NP * KS * 512 : 0; // of 16 rows
+    static constexpr uint32_t QBYTES = QSMEM ? NP * KS * 512 : 0; // q fragments in shared memory, where registers are short
 
     uint32_t qf[QSMEM ? 1 : NP][QSMEM ? 1 : KS][4];
     uint32_t q_smem;
     float o[NT][4];
     float m0, m1, l0, l1;
+    float c0, c1, t0, t1;  // per row: factor of its scores (with the power of two that its q was divided by), lazy threshold
+    float q0, q1;          // that power of two
+    float u0, u1;          // 8-bit: largest scale of V so far as a power of two; o is in units of u * 2^-13
 
     // The 16-byte piece `c` of row `r` in a block: 128-byte rows are XORed by row & 7, 64-byte rows (two to a 128-byte line)
     // by (row / 2) & 3.
@@ -125,9 +137,10 @@ struct PagedMma {
         for (int nt = 0; nt < NT; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.0f;
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.0f;
+        u0 = u1 = 0x1p-100f;
     }
 
-    // Fragments of rows r0 .. r0 + 15 (zeros from r1 on). Of 8-bit keys a lane holds four consecutive elements of a row, and
+    // Fragments of rows r0 .. r0 + ROWS - 1 (zeros from r1 on). Of 8-bit keys a lane holds four consecutive elements of a row, and
     // the elements of q are taken in that order; the order of the sum does not matter as long as both sides have the same.
     __device__ __forceinline__ void load_q(const PagedAttnArgs& a, const PagedItem& w, int kvh, int r0, int r1, int lane, uint32_t smem) {
         const int gq = lane >> 2, tq = lane & 3;
@@ -137,23 +150,45 @@ struct PagedMma {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = r0 + gq + 8 * i, tok = r / a.G;
-            ok[i] = r < r1;
+            ok[i] = r < r1 && !(PACK && i);
             at[i] = (w.tok0 + tok) * a.q_stride + (int64_t)(kvh * a.G + r - tok * a.G) * D;
         }
+        float by[2] = {1.0f, 1.0f};
+        if constexpr (Q8) {
+            float top[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < (PACK ? 1 : 2); ++i) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float2 x = ok[i] ? load2(a.q, at[i] + ks * 16 + tq * 4 + half * 2) : make_float2(0.f, 0.f);
+                        top[i] = fmaxf(top[i], fmaxf(fabsf(x.x), fabsf(x.y)));
+                    }
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                by[i] = __uint_as_float(0x7f000000u - (min(max(__float_as_uint(top[i]), 0x00800000u), 0x7e800000u) & 0x7f800000u));
+            }
+        }
+        q0 = 1.0f / by[0];
+        q1 = 1.0f / by[1];
+        c0 = a.c * q0;
+        c1 = a.c * q1;
+        t0 = (Q8 ? 2.0f : 8.0f) / c0;
+        t1 = (Q8 ? 2.0f : 8.0f) / c1;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            uint32_t f[NP][4];
+            uint32_t f[NP][4] = {};
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < (PACK ? 1 : 2); ++i)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int d = ks * 16 + (Q8 ? tq * 4 + half * 2 : tq * 2 + half * 8);
-                    const int reg = i + 2 * half;
-                    if constexpr (!F32) {
-                        f[0][reg] = ok[i] ? *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + at[i] + d) : 0u;
+                    if constexpr (!F32 && !Q8) {
+                        f[0][i + 2 * half] = ok[i] ? *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + at[i] + d) : 0u;
                     } else {
-                        const float2 x = ok[i] ? *reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + at[i] + d) : make_float2(0.f, 0.f);
-                        split2(x.x, x.y, f[0][reg], f[NP - 1][reg]);
+                        const float2 x = ok[i] ? load2(a.q, at[i] + d) : make_float2(0.f, 0.f);
+                        put(x.x * by[i], x.y * by[i], f, i, half);
                     }
                 }
 #pragma unroll
@@ -169,18 +204,44 @@ struct PagedMma {
         }
     }
 
-    // x = hi + lo in bf16 pairs
-    static __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-        hi = pack_bf16x2(x, y);
-        lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+    static __device__ __forceinline__ float2 load2(const void* p, int64_t at) {
+        if constexpr (F32) return *reinterpret_cast<const float2*>(static_cast<const float*>(p) + at);
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p) + at);
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
     }
 
-    // Two of four int8 (selector picks their bytes) as a bf16 pair, exactly: with the sign bit aside a code is 0 .. 127, which
-    // the seven mantissa bits of 128 .. 255 hold; 128 (or, for a negative code, 256) is taken off again.
+    // A pair in its parts (bf16, or f16 for 8-bit pages), into the fragments of row i (0: gq, 1: gq + 8) and k half
+    static __device__ __forceinline__ void put(float x, float y, uint32_t (&f)[NP][4], int i, int half) {
+        if constexpr (Q8) {
+            const __half2 h = __floats2half2_rn(x, y);
+            f[0][PACK ? 2 * half : i + 2 * half] = *reinterpret_cast<const uint32_t*>(&h);
+            if constexpr (F32) {
+                const float2 g = __half22float2(h);
+                const __half2 l = __floats2half2_rn(x - g.x, y - g.y);
+                f[NP - 1][PACK ? 1 + 2 * half : i + 2 * half] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+            return;
+        }
+        const uint32_t h = pack_bf16x2(x, y);
+        const float x1 = x - __uint_as_float(h << 16), y1 = y - __uint_as_float(h & 0xffff0000u);
+        const uint32_t m = pack_bf16x2(x1, y1);
+        const uint32_t l = pack_bf16x2(x1 - __uint_as_float(m << 16), y1 - __uint_as_float(m & 0xffff0000u));
+        if constexpr (PACK) {
+            f[0][2 * half] = h;
+            f[0][1 + 2 * half] = m;
+            f[NP - 1][2 * half] = l;
+        } else if constexpr (F32) {
+            f[0][i + 2 * half] = h;
+            f[NP > 1 ? 1 : 0][i + 2 * half] = m;
+            f[NP - 1][i + 2 * half] = l;
+        }
+    }
+
+    // Two of four int8, offset to 0 .. 255 by the caller, as an f16 pair, exactly: the selector puts their bytes under the
+    // exponent of 1024 .. 1279, and 1024 + 128 is taken off.
     static __device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
-        const uint32_t x = __byte_perm(w, 0x43434343u, sel);
-        const uint32_t lo = x & 0xff7fff7fu, hi = x & 0xff80ff80u;
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+        const uint32_t x = __byte_perm(w, 0x64646464u, sel), off = 0xe480e480u;
+        const __half2 d = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off));
         return *reinterpret_cast<const uint32_t*>(&d);
     }
 
@@ -195,16 +256,65 @@ struct PagedMma {
     }
 
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
-        mma_bf16_16816(c, x[0], x[1], x[2], x[3], b0, b1);
+        if constexpr (Q8)
+            mma_f16_16816(c, x[0], x[1], x[2], x[3], b0, b1);
+        else
+            mma_bf16_16816(c, x[0], x[1], x[2], x[3], b0, b1);
     }
 
-    // One tile: K at `kt`, V at `kt + V0`, the scales of an 8-bit tile at ks16 / ks16 + 16. Rows gq and gq + 8 of the warp see
-    // the keys [lo_i, hi_i) of the tile's 16; whole: all rows see all of them.
-    __device__ __forceinline__ void step(uint32_t kt, const float* ks16, bool whole, int lo0, int hi0, int lo1, int hi1, float c, int lane) {
-        const int tq = lane & 3;
-        float sc[2][4];
+    // A tile's share of four elements of o. The tensor core adds into its accumulator by truncation, which over hundreds of tiles
+    // goes one way (3e-9 of o per tile measured): in f32 a tile is summed from zero and then added, rounded to nearest.
+    struct Sum {
+        float c[4];
+        __device__ __forceinline__ explicit Sum(const float (&o)[4]) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+            for (int i = 0; i < 4; ++i) c[i] = F32 ? 0.0f : o[i];
+        }
+        __device__ __forceinline__ void add_to(float (&o)[4]) const {
+            if constexpr (F32) {
+                tc::unpack_f32x2(tc::add_f32x2(tc::pack_f32x2(o[0], o[1]), tc::pack_f32x2(c[0], c[1])), o[0], o[1]);
+                tc::unpack_f32x2(tc::add_f32x2(tc::pack_f32x2(o[2], o[3]), tc::pack_f32x2(c[2], c[3])), o[2], o[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = c[i];
+            }
+        }
+    };
+
+    // Scales of an 8-bit tile for the keys of a lane: keys 2 tq, 2 tq + 1 and those plus 8.
+    struct Scales {
+        float2 k[2], v[2];
+        __device__ __forceinline__ void load(const float* ks, const float* vs, int tq) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                k[j] = *reinterpret_cast<const float2*>(ks + j * 8 + tq * 2);
+                v[j] = *reinterpret_cast<const float2*>(vs + j * 8 + tq * 2);
+            }
+        }
+    };
+
+    // The larger of u and the tile's scales of V that the row sees (sc[.][at], sc[.][at + 1]), as a power of two at least as large.
+    static __device__ __forceinline__ float top_scale(const float (&sc)[2][4], const float (&sv)[4], int at, float u) {
+        float x = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x = fmaxf(x, sc[j][at + i] == -INFINITY ? 0.0f : sv[2 * j + i]);
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        return fmaxf(u, __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0x7f800000u));
+    }
+
+    // One tile: K at `kt`, V at `kt + V0`. Rows gq and gq + 8 of the warp see the keys [lo_i, hi_i) of the tile's 16; whole: all rows see all of them.
+    __device__ __forceinline__ void step(uint32_t kt, const Scales& scales, bool whole, int lo0, int hi0, int lo1, int hi1, int lane) {
+        const int tq = lane & 3;
+        // f32: products of low parts have sums of their own, which spares the large ones two thirds of their (truncating) additions
+        float sc[2][4], lo[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+            lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.0f;
+        }
         if constexpr (!Q8) {
             const int row = (lane & 7) + ((lane >> 4) & 1) * 8, half = (lane >> 3) & 1;
 #pragma unroll
@@ -212,16 +322,14 @@ struct PagedMma {
                 uint32_t f[NP][4], b[4];
 #pragma unroll
                 for (int np = 0; np < NP; ++np) frag(np, ks, f[np]);
-                ldmatrix_x4(kt + piece(row, 2 * ks + half), b[0], b[1], b[2], b[3]);
 #pragma unroll
-                for (int np = 0; np < NP; ++np) {
-                    mma(sc[0], f[np], b[0], b[1]);
-                    mma(sc[1], f[np], b[2], b[3]);
-                }
-                if constexpr (PLANES) {
-                    ldmatrix_x4(kt + MAT + piece(row, 2 * ks + half), b[0], b[1], b[2], b[3]);
-                    mma(sc[0], f[0], b[0], b[1]);
-                    mma(sc[1], f[0], b[2], b[3]);
+                for (int pl = 0; pl < PL; ++pl) {
+                    ldmatrix_x4(kt + pl * MAT + piece(row, 2 * ks + half), b[0], b[1], b[2], b[3]);
+#pragma unroll
+                    for (int np = 0; np < NP - pl; ++np) {
+                        mma(np + pl ? lo[0] : sc[0], f[np], b[0], b[1]);
+                        mma(np + pl ? lo[1] : sc[1], f[np], b[2], b[3]);
+                    }
                 }
             }
         } else {
@@ -232,23 +340,38 @@ struct PagedMma {
                 uint32_t r[4];
                 ldmatrix_x4(kt + piece(row, 2 * i + half), r[0], r[1], r[2], r[3]);
 #pragma unroll
+                for (int k = 0; k < 4; ++k) r[k] ^= 0x80808080u;
+#pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) {
+                    const uint32_t x0 = codes2(r[k2], 0x4140), x1 = codes2(r[k2], 0x4342), y0 = codes2(r[2 + k2], 0x4140), y1 = codes2(r[2 + k2], 0x4342);
 #pragma unroll
                     for (int np = 0; np < NP; ++np) {
                         uint32_t f[4];
                         frag(np, 2 * i + k2, f);
-                        mma(sc[0], f, codes2(r[k2], 0x4140), codes2(r[k2], 0x4342));
-                        mma(sc[1], f, codes2(r[2 + k2], 0x4140), codes2(r[2 + k2], 0x4342));
+                        mma(np ? lo[0] : sc[0], f, x0, x1);
+                        mma(np ? lo[1] : sc[1], f, y0, y1);
                     }
                 }
+            }
+        }
+        if constexpr (NP > 1) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[j][i] += lo[j][i];
+        }
+        if constexpr (PACK) {  // the second parts of the lane's row
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                sc[j][0] += sc[j][2];
+                sc[j][1] += sc[j][3];
             }
         }
         float sv[4];  // scales of V for this lane's four keys
         if constexpr (Q8) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float2 k2 = *reinterpret_cast<const float2*>(ks16 + j * 8 + tq * 2);
-                const float2 v2 = *reinterpret_cast<const float2*>(ks16 + 16 + j * 8 + tq * 2);
+                const float2 k2 = scales.k[j], v2 = scales.v[j];
                 sc[j][0] *= k2.x;
                 sc[j][1] *= k2.y;
                 sc[j][2] *= k2.x;
@@ -267,50 +390,68 @@ struct PagedMma {
                     if (key < lo1 || key >= hi1) sc[j][2 + i] = -INFINITY;
                 }
         }
-        float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-        float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+        float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])), x1 = -INFINITY;
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        // the reference maximum moves only when it grows by more than a factor of 2^8: l and o stay exact, they use the same
-        const float thr = 8.0f / c;
-        const bool need0 = x0 > m0 + thr, need1 = x1 > m1 + thr;
-        if (__any_sync(0xffffffffu, need0 || need1)) {
-            const float f0 = need0 ? tc::ex2((m0 - x0) * c) : 1.0f, f1 = need1 ? tc::ex2((m1 - x1) * c) : 1.0f;
+        if constexpr (!PACK) {
+            x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        }
+        // the reference maximum moves only when it grows by more than the threshold: l and o stay exact, they use the same
+        const bool need0 = x0 > m0 + t0, need1 = !PACK && x1 > m1 + t1;
+        bool rescale = need0 || need1;
+        float v0 = u0, v1 = u1;  // the largest scale of V with this tile's
+        if constexpr (Q8) {
+            v0 = top_scale(sc, sv, 0, u0);
+            if constexpr (!PACK) v1 = top_scale(sc, sv, 2, u1);
+            rescale |= v0 > u0 || v1 > u1;
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+            float f0 = need0 ? tc::ex2((m0 - x0) * c0) : 1.0f, f1 = need1 ? tc::ex2((m1 - x1) * c1) : 1.0f;
             if (need0) m0 = x0;
             if (need1) m1 = x1;
             l0 *= f0;
             l1 *= f1;
+            if constexpr (Q8) {
+                f0 *= u0 / v0;
+                f1 *= u1 / v1;
+                u0 = v0;
+                u1 = v1;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 o[nt][0] *= f0;
                 o[nt][1] *= f0;
-                o[nt][2] *= f1;
-                o[nt][3] *= f1;
+                o[nt][2] *= PACK ? f0 : f1;
+                o[nt][3] *= PACK ? f0 : f1;
             }
         }
-        const float b0 = m0 == -INFINITY ? 0.0f : -m0 * c, b1 = m1 == -INFINITY ? 0.0f : -m1 * c;
-        uint32_t pf[NP][4];
+        const float b0 = m0 == -INFINITY ? 0.0f : -m0 * c0, b1 = m1 == -INFINITY ? 0.0f : -m1 * c1;
+        const float w0 = __uint_as_float(0x7f000000u + (13u << 23) - __float_as_uint(u0)), w1 = __uint_as_float(0x7f000000u + (13u << 23) - __float_as_uint(u1));
+        uint32_t pf[NP][4] = {};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             float p[4];
-            p[0] = tc::ex2(fmaf(sc[j][0], c, b0));
-            p[1] = tc::ex2(fmaf(sc[j][1], c, b0));
-            p[2] = tc::ex2(fmaf(sc[j][2], c, b1));
-            p[3] = tc::ex2(fmaf(sc[j][3], c, b1));
+            p[0] = tc::ex2(fmaf(sc[j][0], c0, b0));
+            p[1] = tc::ex2(fmaf(sc[j][1], c0, b0));
             l0 += p[0] + p[1];
-            l1 += p[2] + p[3];
+            if constexpr (!PACK) {
+                p[2] = tc::ex2(fmaf(sc[j][2], c1, b1));
+                p[3] = tc::ex2(fmaf(sc[j][3], c1, b1));
+                l1 += p[2] + p[3];
+            }
             if constexpr (Q8) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = p[i] == 0.0f ? 0.0f : p[i] * sv[2 * j + (i & 1)];  // (a hidden row's scale may be NaN)
+                for (int i = 0; i < (PACK ? 2 : 4); ++i)  // (a hidden row's scale may be anything)
+                    p[i] = p[i] == 0.0f ? 0.0f : p[i] * (sv[2 * j + (i & 1)] * (i < 2 ? w0 : w1));
             }
-            if constexpr (!F32) {
+            if constexpr (!F32 && !Q8) {
                 pf[0][2 * j] = pack_bf16x2(p[0], p[1]);
                 pf[0][2 * j + 1] = pack_bf16x2(p[2], p[3]);
             } else {
-                split2(p[0], p[1], pf[0][2 * j], pf[NP - 1][2 * j]);
-                split2(p[2], p[3], pf[0][2 * j + 1], pf[NP - 1][2 * j + 1]);
+                put(p[0], p[1], pf, 0, j);
+                if constexpr (!PACK) put(p[2], p[3], pf, 1, j);
             }
         }
         const uint32_t vt = kt + V0;
@@ -318,18 +459,19 @@ struct PagedMma {
             const int row = (lane & 7) + ((lane >> 3) & 1) * 8, half = (lane >> 4) & 1;
 #pragma unroll
             for (int n2 = 0; n2 < NT / 2; ++n2) {
-                uint32_t b[4];
-                ldmatrix_x4_trans(vt + piece(row, 2 * n2 + half), b[0], b[1], b[2], b[3]);
+                uint32_t b[PL][4];
 #pragma unroll
-                for (int np = 0; np < NP; ++np) {
-                    mma(o[2 * n2], pf[np], b[0], b[1]);
-                    mma(o[2 * n2 + 1], pf[np], b[2], b[3]);
+                for (int pl = 0; pl < PL; ++pl) ldmatrix_x4_trans(vt + pl * MAT + piece(row, 2 * n2 + half), b[pl][0], b[pl][1], b[pl][2], b[pl][3]);
+                Sum s0(o[2 * n2]), s1(o[2 * n2 + 1]);
+#pragma unroll
+                for (int k = NP * PL - 1; k >= 0; --k) {  // small products first
+                    const int np = k % NP, pl = k / NP;
+                    if (np + pl >= (NP > PL ? NP : PL)) continue;
+                    mma(s0.c, pf[np], b[pl][0], b[pl][1]);
+                    mma(s1.c, pf[np], b[pl][2], b[pl][3]);
                 }
-                if constexpr (PLANES) {
-                    ldmatrix_x4_trans(vt + MAT + piece(row, 2 * n2 + half), b[0], b[1], b[2], b[3]);
-                    mma(o[2 * n2], pf[0], b[0], b[1]);
-                    mma(o[2 * n2 + 1], pf[0], b[2], b[3]);
-                }
+                s0.add_to(o[2 * n2]);
+                s1.add_to(o[2 * n2 + 1]);
             }
         } else {
             // a transposed load of byte pairs: a lane gets elements 2 gq and 2 gq + 1 of a piece for keys 2 tq and 2 tq + 1; the
@@ -340,15 +482,20 @@ struct PagedMma {
                 uint32_t r[4];
                 ldmatrix_x4_trans(vt + piece(row, 2 * i + half), r[0], r[1], r[2], r[3]);
 #pragma unroll
+                for (int k = 0; k < 4; ++k) r[k] ^= 0x80808080u;
+#pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) {
                     const int nt = 2 * (2 * i + k2);
                     const uint32_t e0 = codes2(r[2 * k2], 0x4240), e1 = codes2(r[2 * k2 + 1], 0x4240);
                     const uint32_t d0 = codes2(r[2 * k2], 0x4341), d1 = codes2(r[2 * k2 + 1], 0x4341);
+                    Sum s0(o[nt]), s1(o[nt + 1]);
 #pragma unroll
-                    for (int np = 0; np < NP; ++np) {
-                        mma(o[nt], pf[np], e0, e1);
-                        mma(o[nt + 1], pf[np], d0, d1);
+                    for (int np = NP - 1; np >= 0; --np) {
+                        mma(s0.c, pf[np], e0, e1);
+                        mma(s1.c, pf[np], d0, d1);
                     }
+                    s0.add_to(o[nt]);
+                    s1.add_to(o[nt + 1]);
                 }
             }
         }
@@ -360,7 +507,26 @@ struct PagedMma {
         return nt * 8 + 2 * tq + i;
     }
 
+    // The rows' state as the merges take it: whole rows of o, maxima in units of q . k
     __device__ __forceinline__ void sum_rows() {
+        if constexpr (PACK) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[nt][0] += o[nt][2];
+                o[nt][1] += o[nt][3];
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[nt][0] *= u0 * 0x1p-13f;
+                o[nt][1] *= u0 * 0x1p-13f;
+                o[nt][2] *= u1 * 0x1p-13f;
+                o[nt][3] *= u1 * 0x1p-13f;
+            }
+            m0 *= q0;
+            m1 *= q1;
+        }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -370,7 +536,7 @@ struct PagedMma {
     // Requests the 16 keys from `key` on (a multiple of 16) into `dst`; one lane. Packed keys lie in their rows, paged ones in
     // page `page` of the pool.
     static __device__ __forceinline__ void request(const PagedAttnArgs& a, const CUtensorMap* tk, const CUtensorMap* tv, const PagedItem& w,
-                                                   int kvh, int key, int page, uint32_t dst, uint32_t scales, uint32_t bar) {
+                                                   int kvh, int key, int page, uint32_t dst, uint32_t bar) {
         if (a.paged) {
             const int in_page = key & ((1 << a.pages.page_log2) - 1);
             const int z = (a.layer * a.pages.n_pages + page) * a.pages.Hkv + kvh;
@@ -380,15 +546,10 @@ struct PagedMma {
                 tma_load_3d(dst + b * BLK, tk, x, in_page, z, bar);
                 tma_load_3d(dst + V0 + b * BLK, tv, x, in_page, z, bar);
             }
-            if constexpr (Q8) {
-                const int64_t row = ((int64_t)z << a.pages.page_log2) + in_page;
-                tc::bulk_load(scales, a.pages.ks + row, 64, bar);
-                tc::bulk_load(scales + 64, a.pages.vs + row, 64, bar);
-            }
         } else {
             const int z = w.src + key;
 #pragma unroll
-            for (int p = 0; p < (PLANES ? 2 : 1); ++p)
+            for (int p = 0; p < PL; ++p)
 #pragma unroll
                 for (int b = 0; b < NBLK; ++b) {
                     tma_load_3d(dst + p * MAT + b * BLK, tk, b * 64, kvh, z + p * a.plane_rows, bar);
@@ -401,7 +562,7 @@ struct PagedMma {
     static __device__ __forceinline__ void clear(uint32_t tile, int lo, int hi, int lane) {
         if constexpr (Q8) return;  // codes are finite, and step() drops the scales of what has no weight
         constexpr int per_row = ROW / 16;
-        for (int i = lane; i < 16 * per_row * (PLANES ? 2 : 1); i += 32) {
+        for (int i = lane; i < 16 * per_row * PL; i += 32) {
             const int plane = i / (16 * per_row), r = (i / per_row) & 15, p = i % per_row;
             if (r >= lo && r < hi) continue;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + V0 + plane * MAT + piece(r, p)), "r"(0u) : "memory");
@@ -419,32 +580,40 @@ __device__ __forceinline__ void paged_store4(const PagedAttnArgs& a, int64_t at,
 }
 __device__ __forceinline__ bool finite4(float4 x) { return isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w); }
 
+constexpr int paged_splitk_warps(int D, int fmt, bool f32) {
+    return D == 256 ? (fmt == kKvQ8Head ? 8 : 6) : (f32 || fmt == kKvQ8Head ? 12 : 8);
+}
+
 template <int D, int FMT, bool F32>
 struct PagedSplitKShape {
-    using M = PagedMma<D, FMT, F32>;
-    static constexpr int W = D == 256 ? 4 : 8;
-    static constexpr int NST = FMT == kKvQ8Head ? (D == 64 ? 6 : 4) : (D == 64 ? 4 : 3);
+    // Warps and ring stages. bf16 on bf16 streams at the memory's rate with eight warps; the others are bound by the latency of a
+    // warp's chain (load, expand codes, multiply, softmax, multiply), so that more warps count for more than deeper rings or
+    // fragments in registers. (16 conversations of 1310 to 20000 keys, 32/4 heads of 128, int8, f32 rows: WARPS_NOTE.)
+    static constexpr bool BUSY = F32 || FMT == kKvQ8Head;
+    using M = PagedMma<D, FMT, F32, F32, D == 256 || (D == 128 && BUSY)>;
+    static constexpr int R = M::ROWS;
+    static constexpr int W = paged_splitk_warps(D, FMT, F32);
+    static constexpr int NST = FMT == kKvQ8Head ? (D == 64 ? 6 : (D == 128 ? 4 : 2)) : (D == 64 ? 4 : (BUSY || D == 256 ? 2 : 3));
     static constexpr int LD = D + 8;
     static constexpr uint32_t RING = W * NST * M::TILE;
-    static constexpr uint32_t SCALES = FMT == kKvQ8Head ? W * NST * 128 : 0;
-    static constexpr uint32_t MERGE = W * 16 * LD * 4;
-    static constexpr uint32_t DATA = RING + SCALES > MERGE ? RING + SCALES : MERGE;  // the merge reuses the rings
+    static constexpr uint32_t MERGE = W * R * LD * 4;
+    static constexpr uint32_t DATA = RING > MERGE ? RING : MERGE;  // the merge reuses the rings
     static constexpr uint32_t SMEM = DATA + M::QBYTES + 1024;
 };
 
-// An item is 16 packed rows of one sequence (fewer at its end) and a stretch of keys; blockIdx.y is the KV head.
+// An item is 16 packed rows (f32: 8) of one sequence, fewer at its end, and a stretch of keys; blockIdx.y is the KV head.
 template <int D, int FMT, bool F32>
 __global__ void __launch_bounds__(PagedSplitKShape<D, FMT, F32>::W * 32, 1)
 paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttnArgs a) {
     using namespace tc;
     using S = PagedSplitKShape<D, FMT, F32>;
     using M = typename S::M;
-    constexpr int W = S::W, NST = S::NST, LD = S::LD;
+    constexpr int W = S::W, NST = S::NST, LD = S::LD, R = S::R;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t s_full[W][NST];
-    __shared__ float s_m[W][16], s_l[W][16];  // per warp, then weights of the warps
-    __shared__ float s_top[16], s_sum[16];
-    __shared__ float s_w[16][kPagedSplitMax];
+    __shared__ float s_m[W][R], s_l[W][R];  // per warp, then weights of the warps
+    __shared__ float s_top[R], s_sum[R];
+    __shared__ float s_w[R][kPagedSplitMax];
     __shared__ int s_abort, s_last, s_bad;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -452,9 +621,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     const uint32_t ring = base + warp * NST * M::TILE;
-    const uint32_t scales = base + S::RING + warp * NST * 128;
-    const float* scales_p = reinterpret_cast<const float*>(base_p + S::RING + warp * NST * 128);
-    float* acc = reinterpret_cast<float*>(base_p);  // [W][16][LD] after the rings have drained
+    float* acc = reinterpret_cast<float*>(base_p);  // [W][R][LD] after the rings have drained
     volatile int* abortp = &s_abort;
     if (tid == 0) s_abort = 0;
     if (lane == 0) {
@@ -477,19 +644,31 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             const int key = w.key0 + (warp + t * W) * 16;
             const uint32_t bar = smem_u32(&s_full[warp][stage]);
             const int page = a.paged ? a.plan.table[w.src + (key >> a.pages.page_log2)] : 0;
-            mbar_expect_tx(bar, M::TX);
-            M::request(a, &tmK, &tmV, w, kvh, key, page, ring + stage * M::TILE, scales + stage * 128, bar);
+            mbar_expect_tx(bar, M::TILE);
+            M::request(a, &tmK, &tmV, w, kvh, key, page, ring + stage * M::TILE, bar);
         };
+        // Scales come by ordinary loads, one tile ahead: as copies of 64 bytes each they cost the copy engine as much as the codes
+        typename M::Scales sc_now, sc_next;
+        auto fetch_scales = [&](int t) {
+            if constexpr (M::Q8) {
+                const int key = w.key0 + (warp + t * W) * 16;
+                const int64_t row = a.pages.row(a.layer, a.plan.table[w.src + (key >> a.pages.page_log2)], kvh, key & ((1 << a.pages.page_log2) - 1));
+                sc_next.load(a.pages.ks + row, a.pages.vs + row, tq);
+            }
+        };
+        if (mine > 0) fetch_scales(0);
         if (lane == 0)
             for (int t = 0; t < NST - 1 && t < mine; ++t) issue(t);
         M x;
         x.start();
         x.load_q(a, w, kvh, w.row0, w.row0 + w.rows, lane, base + S::DATA);
-        if constexpr (M::QSMEM) __syncthreads();  // (every warp has written the same fragments)
-        const int p0 = w.pos0 + min(w.row0 + gq, w.row0 + w.rows - 1) / a.G, p1 = w.pos0 + min(w.row0 + gq + 8, w.row0 + w.rows - 1) / a.G;
+        if constexpr (M::QBYTES > 0) __syncthreads();  // (every warp has written the same fragments)
+        const int p0 = w.pos0 + min(w.row0 + gq, w.row0 + w.rows - 1) / a.G, p1 = R == 16 ? w.pos0 + min(w.row0 + gq + 8, w.row0 + w.rows - 1) / a.G : p0;
         const int lo0 = paged_first_key(p0, a.window), lo1 = paged_first_key(p1, a.window);
         for (int t = 0; t < mine; ++t) {
             const uint32_t u = used + t, stage = u % NST;
+            sc_now = sc_next;
+            if (t + 1 < mine) fetch_scales(t + 1);
             if (!mbar_wait_warp(smem_u32(&s_full[warp][stage]), (u / NST) & 1u, abortp)) break;
             const int key = w.key0 + (warp + t * W) * 16;
             const uint32_t kt = ring + stage * M::TILE;
@@ -498,7 +677,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 M::clear(kt, any_lo - key, any_hi - key, lane);
                 __syncwarp();
             }
-            x.step(kt, scales_p + stage * 32, whole, lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, a.c, lane);
+            x.step(kt, sc_now, whole, lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, lane);
             __syncwarp();
             if (lane == 0 && t + NST - 1 < mine) {
                 fence_smem_to_async_proxy();
@@ -517,23 +696,26 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             if constexpr (FMT == kKvQ8Head) {
                 if (nt & 1) continue;  // an even and an odd n-tile make four consecutive elements
                 const int d = M::element(nt, 0, tq);
-                *reinterpret_cast<float4*>(&acc[(warp * 16 + gq) * LD + d]) = make_float4(x.o[nt][0], x.o[nt + 1][0], x.o[nt][1], x.o[nt + 1][1]);
-                *reinterpret_cast<float4*>(&acc[(warp * 16 + gq + 8) * LD + d]) = make_float4(x.o[nt][2], x.o[nt + 1][2], x.o[nt][3], x.o[nt + 1][3]);
+                *reinterpret_cast<float4*>(&acc[(warp * R + gq) * LD + d]) = make_float4(x.o[nt][0], x.o[nt + 1][0], x.o[nt][1], x.o[nt + 1][1]);
+                if constexpr (R == 16)
+                    *reinterpret_cast<float4*>(&acc[(warp * R + gq + 8) * LD + d]) = make_float4(x.o[nt][2], x.o[nt + 1][2], x.o[nt][3], x.o[nt + 1][3]);
             } else {
                 const int d = M::element(nt, 0, tq);
-                *reinterpret_cast<float2*>(&acc[(warp * 16 + gq) * LD + d]) = make_float2(x.o[nt][0], x.o[nt][1]);
-                *reinterpret_cast<float2*>(&acc[(warp * 16 + gq + 8) * LD + d]) = make_float2(x.o[nt][2], x.o[nt][3]);
+                *reinterpret_cast<float2*>(&acc[(warp * R + gq) * LD + d]) = make_float2(x.o[nt][0], x.o[nt][1]);
+                if constexpr (R == 16) *reinterpret_cast<float2*>(&acc[(warp * R + gq + 8) * LD + d]) = make_float2(x.o[nt][2], x.o[nt][3]);
             }
         }
         if (tq == 0) {
             s_m[warp][gq] = x.m0;
-            s_m[warp][gq + 8] = x.m1;
             s_l[warp][gq] = x.l0;
-            s_l[warp][gq + 8] = x.l1;
+            if constexpr (R == 16) {
+                s_m[warp][gq + 8] = x.m1;
+                s_l[warp][gq + 8] = x.l1;
+            }
         }
         if (tid == 0) s_bad = 0;
         __syncthreads();
-        if (tid < 16) {
+        if (tid < R) {
             float top = -INFINITY, sum = 0.0f;
             for (int i = 0; i < W; ++i) top = fmaxf(top, s_m[i][tid]);
             for (int i = 0; i < W; ++i) {
@@ -547,7 +729,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
         __syncthreads();
         const bool split = w.part >= 0;
-        constexpr int STATE = 16 * (D + 2);
+        constexpr int STATE = R * (D + 2);
         float* state0 = a.part + ((int64_t)(split ? w.part : 0) * a.pages.Hkv + kvh) * STATE;  // of the tile's first piece
         const int64_t state_step = (int64_t)a.pages.Hkv * STATE;
         float* mine_state = state0 + w.split * state_step;
@@ -557,7 +739,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
             for (int k = 0; k < W; ++k) {
                 const float f = s_m[k][r];
-                const float4 y = *reinterpret_cast<const float4*>(&acc[(k * 16 + r) * LD + d]);
+                const float4 y = *reinterpret_cast<const float4*>(&acc[(k * R + r) * LD + d]);
                 v.x = fmaf(f, y.x, v.x);
                 v.y = fmaf(f, y.y, v.y);
                 v.z = fmaf(f, y.z, v.z);
@@ -566,15 +748,15 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             if (split) {
                 __stcg(reinterpret_cast<float4*>(mine_state + r * D + d), v);
             } else {
-                const int R = w.row0 + r, tok = R / a.G;
+                const int row = w.row0 + r, tok = row / a.G;
                 const float inv = 1.0f / s_sum[r];
                 v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                 if (!finite4(v)) s_bad = 1;
-                paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + R - tok * a.G) * D + d, v);
+                paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D + d, v);
             }
         }
         if (split) {
-            if (tid < w.rows) __stcg(reinterpret_cast<float2*>(mine_state + 16 * D) + tid, make_float2(s_top[tid], s_sum[tid]));
+            if (tid < w.rows) __stcg(reinterpret_cast<float2*>(mine_state + R * D) + tid, make_float2(s_top[tid], s_sum[tid]));
             __syncthreads();
             if (tid == 0) {
                 __threadfence();
@@ -588,11 +770,11 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 for (int r = warp; r < w.rows; r += W) {
                     float top = -INFINITY;
                     for (int s = lane; s < w.n_split; s += 32)
-                        top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(state0 + s * state_step + 16 * D) + r).x);
+                        top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(state0 + s * state_step + R * D) + r).x);
                     top = warp_max(top);
                     float sum = 0.0f;
                     for (int s = lane; s < w.n_split; s += 32) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(state0 + s * state_step + 16 * D) + r);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(state0 + s * state_step + R * D) + r);
                         const float f = ml.x == -INFINITY ? 0.0f : ex2((ml.x - top) * a.c);
                         s_w[r][s] = f;
                         sum += ml.y == 0.0f ? 0.0f : f * ml.y;
@@ -613,11 +795,11 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                         v.z = fmaf(f, y.z, v.z);
                         v.w = fmaf(f, y.w, v.w);
                     }
-                    const int R = w.row0 + r, tok = R / a.G;
+                    const int row = w.row0 + r, tok = row / a.G;
                     const float inv = 1.0f / s_sum[r];
                     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     if (!finite4(v)) s_bad = 1;
-                    paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + R - tok * a.G) * D + d, v);
+                    paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D + d, v);
                 }
             }
         }
@@ -635,19 +817,22 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
 template <int D, int FMT, bool F32>
 struct PagedRowsShape {
-    using M = PagedMma<D, FMT, F32>;
-    static constexpr int W = 8;
-    static constexpr int SUB = FMT == KV_F32 && D == 256 ? 1 : 2;  // tiles of 16 keys in a stage
+    using M = PagedMma<D, FMT, F32, false, D == 256>;
+    static constexpr int W = D == 256 && F32 ? 4 : 8;  // 16 rows each (fragments of q in shared memory: 24 KB a warp there)
+    static constexpr int SUB = FMT == KV_F32 && D >= 128 ? 1 : 2;  // tiles of 16 keys in a stage
     static constexpr uint32_t STAGE = SUB * M::TILE;
     static constexpr int NST = STAGE >= 32768 ? 2 : 4;
     static constexpr uint32_t RING = NST * STAGE;
     static constexpr uint32_t SCALES = FMT == kKvQ8Head ? NST * SUB * 128 : 0;
     static constexpr uint32_t SMEM = RING + SCALES + W * M::QBYTES + 1024;
+    // consumer warpgroups and a control warpgroup, whose registers go to the others
+    static constexpr int THREADS = W * 32 + 128;
 };
 
-// An item is up to 128 packed rows of one sequence and all the keys that they see; blockIdx.y is the KV head.
+// An item is up to 128 packed rows (f32 at head_dim 256: 64) of one sequence and all the keys that they see; blockIdx.y is the KV
+// head.
 template <int D, int FMT, bool F32>
-__global__ void __launch_bounds__(288, 1)
+__global__ void __launch_bounds__(PagedRowsShape<D, FMT, F32>::THREADS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttnArgs a) {
     using namespace tc;
     using S = PagedRowsShape<D, FMT, F32>;
@@ -672,33 +857,43 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     __syncthreads();
     const int n_items = a.plan.counts[0];
-    uint32_t used = 0, raws = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-        const PagedItem w = a.plan.items[item];
-        const int n_stages = (w.key1 - w.key0 + KT - 1) / KT;
-        const int tok_lo = w.row0 / a.G, tok_hi = (w.row0 + w.rows - 1) / a.G;
-        const int any_lo = paged_first_key(w.pos0 + tok_lo, a.window), any_hi = w.pos0 + tok_hi + 1;
-        if (warp == S::W) {
-            for (int t = 0; t < n_stages; ++t) {
-                const uint32_t u = used + t, stage = u % NST;
-                if (!mbar_wait_warp(smem_u32(&s_empty[stage]), ((u / NST) & 1u) ^ 1u, abortp)) break;
+    uint32_t used = 0;  // stages gone through: ring position and phase
+    // keys that some row of an item sees
+    auto any_lo_of = [&](const PagedItem& w) { return paged_first_key(w.pos0 + w.row0 / a.G, a.window); };
+    auto any_hi_of = [&](const PagedItem& w) { return w.pos0 + (w.row0 + w.rows - 1) / a.G + 1; };
+    if (warp >= S::W) {
+        // control warpgroup: one producer warp, the others have no role
+        if constexpr (S::W == 8) reg_release<56>();
+        uint32_t raws = 0;
+        bool ok = warp == S::W;
+        for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
+            const PagedItem w = a.plan.items[item];
+            const int n_stages = (w.key1 - w.key0 + KT - 1) / KT, any_lo = any_lo_of(w), any_hi = any_hi_of(w);
+            for (int t = 0; t < n_stages; ++t, ++used) {
+                const uint32_t stage = used % NST;
+                if (!(ok = mbar_wait_warp(smem_u32(&s_empty[stage]), ((used / NST) & 1u) ^ 1u, abortp))) break;
                 const int key = w.key0 + t * KT;
                 const bool edge = key < any_lo || key + KT > any_hi;
                 const uint32_t bar = edge ? smem_u32(&s_raw) : smem_u32(&s_full[stage]);
-                const uint32_t dst = base + stage * S::STAGE, sc = base + S::RING + stage * SUB * 128;
+                const uint32_t dst = base + stage * S::STAGE, sc = base + S::RING + stage * SUB * 128;  // (scales: 16 of K, 16 of V per tile)
                 if (lane == 0) {
                     // tiles behind the last visible key have no page: they are left out, and step() is not called for them
                     const int subs = min(SUB, (any_hi - key + 15) >> 4);
-                    mbar_expect_tx(bar, subs * M::TX);
+                    mbar_expect_tx(bar, subs * (M::TILE + (M::Q8 ? 128 : 0)));
                     for (int i = 0; i < subs; ++i) {
                         const int k = key + 16 * i;
                         const int page = a.paged ? a.plan.table[w.src + (k >> a.pages.page_log2)] : 0;
-                        M::request(a, &tmK, &tmV, w, kvh, k, page, dst + i * M::TILE, sc + i * 128, bar);
+                        M::request(a, &tmK, &tmV, w, kvh, k, page, dst + i * M::TILE, bar);
+                        if constexpr (M::Q8) {
+                            const int64_t row = a.pages.row(a.layer, page, kvh, k & ((1 << a.pages.page_log2) - 1));
+                            bulk_load(sc + i * 128, a.pages.ks + row, 64, bar);
+                            bulk_load(sc + i * 128 + 64, a.pages.vs + row, 64, bar);
+                        }
                     }
                 }
                 __syncwarp();
                 if (edge) {
-                    if (!mbar_wait_warp(bar, raws & 1u, abortp)) break;
+                    if (!(ok = mbar_wait_warp(bar, raws & 1u, abortp))) break;
                     ++raws;
                     for (int i = 0; i < SUB; ++i) M::clear(dst + i * M::TILE, any_lo - key - 16 * i, any_hi - key - 16 * i, lane);
                     fence_smem_to_async_proxy();  // (this stage's next copy comes after the arrivals below and the readers')
@@ -706,8 +901,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                     if (lane == 0) mbar_arrive(smem_u32(&s_full[stage]));
                 }
             }
-            used += n_stages;
-        } else {
+        }
+    } else {
+        if constexpr (S::W == 8) reg_acquire<224>();
+        for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+            const PagedItem w = a.plan.items[item];
+            const int n_stages = (w.key1 - w.key0 + KT - 1) / KT;
             const int r0 = w.row0 + warp * 16, r1 = w.row0 + w.rows;  // this warp's rows, cut at r1
             const bool mine = r0 < r1;
             M x;
@@ -725,56 +924,57 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 all_hi = t0 + 1;
             }
             const int lo0 = paged_first_key(p0, a.window), lo1 = paged_first_key(p1, a.window);
-            for (int t = 0; t < n_stages; ++t) {
-                const uint32_t u = used + t, stage = u % NST;
-                if (!mbar_wait_warp(smem_u32(&s_full[stage]), (u / NST) & 1u, abortp)) break;
+            for (int t = 0; t < n_stages; ++t, ++used) {
+                const uint32_t stage = used % NST;
+                if (!mbar_wait_warp(smem_u32(&s_full[stage]), (used / NST) & 1u, abortp)) break;
 #pragma unroll 1
                 for (int i = 0; i < SUB; ++i) {
                     const int key = w.key0 + t * KT + 16 * i;
                     if (!mine || key >= see_hi || key + 16 <= see_lo) continue;
                     const bool whole = key >= all_lo && key + 16 <= all_hi;
-                    x.step(base + stage * S::STAGE + i * M::TILE, reinterpret_cast<const float*>(base_p + S::RING + (stage * SUB + i) * 128), whole,
-                           lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, a.c, lane);
+                    typename M::Scales scales;
+                    const float* sc = reinterpret_cast<const float*>(base_p + S::RING + (stage * SUB + i) * 128);
+                    if constexpr (M::Q8) scales.load(sc, sc + 16, tq);
+                    x.step(base + stage * S::STAGE + i * M::TILE, scales, whole,
+                           lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, lane);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
             }
-            used += n_stages;
-            if (mine && !*abortp) {
-                x.sum_rows();
-                const float i0 = 1.0f / x.l0, i1 = 1.0f / x.l1;
-                bool bad = false;
+            if (*abortp) break;
+            if (!mine) continue;
+            x.sum_rows();
+            const float i0 = 1.0f / x.l0, i1 = 1.0f / x.l1;
+            bool bad = false;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int R = r0 + gq + 8 * half, tok = R / a.G;
-                    if (R >= r1) continue;
-                    const int64_t at = (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + R - tok * a.G) * D;
-                    const float inv = half ? i1 : i0;
+            for (int half = 0; half < 2; ++half) {
+                const int row = r0 + gq + 8 * half, tok = row / a.G;
+                if (row >= r1) continue;
+                const int64_t at = (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D;
+                const float inv = half ? i1 : i0;
 #pragma unroll
-                    for (int nt = 0; nt < M::NT; ++nt) {
-                        if constexpr (FMT == kKvQ8Head) {
-                            if (nt & 1) continue;
-                            const float4 v = make_float4(x.o[nt][2 * half] * inv, x.o[nt + 1][2 * half] * inv, x.o[nt][2 * half + 1] * inv, x.o[nt + 1][2 * half + 1] * inv);
-                            bad |= !finite4(v);
-                            paged_store4<F32>(a, at + M::element(nt, 0, tq), v);
-                        } else {
-                            const float v0 = x.o[nt][2 * half] * inv, v1 = x.o[nt][2 * half + 1] * inv;
-                            bad |= !isfinite(v0) || !isfinite(v1);
-                            const int64_t to = at + M::element(nt, 0, tq);
-                            if constexpr (F32)
-                                *reinterpret_cast<float2*>(static_cast<float*>(a.out) + to) = make_float2(v0, v1);
-                            else
-                                *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + to) = pack_bf16x2(v0, v1);
-                        }
+                for (int nt = 0; nt < M::NT; ++nt) {
+                    if constexpr (FMT == kKvQ8Head) {
+                        if (nt & 1) continue;
+                        const float4 v = make_float4(x.o[nt][2 * half] * inv, x.o[nt + 1][2 * half] * inv, x.o[nt][2 * half + 1] * inv, x.o[nt + 1][2 * half + 1] * inv);
+                        bad |= !finite4(v);
+                        paged_store4<F32>(a, at + M::element(nt, 0, tq), v);
+                    } else {
+                        const float v0 = x.o[nt][2 * half] * inv, v1 = x.o[nt][2 * half + 1] * inv;
+                        bad |= !isfinite(v0) || !isfinite(v1);
+                        const int64_t to = at + M::element(nt, 0, tq);
+                        if constexpr (F32)
+                            *reinterpret_cast<float2*>(static_cast<float*>(a.out) + to) = make_float2(v0, v1);
+                        else
+                            *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + to) = pack_bf16x2(v0, v1);
                     }
                 }
-                if (__any_sync(0xffffffffu, bad)) {
-                    __syncwarp();
-                    for (int r = r0; r < min(r0 + 16, r1); ++r) paged_row_again<D, F32>(a, w, kvh, r, lane);
-                }
+            }
+            if (__any_sync(0xffffffffu, bad)) {
+                __syncwarp();
+                for (int r = r0; r < min(r0 + 16, r1); ++r) paged_row_again<D, F32>(a, w, kvh, r, lane);
             }
         }
-        if (*abortp) break;
     }
     if (s_abort) {
         for (int i = 0; i < 500; ++i) __nanosleep(1000);  // let copies in flight land
@@ -783,19 +983,20 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (tid == 0 && s_abort && a.err) atomicExch(a.err, 1);
 }
 
-// f32 rows of k or v as two bf16 planes: x = hi + lo. Rows of `dim` elements, four per thread.
-__global__ void __launch_bounds__(256) paged_planes_kernel(const float* k, const float* v, int64_t k_stride, int64_t v_stride, int rows, int dim,
+// f32 rows of k or v as three bf16 planes: x = h + m + l. Rows of `dim` elements, four per thread; `counts` holds the rows in use.
+__global__ void __launch_bounds__(256) paged_planes_kernel(const float* k, const float* v, int64_t k_stride, int64_t v_stride, const int* counts, int dim,
                                                            __nv_bfloat16* kp, __nv_bfloat16* vp, int64_t plane) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= (int64_t)rows * dim) return;
+    if (i >= (int64_t)counts[2] * dim) return;
     const int64_t r = i / dim, d = i - r * dim;
-    const float4 x = *reinterpret_cast<const float4*>((blockIdx.y ? v + r * v_stride : k + r * k_stride) + d);
-    const uint32_t h0 = pack_bf16x2(x.x, x.y), h1 = pack_bf16x2(x.z, x.w);
-    const uint32_t l0 = pack_bf16x2(x.x - __uint_as_float(h0 << 16), x.y - __uint_as_float(h0 & 0xffff0000u));
-    const uint32_t l1 = pack_bf16x2(x.z - __uint_as_float(h1 << 16), x.w - __uint_as_float(h1 & 0xffff0000u));
+    float4 x = *reinterpret_cast<const float4*>((blockIdx.y ? v + r * v_stride : k + r * k_stride) + d);
     __nv_bfloat16* to = (blockIdx.y ? vp : kp) + i;
-    *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
-    *reinterpret_cast<uint2*>(to + plane) = make_uint2(l0, l1);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t a = pack_bf16x2(x.x, x.y), b = pack_bf16x2(x.z, x.w);
+        *reinterpret_cast<uint2*>(to + p * plane) = make_uint2(a, b);
+        x = make_float4(x.x - __uint_as_float(a << 16), x.y - __uint_as_float(a & 0xffff0000u), x.z - __uint_as_float(b << 16), x.w - __uint_as_float(b & 0xffff0000u));
+    }
 }
 
 }  // namespace ggr

@@ -77,9 +77,6 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ void lds_f32x4(uint32_t at, uint64_t& lo, uint64_t& hi) {
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(at));
-}
 
 // SCALED: rows are codes, with scales beside them.
 template <int D, bool SCALED>
@@ -354,7 +351,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 vs = paged_first_key(w.pos0 + tok, a.window);
             }
             float m_used = -INFINITY, l = 0.0f;
-            const uint32_t scales = sOut + (uint32_t)warp * 4096u;  // 128 of K, 128 of V
+            unsigned char* scales_p = smem_raw + (sOut - smem_u32(smem_raw)) + warp * 4096;  // 128 of K, 128 of V
             float4 next_ks, next_vs;
             auto fetch_scales = [&](int j) {
                 const int key = j * 128 + lane * 4;
@@ -373,10 +370,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const int k = j - lo_t;
                 if constexpr (SCALED) {
                     __syncwarp();
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales + lane * 16), "f"(next_ks.x), "f"(next_ks.y), "f"(next_ks.z),
-                                 "f"(next_ks.w) : "memory");
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scales + 512 + lane * 16), "f"(next_vs.x), "f"(next_vs.y), "f"(next_vs.z),
-                                 "f"(next_vs.w) : "memory");
+                    reinterpret_cast<float4*>(scales_p)[lane] = next_ks;
+                    reinterpret_cast<float4*>(scales_p + 512)[lane] = next_vs;
                     __syncwarp();
                     if (j + 1 < hi_t) fetch_scales(j + 1);
                 }
@@ -391,8 +386,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int cidx = 0; cidx < 4; ++cidx)
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            uint64_t k01, k23;
-                            lds_f32x4(scales + (cidx * 32 + i) * 4, k01, k23);
+                            const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(scales_p + (cidx * 32 + i) * 4);
+                            const uint64_t k01 = k4.x, k23 = k4.y;
                             float x0, x1, x2, x3;
                             unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1])), k01), x0, x1);
                             unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3])), k23), x2, x3);
@@ -467,8 +462,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         sum_a = add_f32x2(sum_a, pack_f32x2(p0, p1));
                         sum_b = add_f32x2(sum_b, pack_f32x2(p2, p3));
                         if constexpr (SCALED) {
-                            uint64_t v01, v23;
-                            lds_f32x4(scales + 512 + (cidx * 32 + 2 * i) * 4, v01, v23);
+                            const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(scales_p + 512 + (cidx * 32 + 2 * i) * 4);
+                            const uint64_t v01 = v4.x, v23 = v4.y;
                             unpack_f32x2(mul_f32x2(pack_f32x2(p0, p1), v01), p0, p1);
                             unpack_f32x2(mul_f32x2(pack_f32x2(p2, p3), v23), p2, p3);
                         }

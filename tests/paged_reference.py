@@ -57,10 +57,13 @@ def bound(dtype, out, size, reach):
     """How far a result may be from the 64-bit one, element by element.
 
     bf16: the result and each softmax weight are rounded once, by at most 2^-8 of their value.
-    f32: q (and packed k, v) and the weights are taken in two bf16 parts, which leave out at most 2^-16 of a value, as do the
-    dropped products of two low parts: a score is off by at most 3 * 2^-16 * reach, a weight by twice that share (its own and
-    the sum's) and 2^-16, a value by 2^-16 twice. Both: 2^-20 for exponentials, sums and the order they are taken in.
+    f32: q (and packed k, v) and the weights are taken in three bf16 parts, which leave out at most 2^-24 of a value; of the nine
+    products of two such values the three smallest are dropped, at most 2 * 2^-24 + 2^-32 of the whole: a score is off by less
+    than 5 * 2^-24 * reach, a weight by twice that share (its own and the sum's) and 2^-24, a value by 3 * 2^-24.
+    Over 8-bit pages: two f16 parts (of values brought next to 1), which leave out at most 2^-22: a score is off by 2^-22 * reach,
+    a weight by twice that share and 2^-22; codes are exact.
+    All: 2^-20 for exponentials, sums and the order they are taken in.
     """
     if dtype == torch.bfloat16:
         return 2.0 ** -8 * (out.abs() + size) * 1.01 + 2.0 ** -20 * (1 + reach) * size
-    return (6 * reach + 4) * 2.0 ** -16 * size + 2.0 ** -20 * (1 + reach) * size
+    return (10 * reach + 4) * 2.0 ** -24 * size + (2 * reach + 1) * 2.0 ** -22 * size + 2.0 ** -20 * (1 + reach) * size
