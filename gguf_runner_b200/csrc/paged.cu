@@ -95,9 +95,9 @@ struct ggr_batch {
     size_t tc_parts = 0;        // its partial states
     float* d_tc_part = nullptr;
     int* d_sched = nullptr;
-    // 8-bit pages on their way to the tcgen05 kernel: dense bf16 rows, and which pages go there
-    __nv_bfloat16* d_dense = nullptr;
-    float* d_dense_scales = nullptr;
+    // 8-bit pages on their way to the tcgen05 kernel: dense f16 rows and which pages go there, q in f16
+    __half* d_dense = nullptr;
+    __half* d_q16 = nullptr;
     size_t dense_rows = 0;
     CUtensorMap tmKd, tmVd;
     size_t at_dense_entries = 0, at_dense_table = 0;
@@ -191,9 +191,10 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
 
 // The same for the tcgen05 kernel. `tiles`: 128-key tiles of every pair of query tiles, longest first, of which each stands for Hkv
 // items. Items are taken longest first by whichever SM is free, so that only the last ones matter: those after the last whole
-// wave are cut, so far that the SMs end together. A step over a tile takes `t` us, an item 3 us besides (its start, its
+// wave are cut, so far that the SMs end together. A step over a tile takes 2.4 us, an item 3 us besides (its start, its
 // epilogue), a piece's rows one more, and the merge 4. Returns how many pairs stay whole; *piece: the size of the others' pieces.
-int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, double t, int* piece) {
+int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, int* piece) {
+    constexpr double t = 2.4;
     const int n = (int)tiles.size();
     int best_whole = n;
     double best_cost = -1.0;
@@ -344,7 +345,7 @@ extern "C" void ggr_batch_destroy(ggr_batch* b) {
     cudaFree(b->d_tc_part);
     cudaFree(b->d_sched);
     cudaFree(b->d_dense);
-    cudaFree(b->d_dense_scales);
+    cudaFree(b->d_q16);
     delete b;
 }
 
@@ -425,6 +426,8 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     if (ok && b->tc)
         ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 256 * (p.D + 2) * sizeof(float)) == cudaSuccess &&
              cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
+    if (ok && b->tc && pages && pages->v.fmt == GGR_KV_Q8_HEAD)
+        ok = cudaMalloc((void**)&b->d_q16, (size_t)max_tokens * p.Hq * p.D * sizeof(__half)) == cudaSuccess;
     for (int i = 0; ok && i < 2; ++i)
         ok = cudaHostAlloc((void**)&b->h_plan[i], b->bytes, cudaHostAllocDefault) == cudaSuccess &&
              cudaEventCreateWithFlags(&b->up[i], cudaEventDisableTiming) == cudaSuccess;
@@ -541,21 +544,17 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
             if (b->d_dense) {
                 PAGED_TRY(c, cudaStreamSynchronize(p.stream));
                 cudaFree(b->d_dense);
-                cudaFree(b->d_dense_scales);
             }
             b->d_dense = nullptr;
-            b->d_dense_scales = nullptr;
             b->dense_rows = 0;
             const size_t want = (size_t)std::max<int64_t>(dense, 4096);
-            if (want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__nv_bfloat16)) == cudaSuccess &&
-                cudaMalloc((void**)&b->d_dense_scales, 2 * (want + 128) * b->Hkv * sizeof(float)) == cudaSuccess) {
+            if (want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__half)) == cudaSuccess) {
                 if (!make_map3(&b->tmKd, false, b->d_dense, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128) ||
                     !make_map3(&b->tmVd, false, b->d_dense + want * row, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128))
                     return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the dequantised rows");
                 b->dense_rows = want;
             } else {
                 cudaGetLastError();
-                cudaFree(b->d_dense);
                 b->d_dense = nullptr;
             }
         }
@@ -579,7 +578,9 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
                 de[n_dense] = make_int2(lin[i] + j * ps, std::min(ps, kv_len[i] - j * ps));
             }
         }
-        reinterpret_cast<int*>(h + b->at_counts)[b->windows.size() * kKinds * 4 + 1] = n_dense;
+        int* counts = reinterpret_cast<int*>(h + b->at_counts) + b->windows.size() * kKinds * 4;
+        counts[1] = n_dense;
+        counts[2] = (int)tokens;
     }
     const double tile_bytes = 16.0 * 2 * b->D * (q8 ? 1 : 2);
     for (size_t l = 0; l < b->windows.size(); ++l) {
@@ -642,7 +643,7 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
             std::stable_sort(tiles[kTc].begin(), tiles[kTc].end(), [&](const Tile& x, const Tile& y) { return n_tiles(x) > n_tiles(y); });
             for (const Tile& t : tiles[kTc]) pair_tiles.push_back(n_tiles(t));
             int n = 0, n_merge = 0, part = 0, piece = 1;
-            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, q8 ? 4.0 : 2.4, &piece);
+            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, &piece);
             b->scratch.clear();
             for (const Tile& t : tiles[kTc]) {
                 const bool cut = &t - tiles[kTc].data() >= whole;
@@ -748,7 +749,6 @@ template <int D, int FMT>
 int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& args, int rows, bool capturing) {
     if constexpr (D <= 128) {
         constexpr bool q8 = FMT == kKvQ8Head;
-        const int64_t scale_rows = (int64_t)b->dense_rows + 128;  // (whole tiles are read)
         if constexpr (q8) {
             ReadArgs r{};
             r.pages = b->pages->v;
@@ -759,12 +759,13 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
             r.k_out = b->d_dense;
             r.v_out = b->d_dense + b->dense_rows * b->Hkv * b->D;
             r.k_stride = r.v_stride = (int64_t)b->Hkv * b->D;
-            r.ks_out = b->d_dense_scales;
-            r.vs_out = b->d_dense_scales + b->Hkv * scale_rows;
-            r.scale_rows = scale_rows;
+            r.q = static_cast<const __nv_bfloat16*>(args.q);
+            r.q_stride = args.q_stride;
+            r.q_out = b->d_q16;
+            r.q_dim = b->Hq * D;
             {
                 PathTimer t(c, 1);
-                paged_read_kernel<kKvQ8Head, D, kReadCodes><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
+                paged_read_kernel<kKvQ8Head, D, kReadHalf><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
             }
             PAGED_TRY(c, cudaGetLastError());
             path_launched(c);
@@ -776,13 +777,13 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         t.tiles_tokens = b->tc_tokens;
         t.box_rows = b->pages ? std::min(b->pages->page_size, 128) : 128;
         t.linear = !b->pages || q8;
-        t.dense_ks = b->d_dense_scales;
-        t.dense_vs = b->d_dense_scales + b->Hkv * scale_rows;
-        t.dense_rows = scale_rows;
+        t.out_scale = q8 ? 1.0f / kReadVScale : 1.0f;
         t.sched = b->d_sched;
         t.part = b->d_tc_part;
         CUtensorMap tq;
-        if (!make_map3(&tq, false, args.q, D, b->Hq, rows, (uint64_t)D * 2, (uint64_t)args.q_stride * 2, 64, b->G, b->tc_tokens))
+        // (tensor maps move 16-bit elements as they are: bf16 stands for f16 too)
+        const void* q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
+        if (!make_map3(&tq, false, q_rows, D, b->Hq, rows, (uint64_t)D * 2, (uint64_t)(q8 ? b->Hq * D : args.q_stride) * 2, 64, b->G, b->tc_tokens))
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the query rows");
         static KernelSmemSetup setup;
         PAGED_TRY(c, setup.ensure(paged_tc_kernel<D, q8>, p.device, p.smem_optin, (int)kPtSmem<D>));

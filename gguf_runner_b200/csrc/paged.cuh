@@ -9,6 +9,8 @@
 // reads back as NaN instead of as a finite row.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "rope_math.cuh"
 
@@ -212,12 +214,23 @@ struct ReadArgs {
     void* k_out;
     void* v_out;
     int64_t k_stride, v_stride;  // elements between dense rows
-    float* ks_out;               // kReadCodes: scales [KV head][scale_rows]
-    float* vs_out;
-    int64_t scale_rows;
+    // kReadHalf: the new tokens' q goes into f16 rows as well
+    const __nv_bfloat16* q;
+    __half* q_out;
+    int64_t q_stride;
+    int q_dim;
 };
 
-enum ReadOut { kReadF32 = 0, kReadBf16 = 1, kReadCodes = 2 };  // kReadCodes: the codes themselves in bf16, their scales apart
+// kReadHalf: f16 operands of the tcgen05 kernel. V is taken times 64, so that values of 6e-8 to 1000 keep the precision of a
+// bf16 row or better; what f16 cannot hold (or was not finite) becomes NaN, and rows that meet it are computed again from the
+// pages in f32.
+enum ReadOut { kReadF32 = 0, kReadBf16 = 1, kReadHalf = 2 };
+constexpr float kReadVScale = 64.0f;
+
+__device__ __forceinline__ uint32_t half2_or_nan(float x, float y) {
+    const __half2 h = __floats2half2_rn(fabsf(x) <= 65504.0f ? x : NAN, fabsf(y) <= 65504.0f ? y : NAN);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 // Rows of all sequences out of their pages: a warp-wide task is 16 elements of one row, a CTA takes blocks of 16 rows of one
 // KV head of K and of V. The page ids of four blocks are fetched before the rows of any, and the rows of four before the
@@ -280,12 +293,16 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
                     unpack8(raw[i][1], x + 8);
                 } else {
                     const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+                    if (OUT == kReadHalf && is_v) scale[i] *= kReadVScale;
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) x[q] = (float)(int8_t)(w[q >> 2] >> (8 * (q & 3))) * (OUT == kReadCodes ? 1.0f : scale[i]);
-                    if (OUT == kReadCodes && e == 0) (is_v ? a.vs_out : a.ks_out)[head[u] * a.scale_rows + dense[u] + r] = scale[i];
+                    for (int q = 0; q < 16; ++q) x[q] = (float)(int8_t)(w[q >> 2] >> (8 * (q & 3))) * scale[i];
                 }
                 const int64_t to = (int64_t)(dense[u] + r) * stride + (int64_t)head[u] * D + e;
-                if constexpr (OUT != kReadF32) {
+                if constexpr (OUT == kReadHalf) {
+                    uint4* o = reinterpret_cast<uint4*>(static_cast<__half*>(out) + to);
+                    o[0] = make_uint4(half2_or_nan(x[0], x[1]), half2_or_nan(x[2], x[3]), half2_or_nan(x[4], x[5]), half2_or_nan(x[6], x[7]));
+                    o[1] = make_uint4(half2_or_nan(x[8], x[9]), half2_or_nan(x[10], x[11]), half2_or_nan(x[12], x[13]), half2_or_nan(x[14], x[15]));
+                } else if constexpr (OUT == kReadBf16) {
                     uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to);
                     if constexpr (FMT == KV_BF16) {
                         o[0] = raw[i][0];
@@ -300,6 +317,17 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
                     store8_f32(o + 8, x + 8);
                 }
             }
+    }
+    if constexpr (OUT == kReadHalf) {
+        const int vecs = a.q_dim / 8;
+        const int64_t n = (int64_t)a.counts[2] * vecs;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+            const int64_t row = i / vecs, d = (i - row * vecs) * 8;
+            float x[8];
+            load8_in<__nv_bfloat16>(a.q + row * a.q_stride + d, x);
+            *reinterpret_cast<uint4*>(a.q_out + row * a.q_dim + d) =
+                make_uint4(half2_or_nan(x[0], x[1]), half2_or_nan(x[2], x[3]), half2_or_nan(x[4], x[5]), half2_or_nan(x[6], x[7]));
+        }
     }
 }
 

@@ -9,10 +9,10 @@
 //    of the producer warp side by side; each lane looks its page up one tile ahead.
 //  - Items (two query tiles and a stretch of keys) are cut on the host, longest first, and handed out through a counter. Pieces
 //    of a pair of tiles leave un-normalised rows, which paged_tc_merge_kernel weighs in the order of the keys.
-//  - Codes of 8-bit pages come as dense rows of bf16 (paged_read_kernel, which every code survives; 17 us of 480 for 2048
-//    tokens behind 14336, 40/8 heads of 128), and their scales stay apart: the softmax multiplies scores by those of K and
-//    weights by those of V, so that 8-bit rows cost no rounding of their own. A lane fetches four of a tile's 128 scales one
-//    tile ahead, and the warp reads them back from its output staging area.
+//  - 8-bit pages are read into dense f16 rows first (paged_read_kernel, 25 us of READ_NOTE for 2048 tokens behind 14336, 40/8
+//    heads of 128), q into f16 beside them: eleven bits leave code * scale 2^-12 off, an eighth of what bf16 weights are. With
+//    bf16 codes and the scales multiplied into scores and weights by the softmax warps the same launch took 1250 us: two
+//    multiplications and half a shared-memory load per score are too much for warps that one chain of latencies binds.
 // Values that nobody in the item sees (behind the sequence's end, before its window) may be anything, and 0 * NaN is NaN: the
 // producer clears them in the first and last tile, before the MMA issuer hears of the tile. Rows that come out not finite are
 // computed again by paged_row_again.
@@ -26,10 +26,8 @@ struct PagedTcArgs {
     PagedAttnArgs a;
     int tiles_tokens;  // tokens of a query tile: 128 / G
     int box_rows;      // paged: rows of one copy, min(page_size, 128)
-    int linear;        // K and V tiles come from dense rows (packed prompts, or the codes of 8-bit pages)
-    const float* dense_ks;  // 8-bit pages: scales of the dense rows [KV head][dense_rows]
-    const float* dense_vs;
-    int64_t dense_rows;
+    int linear;        // K and V tiles come from dense rows (packed prompts, or 8-bit pages read into f16 rows)
+    float out_scale;   // of the merged rows: 1 / kReadVScale for f16 rows
     int* sched;        // [0] items handed out beyond the first wave, [1] CTAs that have left
     float* part;       // states of pieces: [256][D], then [256] (m, l)
 };
@@ -72,14 +70,15 @@ __device__ __forceinline__ PtRange pt_range(const PagedTcArgs& p, const PagedIte
     return r;
 }
 
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
+template <bool HALF>
+__device__ __forceinline__ uint32_t pt_pack(float x, float y) {
+    if constexpr (!HALF) return pack_bf16x2(x, y);
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// SCALED: rows are codes, with scales beside them.
-template <int D, bool SCALED>
+// HALF: operands are f16 (of 8-bit pages; V times kReadVScale) instead of bf16.
+template <int D, bool HALF>
 __global__ void __launch_bounds__(kPtThreads, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                 const __grid_constant__ PagedTcArgs p) {
@@ -225,7 +224,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             }
         } else if (warp == 9) {
             // ---------------- MMA issuer ----------------
-            constexpr uint32_t IDESC_QK = idesc_bf16(128, 0), IDESC_PV = idesc_bf16(D, 1);
+            constexpr uint32_t TYPES = (1u << 7) | (1u << 10);  // A and B: bf16, or f16 without
+            constexpr uint32_t IDESC_QK = idesc_bf16(128, 0) & ~(HALF ? TYPES : 0u), IDESC_PV = idesc_bf16(D, 1) & ~(HALF ? TYPES : 0u);
             const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024), dV = smem_desc(sV, BLK, 1024);
             const uint32_t tm = __shfl_sync(0xffffffffu, s_tmem_base, 0);
             auto issue_qk = [&](int t, int s) {
@@ -345,58 +345,23 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const int lo_t = rg.lo_of(t), hi_t = rg.hi_of(t), n_t = hi_t - lo_t;
             const int tok = w.row0 + t * p.tiles_tokens + tile_tok;
             const bool valid = tile_tok < p.tiles_tokens && tok < w.n_tok;
-            int vs = 0, ve = 0;
+            // Rows that stand for no token (behind the sequence's end; three of 128 where five heads share a KV head) see everything:
+            // their results go nowhere, and hidden keys would send their warps through the masks of every tile (40/8 heads, 2048
+            // tokens behind 14336: 1186 us instead of 537).
+            int vs = 0, ve = 0x7fffffff;
             if (valid) {
                 ve = w.pos0 + tok + 1;
                 vs = paged_first_key(w.pos0 + tok, a.window);
             }
             float m_used = -INFINITY, l = 0.0f;
-            unsigned char* scales_p = smem_raw + (sOut - smem_u32(smem_raw)) + warp * 4096;  // 128 of K, 128 of V
-            float4 next_ks, next_vs;
-            auto fetch_scales = [&](int j) {
-                const int key = j * 128 + lane * 4;
-                const int64_t at = (int64_t)w.kvh * p.dense_rows + w.lin + key;
-                const int any_lo = paged_first_key(w.pos0 + w.row0, a.window), any_hi = w.pos0 + min(w.row0 + 2 * p.tiles_tokens, w.n_tok);
-                next_ks = __ldg(reinterpret_cast<const float4*>(p.dense_ks + at));
-                next_vs = __ldg(reinterpret_cast<const float4*>(p.dense_vs + at));
-                // a weight of zero times what lies beside the item's keys must stay zero
-                if (key < any_lo || key >= any_hi) next_vs.x = 0.0f;
-                if (key + 1 < any_lo || key + 1 >= any_hi) next_vs.y = 0.0f;
-                if (key + 2 < any_lo || key + 2 >= any_hi) next_vs.z = 0.0f;
-                if (key + 3 < any_lo || key + 3 >= any_hi) next_vs.w = 0.0f;
-            };
-            if (SCALED && lo_t < hi_t) fetch_scales(lo_t);
             for (int j = lo_t; j < hi_t; ++j) {
                 const int k = j - lo_t;
-                if constexpr (SCALED) {
-                    __syncwarp();
-                    reinterpret_cast<float4*>(scales_p)[lane] = next_ks;
-                    reinterpret_cast<float4*>(scales_p + 512)[lane] = next_vs;
-                    __syncwarp();
-                    if (j + 1 < hi_t) fetch_scales(j + 1);
-                }
                 if (!(ok = mbar_wait(s_full(t), (cs + k) & 1, abortp))) break;
                 fence_after_sync();
                 uint32_t sr[4][32];
 #pragma unroll
                 for (int cidx = 0; cidx < 4; ++cidx) tmem_ld32(tS + cidx * 32, sr[cidx]);
                 tmem_wait_ld();
-                if constexpr (SCALED) {
-#pragma unroll
-                    for (int cidx = 0; cidx < 4; ++cidx)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(scales_p + (cidx * 32 + i) * 4);
-                            const uint64_t k01 = k4.x, k23 = k4.y;
-                            float x0, x1, x2, x3;
-                            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1])), k01), x0, x1);
-                            unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3])), k23), x2, x3);
-                            sr[cidx][i] = __float_as_uint(x0);
-                            sr[cidx][i + 1] = __float_as_uint(x1);
-                            sr[cidx][i + 2] = __float_as_uint(x2);
-                            sr[cidx][i + 3] = __float_as_uint(x3);
-                        }
-                }
                 const int key0 = j * 128;
                 const bool cut = key0 < vs || key0 + 128 > ve, any_cut = __any_sync(0xffffffffu, cut);
                 if (cut) {
@@ -450,7 +415,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         const uint64_t tb = fma_f32x2(pack_f32x2(__uint_as_float(sr[cidx][2 * i + 2]), __uint_as_float(sr[cidx][2 * i + 3])), c2, neg2);
                         float x0, x1, p2, p3;
                         unpack_f32x2(ta, x0, x1);
-                        float p0 = ex2(x0), p1 = ex2(x1);
+                        const float p0 = ex2(x0), p1 = ex2(x1);
                         if (kPtExpPolyMask & (1 << ((i >> 1) & 3))) {
                             ex2_poly_x2(tb, p2, p3);
                         } else {
@@ -461,14 +426,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                         sum_a = add_f32x2(sum_a, pack_f32x2(p0, p1));
                         sum_b = add_f32x2(sum_b, pack_f32x2(p2, p3));
-                        if constexpr (SCALED) {
-                            const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(scales_p + 512 + (cidx * 32 + 2 * i) * 4);
-                            const uint64_t v01 = v4.x, v23 = v4.y;
-                            unpack_f32x2(mul_f32x2(pack_f32x2(p0, p1), v01), p0, p1);
-                            unpack_f32x2(mul_f32x2(pack_f32x2(p2, p3), v23), p2, p3);
-                        }
-                        pk[i] = pack_bf16x2(p0, p1);
-                        pk[i + 1] = pack_bf16x2(p2, p3);
+                        pk[i] = pt_pack<HALF>(p0, p1);
+                        pk[i + 1] = pt_pack<HALF>(p2, p3);
                     }
                     if (any_cut) {
                         // the polynomial gives 2^-125 for a hidden key, which a large value there would show: exactly zero instead
@@ -505,7 +464,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (n_t > 0) {
                 // rows leave through a per-warp staging area of 32 rows x 128 bytes, 16-byte pieces XORed by the row, and are
                 // stored as whole 128-byte lines: 64 bf16 columns at a time, or 32 columns of a piece's f32 state
-                const float inv = 1.0f / l;
+                const float inv = (HALF ? 1.0f / kReadVScale : 1.0f) / l;
                 const uint32_t stage = sOut + (uint32_t)warp * 4096u;
                 const int sub_row = lane >> 3, piece = lane & 7;
                 const int64_t my_at = valid ? (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D : -1;
@@ -618,7 +577,7 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_consta
                 o[2 * e + 1] = fmaf(f, x.y, o[2 * e + 1]);
             }
         }
-        const float inv = 1.0f / l;
+        const float inv = p.out_scale / l;
         bool bad = false;
         uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D);
 #pragma unroll
