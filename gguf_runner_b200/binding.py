@@ -315,6 +315,23 @@ def _ptr(x, want_dtype=None):
     return C.c_void_p(a.ctypes.data), PTR_HOST
 
 
+def _raw_stream(device: int) -> int:
+    """The cudaStream_t of torch's current stream on a device."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (without a Stream object: 0.2 us instead of 1.2)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _capturing() -> bool:
+    import torch
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _torch_dtype(name: str):
+    import torch
+    return torch.float32 if name == "f32" else torch.bfloat16
+
+
 class Pages:
     """A pool of cache pages for every layer of a context: K and V [layer][page][KV head][position][head_dim] in bf16, or int8
     with f32 scales [layer][page][KV head][position] (`q8_head`). Without tensors the library allocates (and clears) the pool;
@@ -371,7 +388,7 @@ class Batch:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
         self._L, self.ctx, self.pages, self.dtype = lib(), ctx, pages, dtype
         self.max_tokens, self.n_tokens, self.n_rows = max_tokens, 0, 0
-        self.torch_dtype = "float32" if dtype == "f32" else "bfloat16"
+        self.torch_dtype = _torch_dtype(dtype)
         h = C.c_void_p()
         ctx._check(self._L.ggr_batch_create(ctx._h, None if pages is None else pages._h, DTYPES[dtype], max_seqs, max_tokens, max_pages,
                                             C.byref(h)))
@@ -435,8 +452,7 @@ class AttnContext:
         ordered with the kernels that produced the tensors and those that read the result."""
         for t in tensors:
             if t is not None and _is_torch(t) and t.is_cuda:
-                import torch
-                handle = torch.cuda.current_stream(t.device).cuda_stream or 1  # 0 is the legacy default stream
+                handle = _raw_stream(t.get_device()) or 1  # 0 is the legacy default stream
                 if handle != self._stream:
                     self.set_stream(handle)
                 return
@@ -737,34 +753,37 @@ class AttnContext:
             raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
 
     def _follow_torch_stream_of_device(self):
-        import torch
-        handle = torch.cuda.current_stream(self.config.device).cuda_stream or 1
+        handle = _raw_stream(self.config.device) or 1
         if handle != self._stream:
             self.set_stream(handle)
 
-    def _rows(self, name, x, dtype, n, dim):
-        """Address and row stride of `n` rows (a [rows][dim] tensor whose elements of a row lie together)."""
-        self._check_tensor(name, x, dtype)
-        if x.dim() != 2 or x.shape[0] < n or x.shape[1] != dim or (dim > 1 and x.stride(1) != 1):
-            raise ValueError(f"{name} must have at least {n} rows of {dim} elements, each row contiguous")
-        return x.data_ptr(), (x.stride(0) if x.shape[0] > 1 else dim)
+    def _rows(self, name, x, dtype, n, dim, most=0):
+        """Address and row stride of `n` rows (a [rows][dim] tensor whose elements of a row lie together). A captured call needs
+        `most` rows: replays may find a longer plan. (A token step is a few of these calls: the checks take 0.6 us.)"""
+        if _is_torch(x) and x.dtype is dtype and x.is_cuda and x.get_device() == self.config.device and x.dim() == 2:
+            rows, cols = x.shape
+            step, one = x.stride()
+            if rows >= n and cols == dim and one == 1 and (rows >= most or not _capturing()):
+                return x.data_ptr(), step if rows > 1 else dim
+        self._check_tensor(name, x, str(dtype)[6:])
+        raise ValueError(f"{name} must have at least {n} rows of {dim} elements, each row contiguous"
+                         + (f", and {most} under stream capture" if most > n else ""))
 
-    def _row_out(self, out, like, n, dim, dtype):
-        if out is None:
-            import torch
-            return torch.empty((n, dim), dtype=getattr(torch, dtype), device=like.device)
-        return out
+    def _row_out(self, like, n, dim, dtype):
+        import torch
+        return torch.empty((n, dim), dtype=dtype, device=like.device)
 
     def paged_append(self, batch: Batch, layer: int, k, v, q=None, q_out=None):
         """Rows of k and v into the pages of the batch's new tokens. With q: RoPE on q and k first; returns rotated q."""
-        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
-        kp, ks = self._rows("k", k, dt, n, c.kv_dim)
-        vp, vs = self._rows("v", v, dt, n, c.kv_dim)
+        c, n, dt, most = self.config, batch.n_tokens, batch.torch_dtype, batch.max_tokens
+        kp, ks = self._rows("k", k, dt, n, c.kv_dim, most)
+        vp, vs = self._rows("v", v, dt, n, c.kv_dim, most)
         qp, qs, op = None, 0, None
         if q is not None:
-            q_out = self._row_out(q_out, q, n, c.q_dim, dt)
-            qp, qs = self._rows("q", q, dt, n, c.q_dim)
-            op, os_ = self._rows("q_out", q_out, dt, n, c.q_dim)
+            if q_out is None:
+                q_out = self._row_out(q, most if _capturing() else n, c.q_dim, dt)
+            qp, qs = self._rows("q", q, dt, n, c.q_dim, most)
+            op, os_ = self._rows("q_out", q_out, dt, n, c.q_dim, most)
             if os_ != c.q_dim:
                 raise ValueError("q_out must be dense")
         elif q_out is not None:
@@ -774,42 +793,40 @@ class AttnContext:
         return q_out
 
     def paged_read(self, batch: Batch, layer: int, dtype: str = "bf16", k_out=None, v_out=None):
-        """All cached rows of all sequences of the batch, dequantised: (k, v), each [sum of kv_len][kv_dim]."""
-        import torch
+        """All cached rows of all sequences of the batch, dequantised: (k, v), each [sum of kv_len][kv_dim]. (A captured call
+        is not told how long later plans are: its tensors have to hold the longest.)"""
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
-        name, c, n = "float32" if dtype == "f32" else "bfloat16", self.config, batch.n_rows
-        k_out, v_out = (torch.empty((n, c.kv_dim), dtype=getattr(torch, name), device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
-        kp, ks = self._rows("k_out", k_out, name, n, c.kv_dim)
-        vp, vs = self._rows("v_out", v_out, name, n, c.kv_dim)
+        dt, c, n = _torch_dtype(dtype), self.config, batch.n_rows
+        if k_out is None or v_out is None:
+            import torch
+            k_out, v_out = (torch.empty((n, c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
+        kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim)
+        vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim)
         self._follow_torch_stream(k_out)
         self._check(self._L.ggr_paged_read(self._h, batch._h, layer, DTYPES[dtype], kp, ks, vp, vs))
         return k_out, v_out
 
     def paged_attention(self, batch: Batch, layer: int, q, out=None):
         """Attention of the batch's new tokens (rotated q) over their sequences' pages."""
-        import torch
-        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
-        if torch.cuda.is_current_stream_capturing():
-            n = batch.max_tokens  # replays may find a longer plan
-        out = self._row_out(out, q, n, c.q_dim, dt)
-        qp, qs = self._rows("q", q, dt, n, c.q_dim)
-        op, os_ = self._rows("out", out, dt, n, c.q_dim)
+        c, n, dt, most = self.config, batch.n_tokens, batch.torch_dtype, batch.max_tokens
+        if out is None:
+            out = self._row_out(q, most if _capturing() else n, c.q_dim, dt)
+        qp, qs = self._rows("q", q, dt, n, c.q_dim, most)
+        op, os_ = self._rows("out", out, dt, n, c.q_dim, most)
         self._follow_torch_stream(q)
         self._check(self._L.ggr_paged_attention(self._h, batch._h, layer, qp, qs, op, os_))
         return out
 
     def packed_attention(self, batch: Batch, layer: int, q, k, v, out=None):
         """Causal attention of whole prompts from their rotated q, k and v rows (a batch without pages)."""
-        import torch
-        c, n, dt = self.config, batch.n_tokens, batch.torch_dtype
-        if torch.cuda.is_current_stream_capturing():
-            n = batch.max_tokens  # replays may find a longer plan
-        out = self._row_out(out, q, n, c.q_dim, dt)
-        qp, qs = self._rows("q", q, dt, n, c.q_dim)
-        kp, ks = self._rows("k", k, dt, n, c.kv_dim)
-        vp, vs = self._rows("v", v, dt, n, c.kv_dim)
-        op, os_ = self._rows("out", out, dt, n, c.q_dim)
+        c, n, dt, most = self.config, batch.n_tokens, batch.torch_dtype, batch.max_tokens
+        if out is None:
+            out = self._row_out(q, most if _capturing() else n, c.q_dim, dt)
+        qp, qs = self._rows("q", q, dt, n, c.q_dim, most)
+        kp, ks = self._rows("k", k, dt, n, c.kv_dim, most)
+        vp, vs = self._rows("v", v, dt, n, c.kv_dim, most)
+        op, os_ = self._rows("out", out, dt, n, c.q_dim, most)
         self._follow_torch_stream(q)
         self._check(self._L.ggr_packed_attention(self._h, batch._h, layer, qp, qs, kp, ks, vp, vs, op, os_))
         return out

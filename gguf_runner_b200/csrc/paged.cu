@@ -742,7 +742,7 @@ void launch_read(const ReadArgs& a, bool bf16, int grid, cudaStream_t stream) {
 
 int read_grid(const ggr_batch* b, int64_t entries) {
     const int64_t blocks = entries * (b->pages->page_size / 16) * b->Hkv;
-    return (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)8 * b->sm_count);
+    return (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)16 * b->sm_count);
 }
 
 template <int D, int FMT>
@@ -800,7 +800,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         const int pairs = capturing ? (int)b->tc_parts / 2 : b->n_items[list][kMerge];
         {
             PathTimer timer(c, 2);
-            PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(std::min(pairs * 32, 8 * b->sm_count)), 256, 0, p.stream, t));
+            PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(std::min(pairs * D / 4, 16 * b->sm_count)), 256, 0, p.stream, t));
         }
         path_launched(c);
     }
@@ -817,7 +817,7 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
         if (!n) continue;
         a.plan.counts = b->counts(list, k);
         a.plan.items = b->items(list, k);
-        const dim3 grid(capturing ? most : n, b->Hkv);
+        const dim3 grid(b->Hkv, capturing ? most : std::min(n, 65535));
         if (k == kSplitK) {
             if constexpr (FMT == KV_F32) continue;
             else {
@@ -913,6 +913,7 @@ extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, in
     a.q_bf16 = b->dtype == GGR_DTYPE_BF16;
     a.Hq = b->Hq;
     a.heads = (rotate ? b->Hq : 0) + 2 * b->Hkv;
+    a.heads_inv = (unsigned)(((1ull << 32) + a.heads - 1) / a.heads);
     a.q = q;
     a.k = k;
     a.v = v;
@@ -922,7 +923,9 @@ extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, in
     a.v_stride = v_stride;
     a.qo_stride = qo_stride;
     const int n = capturing ? b->max_tokens : b->n_tokens;
-    a.tokens_per_cta = std::min(4, std::max(1, n / (8 * b->sm_count)));
+    // (two tasks of 16 bytes per thread, once there are CTAs enough)
+    const int tasks = a.heads * b->D / (in_bf16 ? 16 : 8);
+    a.tokens_per_cta = n < 8 * b->sm_count ? 1 : std::max(1, 512 / tasks);
     const int grid = (n + a.tokens_per_cta - 1) / a.tokens_per_cta;
     const size_t smem = rotate ? (size_t)2 * a.tokens_per_cta * a.rope.rope_half * sizeof(float) : 0;
     {

@@ -63,6 +63,7 @@ struct AppendArgs {
     const int* tok_slot;     // page * page_size + row in the page
     int layer, rotate, write_q, in_bf16, q_bf16;
     int Hq, tokens_per_cta, heads;  // heads: of q (when it is rotated), k and v together
+    unsigned heads_inv;             // 2^32 / heads, rounded up: task numbers are divided by a multiplication
     const void* q;
     const void* k;
     const void* v;
@@ -70,25 +71,82 @@ struct AppendArgs {
     int64_t q_stride, k_stride, v_stride, qo_stride;  // elements between rows
 };
 
+// 16 bytes of a row, as they lie and as E f32 elements (E = 4 of f32, 8 of bf16 rows).
 template <bool BF16>
-__device__ __forceinline__ void load8_any(const void* p, int64_t at, float x[8]) {
-    if constexpr (BF16)
-        load8_in<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p) + at, x);
-    else
-        load8_in<float>(static_cast<const float*>(p) + at, x);
+__device__ __forceinline__ uint4 load_raw(const void* p, int64_t at) {
+    return *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(p) + at * (BF16 ? 2 : 4));
+}
+template <bool BF16, int E>
+__device__ __forceinline__ void unpack_raw(const uint4& v, float (&x)[E]) {
+    if constexpr (BF16) {
+        unpack8(v, x);
+    } else {
+        x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    }
+}
+// Codes of four elements, rounded half away from zero. (|x * inv| is at most 127 but for its own rounding, so nothing saturates.)
+__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = (int)roundf(__fmul_rn(x[i], inv));
+    uint32_t hi, w;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(hi) : "r"(c[3]), "r"(c[2]), "r"(0));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(c[1]), "r"(c[0]), "r"(hi));
+    return w;
+}
+template <int E>
+__device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const float (&x)[E]) {
+    if constexpr (E == 8) {
+        *reinterpret_cast<uint4*>(p) = pack8(x);
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
 }
 
-// RoPE and append of a few tokens per CTA. D / 16 lanes share a head, each with elements [8 j, 8 j + 8) of its lower and of
-// its upper half, so that both kinds of RoPE pairs of a fully rotated head lie in one lane and its largest element takes
-// log2(D / 16) shuffles. Bound by the bytes of the rows; one token per CTA while tokens are few (a token step is latency:
-// the angles of a token, one load, one store), several when there are more CTAs than SMs to hold them.
+// RoPE and append of a few tokens per CTA. A lane has E elements of the lower half of a head and E of the upper, 16 bytes each,
+// so that both kinds of RoPE pairs of a fully rotated head lie in one lane, a warp's loads are whole lines, and the head's
+// largest element takes log2(D / 2E) shuffles. Bound by the bytes of the rows; one token per CTA while tokens are few (a token
+// step is latency: the angles of a token, one load, one store), several when there are more CTAs than SMs to hold them. A
+// thread requests the rows of two tasks before it works on either.
 template <bool BF16>
-__global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) paged_append_kernel(AppendArgs a) {
+    constexpr int E = BF16 ? 8 : 4, UN = 2;
     extern __shared__ float sm[];  // cos [tokens_per_cta][half], sin
-    const int D = a.pages.D, lanes = D / 16, half = a.rope.rope_half;
+    const int D = a.pages.D, lanes_log2 = 31 - __clz(D / (2 * E)), lanes = 1 << lanes_log2, half = a.rope.rope_half;
     const int total = a.counts[2], t0 = blockIdx.x * a.tokens_per_cta;
     if (t0 >= total) return;
     const int n = min(a.tokens_per_cta, total - t0);
+    const int Hkv = a.pages.Hkv, nq = a.write_q ? a.Hq : 0, tasks = n * a.heads * lanes;
+    struct Task {
+        const void* src;
+        int64_t at;
+        int t, kind, head, j;
+        bool live;
+    };
+    auto task_of = [&](int i) {
+        Task k;
+        k.live = i < tasks;
+        const int unit = k.live ? i >> lanes_log2 : 0;
+        k.j = i & (lanes - 1);
+        k.t = (int)__umulhi((unsigned)unit, a.heads_inv);
+        const int h = unit - k.t * a.heads;
+        k.kind = h < nq ? 0 : (h < nq + Hkv ? 1 : 2);
+        k.head = k.kind == 0 ? h : (k.kind == 1 ? h - nq : h - nq - Hkv);
+        k.src = k.kind == 0 ? a.q : (k.kind == 1 ? a.k : a.v);
+        k.at = (t0 + k.t) * (k.kind == 0 ? a.q_stride : (k.kind == 1 ? a.k_stride : a.v_stride)) + (int64_t)k.head * D;
+        return k;
+    };
+    uint4 x[UN], y[UN];
+    auto fetch = [&](int i, uint4& lo, uint4& hi) {
+        const Task k = task_of(i);
+        lo = hi = make_uint4(0, 0, 0, 0);
+        if (!k.live) return;
+        lo = load_raw<BF16>(k.src, k.at + k.j * E);
+        hi = load_raw<BF16>(k.src, k.at + D / 2 + k.j * E);
+    };
+#pragma unroll
+    for (int u = 0; u < UN; ++u) fetch(threadIdx.x + u * 256, x[u], y[u]);
     float* cs = sm;
     float* sn = sm + a.tokens_per_cta * half;
     if (a.rotate) {
@@ -99,44 +157,30 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
         }
         __syncthreads();
     }
-    const int Hkv = a.pages.Hkv, nq = a.write_q ? a.Hq : 0;
-    const int tasks = n * a.heads * lanes;
-    // whole warps take part in the shuffles of the last round
-    for (int task = threadIdx.x; task < ((tasks + 31) & ~31); task += 256) {
-        const bool live = task < tasks;
-        const int unit = live ? task / lanes : 0, j = task & (lanes - 1);
-        const int t = unit / a.heads, h = unit - t * a.heads, tok = t0 + t;
-        const int kind = h < nq ? 0 : (h < nq + Hkv ? 1 : 2), hh = kind == 0 ? h : (kind == 1 ? h - nq : h - nq - Hkv);
-        const void* src = kind == 0 ? a.q : (kind == 1 ? a.k : a.v);
-        const int64_t at = tok * (kind == 0 ? a.q_stride : (kind == 1 ? a.k_stride : a.v_stride)) + (int64_t)hh * D;
-        const int e0 = j * 8, e1 = D / 2 + j * 8;
-        float x[8], y[8];
-        if (live) {
-            load8_any<BF16>(src, at + e0, x);
-            load8_any<BF16>(src, at + e1, y);
-        } else {
-#pragma unroll
-            for (int p = 0; p < 8; ++p) x[p] = y[p] = 0.0f;
-        }
-        if (a.rotate && kind < 2 && live) {
-            const float* c = cs + t * half;
-            const float* s = sn + t * half;
+    auto finish = [&](const Task& k, const uint4& raw_x, const uint4& raw_y) {
+        float x[E], y[E];
+        unpack_raw<BF16, E>(raw_x, x);
+        unpack_raw<BF16, E>(raw_y, y);
+        const int e0 = k.j * E, e1 = D / 2 + k.j * E, tok = t0 + k.t;
+        if (a.rotate && k.kind < 2 && k.live) {
+            const float* c = cs + k.t * half;
+            const float* s = sn + k.t * half;
             if (a.rope.rope_dim != D) {  // part of a head: partners may lie in other lanes
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
-                    x[p] = rope_elem(src, at, e0 + p, D, a.rope, c, s, BF16);
-                    y[p] = rope_elem(src, at, e1 + p, D, a.rope, c, s, BF16);
+                for (int p = 0; p < E; ++p) {
+                    x[p] = rope_elem(k.src, k.at, e0 + p, D, a.rope, c, s, BF16);
+                    y[p] = rope_elem(k.src, k.at, e1 + p, D, a.rope, c, s, BF16);
                 }
             } else if (a.rope.style == 0) {
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
+                for (int p = 0; p < E; ++p) {
                     const float lo = x[p], hi = y[p], cc = c[e0 + p], ss = s[e0 + p];
                     x[p] = __fsub_rn(__fmul_rn(lo, cc), __fmul_rn(hi, ss));
                     y[p] = __fadd_rn(__fmul_rn(lo, ss), __fmul_rn(hi, cc));
                 }
             } else {
 #pragma unroll
-                for (int p = 0; p < 8; p += 2) {
+                for (int p = 0; p < E; p += 2) {
                     const float x0 = x[p], x1 = x[p + 1], y0 = y[p], y1 = y[p + 1];
                     const int i0 = (e0 + p) >> 1, i1 = (e1 + p) >> 1;
                     x[p] = __fsub_rn(__fmul_rn(x0, c[i0]), __fmul_rn(x1, s[i0]));
@@ -146,11 +190,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
                 }
             }
         }
-        float top = 0.0f, step = 1.0f;
-        if (a.pages.fmt == kKvQ8Head) {
+        float top = 0.0f;
+        if (a.pages.fmt == kKvQ8Head) {  // (whole warps take part)
             bool odd = false;  // a value that is not finite: max would lose a NaN
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
+            for (int p = 0; p < E; ++p) {
                 top = fmaxf(top, fmaxf(fabsf(x[p]), fabsf(y[p])));
                 odd |= !isfinite(x[p]) | !isfinite(y[p]);
             }
@@ -158,50 +202,67 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
             if (top < 1e-36f) top = 0.0f;  // 127 / m would overflow: such a row counts as zeros
             for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
-        if (!live) continue;
-        if (kind == 0) {
+        if (!k.live) return;
+        if (k.kind == 0) {
             if (a.rope.do_prescale && a.rotate) {
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
+                for (int p = 0; p < E; ++p) {
                     x[p] = __fmul_rn(x[p], a.rope.q_prescale);
                     y[p] = __fmul_rn(y[p], a.rope.q_prescale);
                 }
             }
-            const int64_t to = tok * a.qo_stride + (int64_t)hh * D;
+            const int64_t to = tok * a.qo_stride + (int64_t)k.head * D;
             if (a.q_bf16) {
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.q_out) + to;
-                *reinterpret_cast<uint4*>(o + e0) = pack8(x);
-                *reinterpret_cast<uint4*>(o + e1) = pack8(y);
+                store_bf16<E>(o + e0, x);
+                store_bf16<E>(o + e1, y);
             } else {
                 float* o = static_cast<float*>(a.q_out) + to;
-                store8_f32(o + e0, x);
-                store8_f32(o + e1, y);
+#pragma unroll
+                for (int p = 0; p < E; p += 4) {
+                    *reinterpret_cast<float4*>(o + e0 + p) = make_float4(x[p], x[p + 1], x[p + 2], x[p + 3]);
+                    *reinterpret_cast<float4*>(o + e1 + p) = make_float4(y[p], y[p + 1], y[p + 2], y[p + 3]);
+                }
             }
-            continue;
+            return;
         }
         const int slot = a.tok_slot[tok];
-        const int64_t row = a.pages.row(a.layer, slot >> a.pages.page_log2, hh, slot & ((1 << a.pages.page_log2) - 1));
-        unsigned char* pool = kind == 1 ? a.pages.k : a.pages.v;
+        const int64_t row = a.pages.row(a.layer, slot >> a.pages.page_log2, k.head, slot & ((1 << a.pages.page_log2) - 1));
+        unsigned char* pool = k.kind == 1 ? a.pages.k : a.pages.v;
         if (a.pages.fmt == KV_BF16) {
             __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(pool) + row * D;
-            *reinterpret_cast<uint4*>(o + e0) = pack8(x);
-            *reinterpret_cast<uint4*>(o + e1) = pack8(y);
-            continue;
+            store_bf16<E>(o + e0, x);
+            store_bf16<E>(o + e1, y);
+            return;
         }
         const bool finite = top < INFINITY;
         const float inv = top > 0.0f && finite ? __fdiv_rn(127.0f, top) : 0.0f;
-        if (top > 0.0f) step = finite ? __fdiv_rn(top, 127.0f) : NAN;
-        uint32_t w[4] = {0, 0, 0, 0};
+        uint32_t w[E / 2] = {};
         if (finite) {
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                w[p >> 2] |= (uint32_t)(uint8_t)q8_code(x[p], inv) << (8 * (p & 3));
-                w[2 + (p >> 2)] |= (uint32_t)(uint8_t)q8_code(y[p], inv) << (8 * (p & 3));
+            for (int p = 0; p < E; p += 4) {
+                w[p >> 2] = codes4(x + p, inv);
+                w[(E + p) >> 2] = codes4(y + p, inv);
             }
         }
-        *reinterpret_cast<uint2*>(pool + row * D + e0) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(pool + row * D + e1) = make_uint2(w[2], w[3]);
-        if (j == 0) (kind == 1 ? a.pages.ks : a.pages.vs)[row] = step;
+        if constexpr (E == 8) {
+            *reinterpret_cast<uint2*>(pool + row * D + e0) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(pool + row * D + e1) = make_uint2(w[2], w[3]);
+        } else {
+            *reinterpret_cast<uint32_t*>(pool + row * D + e0) = w[0];
+            *reinterpret_cast<uint32_t*>(pool + row * D + e1) = w[1];
+        }
+        if (k.j == 0) (k.kind == 1 ? a.pages.ks : a.pages.vs)[row] = top > 0.0f ? (finite ? __fdiv_rn(top, 127.0f) : NAN) : 1.0f;
+    };
+    const int whole = (tasks + 31) & ~31;
+    for (int i0 = threadIdx.x; i0 < whole; i0 += 256 * UN) {
+        if (i0 != (int)threadIdx.x) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u) fetch(i0 + u * 256, x[u], y[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (i0 + u * 256 < whole) finish(task_of(i0 + u * 256), x[u], y[u]);
     }
 }
 
@@ -232,22 +293,19 @@ __device__ __forceinline__ uint32_t half2_or_nan(float x, float y) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Rows of all sequences out of their pages: a warp-wide task is 16 elements of one row, a CTA takes blocks of 16 rows of one
-// KV head of K and of V. The page ids of four blocks are fetched before the rows of any, and the rows of four before the
-// first is stored: a block alone is two dependent loads.
+// Rows of all sequences out of their pages. A thread has 16 bytes of output at a time (E elements), so that a warp's stores, and
+// its loads, are whole lines; a CTA takes blocks of 16 rows of one KV head of K and of V, UN of them at once: the page ids of
+// all are fetched before the rows of any, and all rows before the first is stored (a block alone is two dependent loads).
 template <int FMT, int D, int OUT>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
-    constexpr int per_row = D / 16, rows_per_pass = 128 / per_row;  // 128 threads for K, 128 for V
-    constexpr int passes = (16 + rows_per_pass - 1) / rows_per_pass;
-    constexpr int UN = 4 / passes > 0 ? 4 / passes : 1;
+    constexpr int E = OUT == kReadF32 ? 4 : 8;
+    constexpr int per_row = D / E, rows_per_pass = 256 / per_row > 16 ? 16 : 256 / per_row, passes = 16 / rows_per_pass;
+    constexpr int used_threads = rows_per_pass * per_row;  // (head_dim 64 in 16 bits: half of them)
+    constexpr int UN = passes >= 4 ? 1 : (passes == 2 ? 2 : 4);
     const int sub_log2 = a.pages.page_log2 - 4, Hkv = a.pages.Hkv;
-    const bool is_v = threadIdx.x >= 128;
-    const int tid = threadIdx.x & 127, r0 = tid / per_row, e = (tid % per_row) * 16;
+    const int tid = threadIdx.x % used_threads, r0 = tid / per_row, e = (tid % per_row) * E;
+    const bool idle = threadIdx.x >= used_threads;
     const int64_t blocks = ((int64_t)a.counts[1] << sub_log2) * Hkv;
-    const unsigned char* pool = is_v ? a.pages.v : a.pages.k;
-    const float* scales = is_v ? a.pages.vs : a.pages.ks;
-    void* out = is_v ? a.v_out : a.k_out;
-    const int64_t stride = is_v ? a.v_stride : a.k_stride;
     for (int64_t b0 = (int64_t)blockIdx.x * UN; b0 < blocks; b0 += (int64_t)gridDim.x * UN) {
         int slot[UN], dense[UN], used[UN], head[UN];  // of a block's first row: where it lies in the pool and in the output
 #pragma unroll
@@ -260,63 +318,65 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
                 const int2 at = a.entries[entry];
                 slot[u] = (a.table[entry] << a.pages.page_log2) + sub;
                 dense[u] = at.x + sub;
-                used[u] = max(0, min(16, at.y - sub));
+                used[u] = idle ? 0 : max(0, min(16, at.y - sub));
             }
         }
-        uint4 raw[UN * passes][FMT == KV_BF16 ? 2 : 1];
-        float scale[UN * passes];
+        uint32_t raw[2][UN * passes][FMT == KV_BF16 ? E / 2 : E / 4];
+        float scale[2][UN * passes];
 #pragma unroll
         for (int u = 0; u < UN; ++u)
 #pragma unroll
-            for (int p = 0; p < passes; ++p) {
-                const int r = p * rows_per_pass + r0, i = u * passes + p;
-                if (r >= used[u]) continue;
-                const int64_t row = a.pages.row(a.layer, slot[u] >> a.pages.page_log2, head[u], (slot[u] & ((1 << a.pages.page_log2) - 1)) + r);
-                if constexpr (FMT == KV_BF16) {
-                    const uint4* src = reinterpret_cast<const uint4*>(pool + (row * D + e) * 2);
-                    raw[i][0] = __ldg(src);
-                    raw[i][1] = __ldg(src + 1);
-                } else {
-                    raw[i][0] = __ldg(reinterpret_cast<const uint4*>(pool + row * D + e));
-                    scale[i] = __ldg(scales + row);
-                }
-            }
+            for (int p = 0; p < passes; ++p)
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-#pragma unroll
-            for (int p = 0; p < passes; ++p) {
-                const int r = p * rows_per_pass + r0, i = u * passes + p;
-                if (r >= used[u]) continue;
-                float x[16];
-                if constexpr (FMT == KV_BF16) {
-                    unpack8(raw[i][0], x);
-                    unpack8(raw[i][1], x + 8);
-                } else {
-                    const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
-                    if (OUT == kReadHalf && is_v) scale[i] *= kReadVScale;
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) x[q] = (float)(int8_t)(w[q >> 2] >> (8 * (q & 3))) * scale[i];
-                }
-                const int64_t to = (int64_t)(dense[u] + r) * stride + (int64_t)head[u] * D + e;
-                if constexpr (OUT == kReadHalf) {
-                    uint4* o = reinterpret_cast<uint4*>(static_cast<__half*>(out) + to);
-                    o[0] = make_uint4(half2_or_nan(x[0], x[1]), half2_or_nan(x[2], x[3]), half2_or_nan(x[4], x[5]), half2_or_nan(x[6], x[7]));
-                    o[1] = make_uint4(half2_or_nan(x[8], x[9]), half2_or_nan(x[10], x[11]), half2_or_nan(x[12], x[13]), half2_or_nan(x[14], x[15]));
-                } else if constexpr (OUT == kReadBf16) {
-                    uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to);
-                    if constexpr (FMT == KV_BF16) {
-                        o[0] = raw[i][0];
-                        o[1] = raw[i][1];
+                for (int v = 0; v < 2; ++v) {
+                    const int r = p * rows_per_pass + r0, i = u * passes + p;
+                    if (r >= used[u]) continue;
+                    const int64_t row = a.pages.row(a.layer, slot[u] >> a.pages.page_log2, head[u], (slot[u] & ((1 << a.pages.page_log2) - 1)) + r);
+                    const unsigned char* src = (v ? a.pages.v : a.pages.k) + (row * D + e) * (FMT == KV_BF16 ? 2 : 1);
+                    if constexpr (FMT == KV_BF16 && E == 8) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
+                        raw[v][i][0] = x.x, raw[v][i][1] = x.y, raw[v][i][2] = x.z, raw[v][i][3] = x.w;
+                    } else if constexpr (FMT == KV_BF16 || E == 8) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(src));
+                        raw[v][i][0] = x.x, raw[v][i][1] = x.y;
                     } else {
-                        o[0] = pack8(x);
-                        o[1] = pack8(x + 8);
+                        raw[v][i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
                     }
-                } else {
-                    float* o = static_cast<float*>(out) + to;
-                    store8_f32(o, x);
-                    store8_f32(o + 8, x + 8);
+                    if constexpr (FMT != KV_BF16) scale[v][i] = __ldg((v ? a.pages.vs : a.pages.ks) + row);
                 }
-            }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int p = 0; p < passes; ++p)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const int r = p * rows_per_pass + r0, i = u * passes + p;
+                    if (r >= used[u]) continue;
+                    float x[E];
+                    if constexpr (FMT == KV_BF16) {
+#pragma unroll
+                        for (int q = 0; q < E; q += 2) {
+                            x[q] = __uint_as_float(raw[v][i][q / 2] << 16);
+                            x[q + 1] = __uint_as_float(raw[v][i][q / 2] & 0xffff0000u);
+                        }
+                    } else {
+                        const float f = OUT == kReadHalf && v ? scale[v][i] * kReadVScale : scale[v][i];
+#pragma unroll
+                        for (int q = 0; q < E; ++q) x[q] = (float)(int8_t)(raw[v][i][q >> 2] >> (8 * (q & 3))) * f;
+                    }
+                    void* out = v ? a.v_out : a.k_out;
+                    const int64_t to = (int64_t)(dense[u] + r) * (v ? a.v_stride : a.k_stride) + (int64_t)head[u] * D + e;
+                    if constexpr (OUT == kReadF32) {
+                        *reinterpret_cast<float4*>(static_cast<float*>(out) + to) = make_float4(x[0], x[1], x[2], x[3]);
+                    } else if constexpr (OUT == kReadHalf) {
+                        *reinterpret_cast<uint4*>(static_cast<__half*>(out) + to) =
+                            make_uint4(half2_or_nan(x[0], x[1]), half2_or_nan(x[2], x[3]), half2_or_nan(x[4], x[5]), half2_or_nan(x[6], x[7]));
+                    } else if constexpr (FMT == KV_BF16) {
+                        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) = make_uint4(raw[v][i][0], raw[v][i][1], raw[v][i][2], raw[v][i][3]);
+                    } else {
+                        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) = pack8(x);
+                    }
+                }
     }
     if constexpr (OUT == kReadHalf) {
         const int vecs = a.q_dim / 8;
@@ -324,7 +384,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
             const int64_t row = i / vecs, d = (i - row * vecs) * 8;
             float x[8];
-            load8_in<__nv_bfloat16>(a.q + row * a.q_stride + d, x);
+            unpack8(*reinterpret_cast<const uint4*>(a.q + row * a.q_stride + d), x);
             *reinterpret_cast<uint4*>(a.q_out + row * a.q_dim + d) =
                 make_uint4(half2_or_nan(x[0], x[1]), half2_or_nan(x[2], x[3]), half2_or_nan(x[4], x[5]), half2_or_nan(x[6], x[7]));
         }

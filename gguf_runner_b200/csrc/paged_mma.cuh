@@ -309,11 +309,13 @@ struct PagedMma {
     __device__ __forceinline__ void step(uint32_t kt, const Scales& scales, bool whole, int lo0, int hi0, int lo1, int hi1, int lane) {
         const int tq = lane & 3;
         // f32: products of low parts have sums of their own, which spares the large ones two thirds of their (truncating) additions
-        float sc[2][4], lo[2][4];
+        // (and, where planes give five of them per k-step, two chains)
+        float sc[2][4], lo[2][4], lo2[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
             lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.0f;
+            lo2[j][0] = lo2[j][1] = lo2[j][2] = lo2[j][3] = 0.0f;
         }
         if constexpr (!Q8) {
             const int row = (lane & 7) + ((lane >> 4) & 1) * 8, half = (lane >> 3) & 1;
@@ -327,8 +329,8 @@ struct PagedMma {
                     ldmatrix_x4(kt + pl * MAT + piece(row, 2 * ks + half), b[0], b[1], b[2], b[3]);
 #pragma unroll
                     for (int np = 0; np < NP - pl; ++np) {
-                        mma(np + pl ? lo[0] : sc[0], f[np], b[0], b[1]);
-                        mma(np + pl ? lo[1] : sc[1], f[np], b[2], b[3]);
+                        mma(np + pl == 0 ? sc[0] : (pl == 1 ? lo2[0] : lo[0]), f[np], b[0], b[1]);
+                        mma(np + pl == 0 ? sc[1] : (pl == 1 ? lo2[1] : lo[1]), f[np], b[2], b[3]);
                     }
                 }
             }
@@ -358,7 +360,7 @@ struct PagedMma {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[j][i] += lo[j][i];
+                for (int i = 0; i < 4; ++i) sc[j][i] += PLANES ? lo[j][i] + lo2[j][i] : lo[j][i];
         }
         if constexpr (PACK) {  // the second parts of the lane's row
 #pragma unroll
@@ -601,7 +603,7 @@ struct PagedSplitKShape {
     static constexpr uint32_t SMEM = DATA + M::QBYTES + 1024;
 };
 
-// An item is 16 packed rows (f32: 8) of one sequence, fewer at its end, and a stretch of keys; blockIdx.y is the KV head.
+// An item is 16 packed rows (f32: 8) of one sequence, fewer at its end, and a stretch of keys; blockIdx.x is the KV head.
 template <int D, int FMT, bool F32>
 __global__ void __launch_bounds__(PagedSplitKShape<D, FMT, F32>::W * 32, 1)
 paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedAttnArgs a) {
@@ -617,7 +619,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     __shared__ int s_abort, s_last, s_bad;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.y;
+    const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.x;
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     const uint32_t ring = base + warp * NST * M::TILE;
@@ -632,7 +634,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
     const int n_items = a.plan.counts[0];
     uint32_t used = 0;  // tiles this warp has been through: ring position and phase
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int item = blockIdx.y; item < n_items; item += gridDim.y) {
         const PagedItem w = a.plan.items[item];
         const int n_tiles = (w.key1 - w.key0 + 15) >> 4, mine = n_tiles > warp ? (n_tiles - warp + W - 1) / W : 0;
         // keys that some row, and that every row, of the tile sees
@@ -829,7 +831,7 @@ struct PagedRowsShape {
     static constexpr int THREADS = W * 32 + 128;
 };
 
-// An item is up to 128 packed rows (f32 at head_dim 256: 64) of one sequence and all the keys that they see; blockIdx.y is the KV
+// An item is up to 128 packed rows (f32 at head_dim 256: 64) of one sequence and all the keys that they see; blockIdx.x is the KV
 // head.
 template <int D, int FMT, bool F32>
 __global__ void __launch_bounds__(PagedRowsShape<D, FMT, F32>::THREADS, 1)
@@ -842,7 +844,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     __shared__ __align__(8) uint64_t s_full[NST], s_empty[NST], s_raw;
     __shared__ int s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.y;
+    const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.x;
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     volatile int* abortp = &s_abort;
@@ -866,7 +868,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if constexpr (S::W == 8) reg_release<56>();
         uint32_t raws = 0;
         bool ok = warp == S::W;
-        for (int item = blockIdx.x; ok && item < n_items; item += gridDim.x) {
+        for (int item = blockIdx.y; ok && item < n_items; item += gridDim.y) {
             const PagedItem w = a.plan.items[item];
             const int n_stages = (w.key1 - w.key0 + KT - 1) / KT, any_lo = any_lo_of(w), any_hi = any_hi_of(w);
             for (int t = 0; t < n_stages; ++t, ++used) {
@@ -904,7 +906,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
     } else {
         if constexpr (S::W == 8) reg_acquire<224>();
-        for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        for (int item = blockIdx.y; item < n_items; item += gridDim.y) {
             const PagedItem w = a.plan.items[item];
             const int n_stages = (w.key1 - w.key0 + KT - 1) / KT;
             const int r0 = w.row0 + warp * 16, r1 = w.row0 + w.rows;  // this warp's rows, cut at r1

@@ -543,52 +543,63 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
 }
 
-// Weighs the pieces of every pair of query tiles that was cut: a warp per row, pieces in the order of their keys. The list holds
-// the first piece of each pair.
+// Weighs the pieces of every pair of query tiles that was cut, in the order of their keys. D / 4 lanes share a row, 16 bytes of
+// each piece apiece, so that a row costs two round trips: the pieces' (m, l), then their rows. The list holds the first piece of
+// each pair.
 template <int D>
 __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_constant__ PagedTcArgs p) {
     grid_wait();
     const PagedAttnArgs& a = p.a;
-    constexpr int V = D / 32;  // elements of a lane
-    const int lane = threadIdx.x & 31;
+    constexpr int L = D / 4, PER = 256 / L;  // lanes of a row, rows of a CTA
+    const int lane = threadIdx.x & 31, sub = threadIdx.x % L;
     const int n = a.plan.counts[0] * 256;
-    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
+    for (int i = blockIdx.x * PER + threadIdx.x / L; i < n; i += gridDim.x * PER) {
         const PagedItem& w = a.plan.items[i >> 8];
         const int r = i & 255, t = r >> 7, tile_tok = (r & 127) / a.G, head = (r & 127) - tile_tok * a.G;
         const int tok = w.row0 + t * p.tiles_tokens + tile_tok;
-        if (tile_tok >= p.tiles_tokens || tok >= w.n_tok) continue;
+        const bool valid = tile_tok < p.tiles_tokens && tok < w.n_tok;
         const float* state = p.part + (int64_t)w.part * kPtState<D>;
-        float top = -INFINITY;
-        for (int s = lane; s < w.n_split; s += 32)
-            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(state + (int64_t)s * kPtState<D> + 256 * D) + r).x);
-        top = warp_max(top);
-        float o[V] = {}, l = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < w.n_split; ++s) {
-            const float* st = state + (int64_t)s * kPtState<D>;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(st + 256 * D) + r);
-            if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing seen: no rows were left either
-            const float f = tc::ex2((ml.x - top) * a.c);
-            l = fmaf(f, ml.y, l);
+        // pieces in groups of L: a lane holds (m, l) of one, then its weight
+        float top = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const int n_split = w.n_split;
+        for (int s0 = 0; s0 < n_split; s0 += L) {
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (valid && s0 + sub < n_split) ml = __ldcg(reinterpret_cast<const float2*>(state + (int64_t)(s0 + sub) * kPtState<D> + 256 * D) + r);
+            float m = ml.x;
 #pragma unroll
-            for (int e = 0; e < V / 2; ++e) {
-                const float2 x = __ldcg(reinterpret_cast<const float2*>(st + (int64_t)r * D + e * 64) + lane);
-                o[2 * e] = fmaf(f, x.x, o[2 * e]);
-                o[2 * e + 1] = fmaf(f, x.y, o[2 * e + 1]);
+            for (int k = L / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+            const float now = fmaxf(top, m), back = top == -INFINITY ? 0.0f : tc::ex2((top - now) * a.c);
+            top = now;
+            l *= back;
+            o = make_float4(o.x * back, o.y * back, o.z * back, o.w * back);
+            // (nothing seen, and so no rows left: weight 0; a NaN stays one)
+            const bool none = ml.x == -INFINITY && ml.y == 0.0f;
+            const float f = none ? 0.0f : tc::ex2((ml.x - now) * a.c);
+            const int here = min(L, n_split - s0);
+#pragma unroll 4
+            for (int s = 0; s < here; ++s) {
+                const int from = (lane & ~(L - 1)) + s;
+                const float fs = __shfl_sync(0xffffffffu, f, from), ls = __shfl_sync(0xffffffffu, ml.y, from);
+                const int skip = __shfl_sync(0xffffffffu, none ? 1 : 0, from);  // (by all lanes: head_dim 64 has two rows in a warp)
+                if (!valid || skip) continue;
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(state + (int64_t)(s0 + s) * kPtState<D> + (int64_t)r * D) + sub);
+                l = fmaf(fs, ls, l);
+                o.x = fmaf(fs, x.x, o.x);
+                o.y = fmaf(fs, x.y, o.y);
+                o.z = fmaf(fs, x.z, o.z);
+                o.w = fmaf(fs, x.w, o.w);
             }
         }
         const float inv = p.out_scale / l;
-        bool bad = false;
-        uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D);
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-            const float x = o[2 * e] * inv, y = o[2 * e + 1] * inv;
-            bad |= !isfinite(x) | !isfinite(y);
-            out[e * 32 + lane] = pack_bf16x2(x, y);
-        }
-        if (__any_sync(0xffffffffu, bad)) {
-            __syncwarp();
-            paged_row_again<D, false>(a, w, w.kvh, tok * a.G + head, lane);
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        const bool bad = valid && !finite4(o);
+        if (valid) paged_store4<false>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D + sub * 4, o);
+        unsigned again = __ballot_sync(0xffffffffu, bad);
+        while (again) {
+            const int from = __ffs(again) - 1;
+            again &= ~((L == 32 ? 0xffffffffu : ((1u << L) - 1)) << (from & ~(L - 1)));
+            paged_row_again<D, false>(a, w, w.kvh, __shfl_sync(0xffffffffu, tok * a.G + head, from), lane);
         }
     }
 }
