@@ -20,6 +20,7 @@
 #include "paged.cuh"
 #include "paged_mma.cuh"
 #include "paged_tc.cuh"
+#include "paged_tc_wide.cuh"
 #include "path_view.h"
 
 using namespace ggr;
@@ -32,7 +33,7 @@ struct ggr_pages {
     PageView v{};
     void* owned[4] = {nullptr, nullptr, nullptr, nullptr};
     CUtensorMap tmK16, tmV16;    // 16 rows of a page, one 64- or 128-byte block of columns
-    CUtensorMap tmK128, tmV128;  // bf16: min(page_size, 128) rows
+    CUtensorMap tmK128, tmV128;  // bf16: min(page_size, 128) rows (head_dim 256: at most 64)
 };
 
 namespace {
@@ -40,6 +41,9 @@ namespace {
 // Packed rows (new tokens times query heads of a KV head) of a sequence above which it goes to the tcgen05 kernel, and above
 // which (32-bit precision, head_dim 256) to the kernel whose warps share the keys.
 constexpr int kTcMinRows = 64, kRowsMinRows = 64;
+// Keys of a tile of the tcgen05 kernels, query tiles of an item
+constexpr int tc_key_tile(int D) { return D == 256 ? kPwBN : 128; }
+constexpr int tc_item_tiles(int D) { return D == 256 ? 1 : 2; }
 constexpr int kMaxLists = 4;  // distinct windows of a model's layers
 // lists of a plan: items of the three attention kernels, and the pairs of query tiles whose pieces are merged
 enum Kind { kSplitK = 0, kRows = 1, kTc = 2, kMerge = 3, kKinds = 4 };
@@ -192,9 +196,9 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
 // The same for the tcgen05 kernel. `tiles`: 128-key tiles of every pair of query tiles, longest first, of which each stands for Hkv
 // items. Items are taken longest first by whichever SM is free, so that only the last ones matter: those after the last whole
 // wave are cut, so far that the SMs end together. A step over a tile takes 2.4 us, an item 3 us besides (its start, its
-// epilogue), a piece's rows one more, and the merge 4. Returns how many pairs stay whole; *piece: the size of the others' pieces.
-int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, int* piece) {
-    constexpr double t = 2.4;
+// epilogue; at head_dim 256 0.75 per 64-key tile and 6), a piece's rows one more, and the merge 4 and 0.03 per piece. Returns how many pairs stay whole; *piece: the size of the others' pieces.
+int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, bool wide, int* piece) {
+    const double t = wide ? 0.75 : 2.4, t0 = wide ? 6.0 : 3.0;
     const int n = (int)tiles.size();
     int best_whole = n;
     double best_cost = -1.0;
@@ -212,12 +216,12 @@ int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t m
             std::push_heap(ends.begin(), ends.end(), std::greater<double>());
         };
         for (int i = 0; i < whole; ++i)
-            for (int h = 0; h < Hkv; ++h) add(3.0 + tiles[i] * t);
+            for (int h = 0; h < Hkv; ++h) add(t0 + tiles[i] * t);
         for (int i = whole; i < n; ++i) {
             const int k = (tiles[i] + size - 1) / size;
-            for (int h = 0; h < Hkv * k; ++h) add(4.0 + (double)((tiles[i] + k - 1) / k) * t);
+            for (int h = 0; h < Hkv * k; ++h) add(t0 + 1.0 + (double)((tiles[i] + k - 1) / k) * t);
         }
-        const double cost = last + (whole < n ? 4.0 : 0.0);
+        const double cost = last + (whole < n ? 4.0 + 0.03 * cut : 0.0);
         if (best_cost < 0.0 || cost < best_cost) {
             best_cost = cost;
             best_whole = whole;
@@ -301,10 +305,10 @@ extern "C" int ggr_pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_s
             for (void* x : pg->owned) cudaFree(x);
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pool");
         }
-    if (!q8 && p.D <= 128)
+    if (!q8)
         for (int i = 0; i < 2; ++i)
             if (!make_map3(i ? &pg->tmV128 : &pg->tmK128, false, i ? view.v : view.k, p.D, page_size, groups, row_bytes, row_bytes * page_size, 64,
-                           std::min(page_size, 128), 1)) {
+                           std::min(page_size, tc_key_tile(p.D)), 1)) {
                 for (void* x : pg->owned) cudaFree(x);
                 return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pool");
             }
@@ -392,10 +396,10 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     b->rows_step = dtype == GGR_DTYPE_F32 && p.D == 256 ? 64 : 128;
     b->item_cap[kSplitK] = (rows + step - 1) / step + max_seqs + b->part_tiles;
     b->item_cap[kRows] = (rows + b->rows_step - 1) / b->rows_step + max_seqs;
-    b->tc = dtype == GGR_DTYPE_BF16 && p.D <= 128 && p.G <= 128;
+    b->tc = dtype == GGR_DTYPE_BF16 && p.G <= 128;
     if (b->tc) {
         b->tc_tokens = 128 / p.G;
-        const size_t pairs = (((size_t)max_tokens + 2 * b->tc_tokens - 1) / (2 * b->tc_tokens) + max_seqs) * p.Hkv;
+        const size_t item_tokens = tc_item_tiles(p.D) * b->tc_tokens, pairs = (((size_t)max_tokens + item_tokens - 1) / item_tokens + max_seqs) * p.Hkv;
         b->tc_parts = 2 * (size_t)p.sm_count;
         b->item_cap[kTc] = pairs + b->tc_parts;
         b->item_cap[kMerge] = b->tc_parts;
@@ -424,7 +428,7 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
     if (ok && !pages && dtype == GGR_DTYPE_F32)
         ok = cudaMalloc((void**)&b->d_planes, (size_t)6 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
     if (ok && b->tc)
-        ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 256 * (p.D + 2) * sizeof(float)) == cudaSuccess &&
+        ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 128 * tc_item_tiles(p.D) * (p.D + 2) * sizeof(float)) == cudaSuccess &&
              cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
     if (ok && b->tc && pages && pages->v.fmt == GGR_KV_Q8_HEAD)
         ok = cudaMalloc((void**)&b->d_q16, (size_t)max_tokens * p.Hq * p.D * sizeof(__half)) == cudaSuccess;
@@ -549,8 +553,8 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
             b->dense_rows = 0;
             const size_t want = (size_t)std::max<int64_t>(dense, 4096);
             if (want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__half)) == cudaSuccess) {
-                if (!make_map3(&b->tmKd, false, b->d_dense, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128) ||
-                    !make_map3(&b->tmVd, false, b->d_dense + want * row, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, 128))
+                if (!make_map3(&b->tmKd, false, b->d_dense, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, tc_key_tile(b->D)) ||
+                    !make_map3(&b->tmVd, false, b->d_dense + want * row, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, tc_key_tile(b->D)))
                     return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the dequantised rows");
                 b->dense_rows = want;
             } else {
@@ -587,11 +591,13 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
         const int window = b->windows[l];
         std::vector<Tile> tiles[kKinds];
         std::vector<int> pair_tiles;
+        const int kt = tc_key_tile(b->D);
         for (int i = 0; i < n_seqs; ++i) {
             const int first = kv_len[i] - q_len[i], n_rows = q_len[i] * b->G;
             if (kind[i] == kTc) {
-                for (int t = 0; t < q_len[i]; t += 2 * b->tc_tokens) {
-                    const int lo = first_key(first + t, window) & ~127, hi = std::min(first + t + 2 * b->tc_tokens, kv_len[i]);
+                const int step = tc_item_tiles(b->D) * b->tc_tokens;
+                for (int t = 0; t < q_len[i]; t += step) {
+                    const int lo = first_key(first + t, window) & ~(kt - 1), hi = std::min(first + t + step, kv_len[i]);
                     tiles[kTc].push_back({i, t, 0, lo, hi});
                 }
                 continue;
@@ -639,11 +645,11 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
         }
         {
             PagedItem* merge = reinterpret_cast<PagedItem*>(h + b->at_items[l][kMerge]);
-            auto n_tiles = [](const Tile& t) { return (t.key1 - t.key0 + 127) / 128; };
+            auto n_tiles = [kt](const Tile& t) { return (t.key1 - t.key0 + kt - 1) / kt; };
             std::stable_sort(tiles[kTc].begin(), tiles[kTc].end(), [&](const Tile& x, const Tile& y) { return n_tiles(x) > n_tiles(y); });
             for (const Tile& t : tiles[kTc]) pair_tiles.push_back(n_tiles(t));
             int n = 0, n_merge = 0, part = 0, piece = 1;
-            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, &piece);
+            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, b->D == 256, &piece);
             b->scratch.clear();
             for (const Tile& t : tiles[kTc]) {
                 const bool cut = &t - tiles[kTc].data() >= whole;
@@ -664,8 +670,8 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
                     }
                     for (int s = 0; s < it.n_split; ++s) {
                         it.split = s;
-                        it.key0 = t.key0 + s * each * 128;
-                        it.key1 = std::min(t.key1, it.key0 + each * 128);
+                        it.key0 = t.key0 + s * each * kt;
+                        it.key1 = std::min(t.key1, it.key0 + each * kt);
                         b->scratch.push_back(it);
                         if (s == 0 && it.n_split > 1) merge[n_merge++] = it;
                     }
@@ -747,63 +753,70 @@ int read_grid(const ggr_batch* b, int64_t entries) {
 
 template <int D, int FMT>
 int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& args, int rows, bool capturing) {
-    if constexpr (D <= 128) {
-        constexpr bool q8 = FMT == kKvQ8Head;
-        if constexpr (q8) {
-            ReadArgs r{};
-            r.pages = b->pages->v;
-            r.counts = b->dense_counts();
-            r.table = reinterpret_cast<const int*>(b->d_plan + b->at_dense_table);
-            r.entries = reinterpret_cast<const int2*>(b->d_plan + b->at_dense_entries);
-            r.layer = args.layer;
-            r.k_out = b->d_dense;
-            r.v_out = b->d_dense + b->dense_rows * b->Hkv * b->D;
-            r.k_stride = r.v_stride = (int64_t)b->Hkv * b->D;
-            r.q = static_cast<const __nv_bfloat16*>(args.q);
-            r.q_stride = args.q_stride;
-            r.q_out = b->d_q16;
-            r.q_dim = b->Hq * D;
-            {
-                PathTimer t(c, 1);
-                paged_read_kernel<kKvQ8Head, D, kReadHalf><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
-            }
-            PAGED_TRY(c, cudaGetLastError());
-            path_launched(c);
+    constexpr bool q8 = FMT == kKvQ8Head;
+    if constexpr (q8) {
+        ReadArgs r{};
+        r.pages = b->pages->v;
+        r.counts = b->dense_counts();
+        r.table = reinterpret_cast<const int*>(b->d_plan + b->at_dense_table);
+        r.entries = reinterpret_cast<const int2*>(b->d_plan + b->at_dense_entries);
+        r.layer = args.layer;
+        r.k_out = b->d_dense;
+        r.v_out = b->d_dense + b->dense_rows * b->Hkv * b->D;
+        r.k_stride = r.v_stride = (int64_t)b->Hkv * b->D;
+        r.q = static_cast<const __nv_bfloat16*>(args.q);
+        r.q_stride = args.q_stride;
+        r.q_out = b->d_q16;
+        r.q_dim = b->Hq * D;
+        {
+            PathTimer t(c, 1);
+            paged_read_kernel<kKvQ8Head, D, kReadHalf><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
         }
-        PagedTcArgs t{};
-        t.a = args;
-        t.a.plan.counts = b->counts(list, kTc);
-        t.a.plan.items = b->items(list, kTc);
-        t.tiles_tokens = b->tc_tokens;
-        t.box_rows = b->pages ? std::min(b->pages->page_size, 128) : 128;
-        t.linear = !b->pages || q8;
-        t.out_scale = q8 ? 1.0f / kReadVScale : 1.0f;
-        t.sched = b->d_sched;
-        t.part = b->d_tc_part;
-        CUtensorMap tq;
-        // (tensor maps move 16-bit elements as they are: bf16 stands for f16 too)
+        PAGED_TRY(c, cudaGetLastError());
+        path_launched(c);
+    }
+    PagedTcArgs t{};
+    t.a = args;
+    t.a.plan.counts = b->counts(list, kTc);
+    t.a.plan.items = b->items(list, kTc);
+    t.tiles_tokens = b->tc_tokens;
+    t.box_rows = b->pages ? std::min(b->pages->page_size, tc_key_tile(D)) : tc_key_tile(D);
+    t.linear = !b->pages || q8;
+    t.out_scale = q8 ? 1.0f / kReadVScale : 1.0f;
+    t.sched = b->d_sched;
+    t.part = b->d_tc_part;
+    // (tensor maps move 16-bit elements as they are: bf16 stands for f16 too)
+    const CUtensorMap &tk = q8 ? b->tmKd : *m.k128, &tv = q8 ? b->tmVd : *m.v128;
+    const int n = b->n_items[list][kTc];
+    if constexpr (D == 256) {
+        static KernelSmemSetup setup;
+        PAGED_TRY(c, setup.ensure(paged_tc_wide_kernel<q8>, p.device, p.smem_optin, (int)kPwSmem));
+        t.q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
+        t.q_rows_stride = q8 ? b->Hq * D : args.q_stride;
+        PathTimer timer(c, 0);
+        paged_tc_wide_kernel<q8><<<capturing ? (int)b->item_cap[kTc] : n, kPwThreads, kPwSmem, p.stream>>>(tk, tv, t);
+    } else {
         const void* q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
+        CUtensorMap tq;
         if (!make_map3(&tq, false, q_rows, D, b->Hq, rows, (uint64_t)D * 2, (uint64_t)(q8 ? b->Hq * D : args.q_stride) * 2, 64, b->G, b->tc_tokens))
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the query rows");
         static KernelSmemSetup setup;
         PAGED_TRY(c, setup.ensure(paged_tc_kernel<D, q8>, p.device, p.smem_optin, (int)kPtSmem<D>));
-        {
-            PathTimer timer(c, 0);
-            paged_tc_kernel<D, q8><<<capturing ? b->sm_count : std::min(b->sm_count, b->n_items[list][kTc]), kPtThreads, kPtSmem<D>, p.stream>>>(
-                tq, q8 ? b->tmKd : *m.k128, q8 ? b->tmVd : *m.v128, t);
-        }
-        PAGED_TRY(c, cudaGetLastError());
-        path_launched(c);
-        if (!capturing && !b->n_items[list][kMerge]) return GGR_OK;
-        t.a.plan.counts = b->counts(list, kMerge);
-        t.a.plan.items = b->items(list, kMerge);
-        const int pairs = capturing ? (int)b->tc_parts / 2 : b->n_items[list][kMerge];
-        {
-            PathTimer timer(c, 2);
-            PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(std::min(pairs * D / 4, 16 * b->sm_count)), 256, 0, p.stream, t));
-        }
-        path_launched(c);
+        PathTimer timer(c, 0);
+        paged_tc_kernel<D, q8><<<capturing ? b->sm_count : std::min(b->sm_count, n), kPtThreads, kPtSmem<D>, p.stream>>>(tq, tk, tv, t);
     }
+    PAGED_TRY(c, cudaGetLastError());
+    path_launched(c);
+    if (!capturing && !b->n_items[list][kMerge]) return GGR_OK;
+    t.a.plan.counts = b->counts(list, kMerge);
+    t.a.plan.items = b->items(list, kMerge);
+    const int cut = capturing ? (int)b->tc_parts / 2 : b->n_items[list][kMerge];
+    {
+        PathTimer timer(c, 2);
+        const int grid = std::min(cut * (D == 256 ? 16 : D / 4), 16 * b->sm_count);
+        PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(grid), 256, 0, p.stream, t));
+    }
+    path_launched(c);
     return GGR_OK;
 }
 
@@ -838,7 +851,7 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
         path_launched(c);
         if (capturing) b->captured |= 1u << k;
     }
-    if constexpr (!F32 && D <= 128) {
+    if constexpr (!F32) {
         if (b->n_items[list][kTc]) {
             const int rc = launch_tc<D, FMT>(c, p, b, list, m, a, rows, capturing);
             if (rc) return rc;
@@ -1059,8 +1072,8 @@ extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer
     const uint64_t sy = (uint64_t)b->D * 2;
     if (!make_map3(&tk, false, k, b->D, b->Hkv, rows, sy, (uint64_t)k_stride * 2, 64, 1, 16) ||
         !make_map3(&tv, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, 16) ||
-        !make_map3(&tk128, false, k, b->D, b->Hkv, rows, sy, (uint64_t)k_stride * 2, 64, 1, 128) ||
-        !make_map3(&tv128, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, 128))
+        !make_map3(&tk128, false, k, b->D, b->Hkv, rows, sy, (uint64_t)k_stride * 2, 64, 1, tc_key_tile(b->D)) ||
+        !make_map3(&tv128, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, tc_key_tile(b->D)))
         return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
     return launch_by_dim<KV_BF16, false>(c, p, b, list, m, a, rows, capturing);
 }

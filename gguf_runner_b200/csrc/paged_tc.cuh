@@ -27,6 +27,8 @@ struct PagedTcArgs {
     int tiles_tokens;  // tokens of a query tile: 128 / G
     int box_rows;      // paged: rows of one copy, min(page_size, 128)
     int linear;        // K and V tiles come from dense rows (packed prompts, or 8-bit pages read into f16 rows)
+    const void* q_rows;      // head_dim 256: the 16-bit rows of q that are multiplied (of 8-bit pages the f16 ones)
+    int64_t q_rows_stride;
     float out_scale;   // of the merged rows: 1 / kReadVScale for f16 rows
     int* sched;        // [0] items handed out beyond the first wave, [1] CTAs that have left
     float* part;       // states of pieces: [256][D], then [256] (m, l)
@@ -543,36 +545,40 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
 }
 
-// Weighs the pieces of every pair of query tiles that was cut, in the order of their keys. D / 4 lanes share a row, 16 bytes of
-// each piece apiece, so that a row costs two round trips: the pieces' (m, l), then their rows. The list holds the first piece of
-// each pair.
+// Weighs the pieces of every cut item, in the order of their keys. L lanes share a row, 16 bytes of each piece apiece (head_dim
+// 256: twice), so that a row costs two round trips: the pieces' (m, l), then their rows. The list holds the first piece of each
+// item; ROWS: of an item (two query tiles, at head_dim 256 one).
 template <int D>
 __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_constant__ PagedTcArgs p) {
     grid_wait();
     const PagedAttnArgs& a = p.a;
-    constexpr int L = D / 4, PER = 256 / L;  // lanes of a row, rows of a CTA
+    constexpr int ROWS = D == 256 ? 128 : 256, STATE = ROWS * (D + 2);
+    constexpr int L = D == 64 ? 16 : 32, V = D / (4 * L), PER = 256 / L;  // lanes of a row, 16-byte pieces of a lane, rows of a CTA
     const int lane = threadIdx.x & 31, sub = threadIdx.x % L;
-    const int n = a.plan.counts[0] * 256;
+    const int n = a.plan.counts[0] * ROWS;
     for (int i = blockIdx.x * PER + threadIdx.x / L; i < n; i += gridDim.x * PER) {
-        const PagedItem& w = a.plan.items[i >> 8];
-        const int r = i & 255, t = r >> 7, tile_tok = (r & 127) / a.G, head = (r & 127) - tile_tok * a.G;
+        const PagedItem& w = a.plan.items[i / ROWS];
+        const int r = i % ROWS, t = r >> 7, tile_tok = (r & 127) / a.G, head = (r & 127) - tile_tok * a.G;
         const int tok = w.row0 + t * p.tiles_tokens + tile_tok;
         const bool valid = tile_tok < p.tiles_tokens && tok < w.n_tok;
-        const float* state = p.part + (int64_t)w.part * kPtState<D>;
+        const float* state = p.part + (int64_t)w.part * STATE;
         // pieces in groups of L: a lane holds (m, l) of one, then its weight
         float top = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float4 o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const int n_split = w.n_split;
         for (int s0 = 0; s0 < n_split; s0 += L) {
             float2 ml = make_float2(-INFINITY, 0.0f);
-            if (valid && s0 + sub < n_split) ml = __ldcg(reinterpret_cast<const float2*>(state + (int64_t)(s0 + sub) * kPtState<D> + 256 * D) + r);
+            if (valid && s0 + sub < n_split) ml = __ldcg(reinterpret_cast<const float2*>(state + (int64_t)(s0 + sub) * STATE + ROWS * D) + r);
             float m = ml.x;
 #pragma unroll
             for (int k = L / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
             const float now = fmaxf(top, m), back = top == -INFINITY ? 0.0f : tc::ex2((top - now) * a.c);
             top = now;
             l *= back;
-            o = make_float4(o.x * back, o.y * back, o.z * back, o.w * back);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] = make_float4(o[v].x * back, o[v].y * back, o[v].z * back, o[v].w * back);
             // (nothing seen, and so no rows left: weight 0; a NaN stays one)
             const bool none = ml.x == -INFINITY && ml.y == 0.0f;
             const float f = none ? 0.0f : tc::ex2((ml.x - now) * a.c);
@@ -583,22 +589,30 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_consta
                 const float fs = __shfl_sync(0xffffffffu, f, from), ls = __shfl_sync(0xffffffffu, ml.y, from);
                 const int skip = __shfl_sync(0xffffffffu, none ? 1 : 0, from);  // (by all lanes: head_dim 64 has two rows in a warp)
                 if (!valid || skip) continue;
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(state + (int64_t)(s0 + s) * kPtState<D> + (int64_t)r * D) + sub);
                 l = fmaf(fs, ls, l);
-                o.x = fmaf(fs, x.x, o.x);
-                o.y = fmaf(fs, x.y, o.y);
-                o.z = fmaf(fs, x.z, o.z);
-                o.w = fmaf(fs, x.w, o.w);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4*>(state + (int64_t)(s0 + s) * STATE + (int64_t)r * D) + v * L + sub);
+                    o[v].x = fmaf(fs, x.x, o[v].x);
+                    o[v].y = fmaf(fs, x.y, o[v].y);
+                    o[v].z = fmaf(fs, x.z, o[v].z);
+                    o[v].w = fmaf(fs, x.w, o[v].w);
+                }
             }
         }
         const float inv = p.out_scale / l;
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        const bool bad = valid && !finite4(o);
-        if (valid) paged_store4<false>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D + sub * 4, o);
+        bool bad = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            o[v] = make_float4(o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
+            bad |= valid && !finite4(o[v]);
+            if (valid) paged_store4<false>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D + (v * L + sub) * 4, o[v]);
+        }
         unsigned again = __ballot_sync(0xffffffffu, bad);
         while (again) {
             const int from = __ffs(again) - 1;
             again &= ~((L == 32 ? 0xffffffffu : ((1u << L) - 1)) << (from & ~(L - 1)));
+            __syncwarp();
             paged_row_again<D, false>(a, w, w.kvh, __shfl_sync(0xffffffffu, tok * a.G + head, from), lane);
         }
     }
