@@ -3025,6 +3025,7 @@ RopeParams path_rope(const ggr_attn_ctx* c, int layer) { return rope_params(c, l
 int path_fail(ggr_attn_ctx* c, int status, const std::string& msg) { return fail(c, status, msg); }
 void path_create_error(const std::string& msg) { g_create_err = msg; }
 bool path_capturing(ggr_attn_ctx* c) { return capturing(c); }
+bool path_timing(const ggr_attn_ctx* c) { return c->timing; }
 void path_launched(ggr_attn_ctx* c) { c->launches++; }
 cudaEvent_t path_timer_start(ggr_attn_ctx* c, int kind) {
     LaunchTimer t(c, kind);

@@ -194,34 +194,38 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
 }
 
 // The same for the tcgen05 kernel. `tiles`: 128-key tiles of every pair of query tiles, longest first, of which each stands for Hkv
-// items. Items are taken longest first by whichever SM is free, so that only the last ones matter: those after the last whole
-// wave are cut, so far that the SMs end together. A step over a tile takes 2.4 us, an item 3 us besides (its start, its
+// items. Items are taken longest first by whichever SM is free, so that only the longest and the last ones matter: those
+// above some length or after some whole wave are cut, so far that the SMs end together. A step over a tile takes 2.1 us, an item 3 us besides (its start, its
 // epilogue; at head_dim 256 0.75 per 64-key tile and 6), a piece's rows one more, and the merge 4 and 0.03 per piece. Returns how many pairs stay whole; *piece: the size of the others' pieces.
 int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, bool wide, int* piece) {
-    const double t = wide ? 0.75 : 2.4, t0 = wide ? 6.0 : 3.0;
+    const double t = wide ? 0.75 : 2.1, t0 = wide ? 6.0 : 3.0;
     const int n = (int)tiles.size();
     int best_whole = n;
     double best_cost = -1.0;
     std::vector<double> ends;
+    std::vector<std::pair<int, int>> sizes;  // tiles of a piece, how many such (negative: cut)
     auto consider = [&](int whole, int size) {
         size_t cut = 0;
-        for (int i = whole; i < n; ++i) cut += (tiles[i] + size - 1) / size * Hkv;
+        for (int i = whole; i < n; ++i) cut += tiles[i] > size ? (size_t)(tiles[i] + size - 1) / size * Hkv : 0;
         if (cut > max_pieces) return;
-        // (a heap of the times at which the SMs are free)
+        // pieces in the order they are taken in, onto a heap of the times at which the SMs are free
+        sizes.clear();
+        for (int i = 0; i < n; ++i) {
+            const int k = i < whole ? 1 : (tiles[i] + size - 1) / size;
+            sizes.emplace_back((tiles[i] + k - 1) / k, k * Hkv * (k > 1 ? -1 : 1));
+        }
+        std::stable_sort(sizes.begin(), sizes.end(), [](const auto& x, const auto& y) { return x.first > y.first; });
         ends.assign(sm_count, 0.0);
         double last = 0.0;
-        auto add = [&](double d) {
-            std::pop_heap(ends.begin(), ends.end(), std::greater<double>());
-            last = std::max(last, ends.back() += d);
-            std::push_heap(ends.begin(), ends.end(), std::greater<double>());
-        };
-        for (int i = 0; i < whole; ++i)
-            for (int h = 0; h < Hkv; ++h) add(t0 + tiles[i] * t);
-        for (int i = whole; i < n; ++i) {
-            const int k = (tiles[i] + size - 1) / size;
-            for (int h = 0; h < Hkv * k; ++h) add(t0 + 1.0 + (double)((tiles[i] + k - 1) / k) * t);
+        for (const auto& s : sizes) {
+            const double d = t0 + (s.second < 0 ? 1.0 : 0.0) + s.first * t;
+            for (int k = std::abs(s.second); k > 0; --k) {
+                std::pop_heap(ends.begin(), ends.end(), std::greater<double>());
+                last = std::max(last, ends.back() += d);
+                std::push_heap(ends.begin(), ends.end(), std::greater<double>());
+            }
         }
-        const double cost = last + (whole < n ? 4.0 + 0.03 * cut : 0.0);
+        const double cost = last + (cut ? 4.0 + 0.03 * cut : 0.0);
         if (best_cost < 0.0 || cost < best_cost) {
             best_cost = cost;
             best_whole = whole;
@@ -231,11 +235,15 @@ int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t m
     *piece = 1;
     if (!n || (int64_t)n * Hkv > 8 * sm_count) return n;
     consider(n, 1);
+    // the longest ones, wherever they stand (ragged lengths)
+    for (double f : {0.85, 0.7, 0.5, 0.34, 0.25, 0.17})
+        if (tiles[0] * f >= 2.0) consider(0, (int)std::ceil(tiles[0] * f));
+    // and the last wave of equal ones
     const int waves = (int)((int64_t)n * Hkv / sm_count);
-    for (int w = waves; w >= std::max(0, waves - 1); --w) {
+    for (int w = waves; w >= std::max(1, waves - 1); --w) {
         const int whole = (int)((int64_t)w * sm_count / Hkv);
         if (whole >= n) continue;
-        for (int k : {2, 3, 4, 5, 6, 8, 12, 16})
+        for (int k : {2, 3, 4, 6, 8, 12})
             if (tiles[whole] / k >= 2) consider(whole, (tiles[whole] + k - 1) / k);
     }
     return best_whole;
@@ -751,10 +759,10 @@ int read_grid(const ggr_batch* b, int64_t entries) {
     return (int)std::min<int64_t>((blocks + 1) / 2, (int64_t)16 * b->sm_count);
 }
 
-template <int D, int FMT>
-int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& args, int rows, bool capturing) {
-    constexpr bool q8 = FMT == kKvQ8Head;
-    if constexpr (q8) {
+// 8-bit pages and q as the f16 rows that the tcgen05 kernels multiply
+template <int D>
+int launch_dense_rows(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, const PagedAttnArgs& args, bool capturing) {
+    {
         ReadArgs r{};
         r.pages = b->pages->v;
         r.counts = b->dense_counts();
@@ -775,7 +783,15 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
     }
+    return GGR_OK;
+}
+
+// `behind`: right behind a warp-level kernel of the same call that lets it in
+template <int D, int FMT>
+int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const Maps& m, const PagedAttnArgs& args, int rows, bool capturing, bool behind) {
+    constexpr bool q8 = FMT == kKvQ8Head;
     PagedTcArgs t{};
+    t.behind = behind;
     t.a = args;
     t.a.plan.counts = b->counts(list, kTc);
     t.a.plan.items = b->items(list, kTc);
@@ -794,7 +810,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         t.q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
         t.q_rows_stride = q8 ? b->Hq * D : args.q_stride;
         PathTimer timer(c, 0);
-        paged_tc_wide_kernel<q8><<<capturing ? (int)b->item_cap[kTc] : n, kPwThreads, kPwSmem, p.stream>>>(tk, tv, t);
+        PAGED_TRY(c, launch_chained(behind, paged_tc_wide_kernel<q8>, dim3(capturing ? (int)b->item_cap[kTc] : n), kPwThreads, kPwSmem, p.stream, tk, tv, t));
     } else {
         const void* q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
         CUtensorMap tq;
@@ -803,7 +819,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         static KernelSmemSetup setup;
         PAGED_TRY(c, setup.ensure(paged_tc_kernel<D, q8>, p.device, p.smem_optin, (int)kPtSmem<D>));
         PathTimer timer(c, 0);
-        paged_tc_kernel<D, q8><<<capturing ? b->sm_count : std::min(b->sm_count, n), kPtThreads, kPtSmem<D>, p.stream>>>(tq, tk, tv, t);
+        PAGED_TRY(c, launch_chained(behind, paged_tc_kernel<D, q8>, dim3(capturing ? b->sm_count : std::min(b->sm_count, n)), kPtThreads, kPtSmem<D>, p.stream, tq, tk, tv, t));
     }
     PAGED_TRY(c, cudaGetLastError());
     path_launched(c);
@@ -825,9 +841,20 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
     if (capturing && !b->n_tokens) return path_fail(c, GGR_ERR_INVALID, "a captured launch needs a plan with tokens: it holds the kernels of that plan");
     // a captured launch has to serve whatever plan its replays find: enough CTAs for any, items dealt in turn
     const int most = (2 * b->sm_count + b->Hkv - 1) / b->Hkv;
+    const bool tc = b->n_items[list][kTc] > 0;
+    if constexpr (!F32 && FMT == kKvQ8Head) {
+        if (tc) {
+            const int rc = launch_dense_rows<D>(c, p, b, a, capturing);
+            if (rc) return rc;
+        }
+    }
+    bool behind = false;
     for (int k = 0; k < kTc; ++k) {
         const int n = b->n_items[list][k];
         if (!n) continue;
+        // (not between event pairs, and not in a capture, whose edges are full ones; with both kinds the first one is waited for)
+        a.lets_in = tc && !capturing && !path_timing(c) && (k == kRows || !b->n_items[list][kRows]);
+        behind = a.lets_in;
         a.plan.counts = b->counts(list, k);
         a.plan.items = b->items(list, k);
         const dim3 grid(b->Hkv, capturing ? most : std::min(n, 65535));
@@ -852,8 +879,8 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
         if (capturing) b->captured |= 1u << k;
     }
     if constexpr (!F32) {
-        if (b->n_items[list][kTc]) {
-            const int rc = launch_tc<D, FMT>(c, p, b, list, m, a, rows, capturing);
+        if (tc) {
+            const int rc = launch_tc<D, FMT>(c, p, b, list, m, a, rows, capturing, behind);
             if (rc) return rc;
             if (capturing) b->captured |= 1u << kTc;
         }

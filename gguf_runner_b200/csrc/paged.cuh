@@ -33,7 +33,7 @@ struct PageView {
 // One piece of attention work: packed rows [row0, row0 + rows) of a sequence against keys [key0, key1). Row r of a sequence
 // and KV head stands for its new token r / G and query head r % G of the group, so that a key tile serves all heads that
 // share it, whatever the number of tokens.
-struct PagedItem {
+struct alignas(16) PagedItem {
     int tok0;   // row of the sequence's first new token in q and out
     int pos0;   // its position
     int n_tok;  // new tokens of the sequence

@@ -49,6 +49,11 @@ struct PagedAttnArgs {
     float* part;             // states of key splits: per (tile, KV head) [rows][D], then [rows] (m, l)
     unsigned* tickets;       // zero between launches
     int* err;
+    // A step that has sequences for the tcgen05 kernel as well: that one is launched programmatically behind this one and reads
+    // nothing that it writes, so that its CTAs take the SMs as this one's leave them. Whatever came before this launch has
+    // completed by then (it is itself an ordinary launch); the tcgen05 kernel waits for this one before it ends, which keeps the
+    // order for all that follows.
+    int lets_in;
 };
 
 __device__ __forceinline__ int paged_first_key(int pos, int window) { return window > 0 ? max(0, pos + 1 - window) : 0; }
@@ -154,17 +159,22 @@ struct PagedMma {
             at[i] = (w.tok0 + tok) * a.q_stride + (int64_t)(kvh * a.G + r - tok * a.G) * D;
         }
         float by[2] = {1.0f, 1.0f};
+        float2 held[Q8 ? KS : 1][2][2];
         if constexpr (Q8) {
             float top[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < (PACK ? 1 : 2); ++i)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        held[ks][i][half] = ok[i] ? load2(a.q, at[i] + ks * 16 + tq * 4 + half * 2) : make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < (PACK ? 1 : 2); ++i) {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float2 x = ok[i] ? load2(a.q, at[i] + ks * 16 + tq * 4 + half * 2) : make_float2(0.f, 0.f);
-                        top[i] = fmaxf(top[i], fmaxf(fabsf(x.x), fabsf(x.y)));
-                    }
+                    for (int half = 0; half < 2; ++half) top[i] = fmaxf(top[i], fmaxf(fabsf(held[ks][i][half].x), fabsf(held[ks][i][half].y)));
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
                 by[i] = __uint_as_float(0x7f000000u - (min(max(__float_as_uint(top[i]), 0x00800000u), 0x7e800000u) & 0x7f800000u));
@@ -187,7 +197,11 @@ struct PagedMma {
                     if constexpr (!F32 && !Q8) {
                         f[0][i + 2 * half] = ok[i] ? *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + at[i] + d) : 0u;
                     } else {
-                        const float2 x = ok[i] ? load2(a.q, at[i] + d) : make_float2(0.f, 0.f);
+                        float2 x;
+                        if constexpr (Q8)
+                            x = held[ks][i][half];
+                        else
+                            x = ok[i] ? load2(a.q, at[i] + d) : make_float2(0.f, 0.f);
                         put(x.x * by[i], x.y * by[i], f, i, half);
                     }
                 }
@@ -592,7 +606,7 @@ struct PagedSplitKShape {
     // warp's chain (load, expand codes, multiply, softmax, multiply), so that more warps count for more than deeper rings or
     // fragments in registers. (16 conversations of 1310 to 20000 keys, 32/4 heads of 128, int8, f32 rows: WARPS_NOTE.)
     static constexpr bool BUSY = F32 || FMT == kKvQ8Head;
-    using M = PagedMma<D, FMT, F32, F32, D == 256 || (D == 128 && BUSY)>;
+    using M = PagedMma<D, FMT, F32, F32, D == 256 || (D == 128 && F32 && FMT == KV_BF16)>;
     static constexpr int R = M::ROWS;
     static constexpr int W = paged_splitk_warps(D, FMT, F32);
     static constexpr int NST = FMT == kKvQ8Head ? (D == 64 ? 6 : (D == 128 ? 4 : 2)) : (D == 64 ? 4 : (BUSY || D == 256 ? 2 : 3));
@@ -625,6 +639,12 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t ring = base + warp * NST * M::TILE;
     float* acc = reinterpret_cast<float*>(base_p);  // [W][R][LD] after the rings have drained
     volatile int* abortp = &s_abort;
+    if (a.lets_in) grid_allow_dependents();
+    // The first item and the number of items are requested together (the list is longer than any grid), and travel while the
+    // barriers are set up: what a token step of one conversation takes is a chain of such round trips.
+    int item = blockIdx.y;
+    PagedItem w = a.plan.items[item];
+    const int n_items = a.plan.counts[0];
     if (tid == 0) s_abort = 0;
     if (lane == 0) {
         for (int s = 0; s < NST; ++s) mbar_init(smem_u32(&s_full[warp][s]), 1);
@@ -632,10 +652,9 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     __syncthreads();
 
-    const int n_items = a.plan.counts[0];
     uint32_t used = 0;  // tiles this warp has been through: ring position and phase
-    for (int item = blockIdx.y; item < n_items; item += gridDim.y) {
-        const PagedItem w = a.plan.items[item];
+    for (; item < n_items; item += gridDim.y) {
+        if (item != (int)blockIdx.y) w = a.plan.items[item];
         const int n_tiles = (w.key1 - w.key0 + 15) >> 4, mine = n_tiles > warp ? (n_tiles - warp + W - 1) / W : 0;
         // keys that some row, and that every row, of the tile sees
         const int tok_lo = w.row0 / a.G, tok_hi = (w.row0 + w.rows - 1) / a.G;
@@ -848,6 +867,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     volatile int* abortp = &s_abort;
+    if (a.lets_in) grid_allow_dependents();
     if (tid == 0) {
         s_abort = 0;
         for (int s = 0; s < NST; ++s) {

@@ -30,6 +30,7 @@ struct PagedTcArgs {
     const void* q_rows;      // head_dim 256: the 16-bit rows of q that are multiplied (of 8-bit pages the f16 ones)
     int64_t q_rows_stride;
     float out_scale;   // of the merged rows: 1 / kReadVScale for f16 rows
+    int behind;        // launched programmatically behind the warp-level kernel of the same call (PagedAttnArgs::lets_in)
     int* sched;        // [0] items handed out beyond the first wave, [1] CTAs that have left
     float* part;       // states of pieces: [256][D], then [256] (m, l)
 };
@@ -534,6 +535,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     fence_after_sync();
     if (warp == 9) tmem_dealloc(tmem, 512);
     if (tid == 0) {
+        if (p.behind) grid_wait();
         if (s_abort && a.err) atomicExch(a.err, 1);
         // the last CTA to leave rewinds the work counter for the next launch
         __threadfence();

@@ -28,7 +28,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     __shared__ int s_abort;
 
     const PagedAttnArgs& a = p.a;
-    if ((int)blockIdx.x >= a.plan.counts[0]) return;  // (a captured launch has CTAs for the longest plan)
+    if ((int)blockIdx.x >= a.plan.counts[0]) return;  // (a captured launch has CTAs for the longest plan, and is not chained)
     const PagedItem w = a.plan.items[blockIdx.x];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -386,7 +386,10 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     __syncthreads();
     fence_after_sync();
     if (warp == 5) tmem_dealloc(tmem, 512);
-    if (tid == 0 && s_abort && a.err) atomicExch(a.err, 1);
+    if (tid == 0) {
+        if (p.behind) grid_wait();
+        if (s_abort && a.err) atomicExch(a.err, 1);
+    }
 }
 
 }  // namespace ggr

@@ -30,6 +30,7 @@ RopeParams path_rope(const ggr_attn_ctx* c, int layer);
 int path_fail(ggr_attn_ctx* c, int status, const std::string& msg);
 void path_create_error(const std::string& msg);
 bool path_capturing(ggr_attn_ctx* c);
+bool path_timing(const ggr_attn_ctx* c);
 void path_launched(ggr_attn_ctx* c);
 // event pair around one launch when kernel timing is on: kind as in ggr_attn_kernel_time
 cudaEvent_t path_timer_start(ggr_attn_ctx* c, int kind);
