@@ -15,6 +15,7 @@ from .binding import (  # noqa: F401
     Pages,
     RopePositionPlan,
     Weights,
+    batch_check,
     gemma_layer_windows,
     lib,
     library_path,

@@ -84,7 +84,7 @@ EXPORTED_SYMBOLS = [
     "ggr_rope_plan_new", "ggr_rope_plan_free", "ggr_rope_plan_append_text", "ggr_rope_plan_append_grid",
     "ggr_rope_plan_len", "ggr_rope_plan_next_text", "ggr_rope_plan_at", "ggr_rope_plan_export",
     "ggr_pages_create", "ggr_pages_destroy", "ggr_pages_device_ptrs", "ggr_batch_create", "ggr_batch_destroy", "ggr_batch_set",
-    "ggr_paged_append", "ggr_paged_read", "ggr_paged_attention", "ggr_packed_attention",
+    "ggr_batch_check", "ggr_paged_append", "ggr_paged_read", "ggr_paged_attention", "ggr_packed_attention",
     "ggr_rope_axis", "ggr_media_plan_validate", "ggr_media_chunk_end", "ggr_gemma_layer_windows",
 ]
 
@@ -169,6 +169,7 @@ def lib() -> C.CDLL:
     L.ggr_batch_destroy.argtypes = [vp]
     L.ggr_batch_destroy.restype = None
     L.ggr_batch_set.argtypes = [vp, i32, vp, vp, vp, i32]
+    L.ggr_batch_check.argtypes = [i32, i32, i32, vp, vp, vp, i32, i32, i32]
     L.ggr_paged_append.argtypes = [vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp]
     L.ggr_paged_read.argtypes = [vp, vp, i32, i32, vp, i64, vp, i64]
     L.ggr_paged_attention.argtypes = [vp, vp, i32, vp, i64, vp, i64]
@@ -973,6 +974,16 @@ class MediaAttentionPlan:
 def rope_axis(layout: int, frequency: int, sections: Sequence[int]) -> int:
     sec = (C.c_int32 * 4)(*[int(s) for s in sections])
     return int(lib().ggr_rope_axis(layout, frequency, sec))
+
+
+def batch_check(q_len, kv_len=None, page_table=None, page_size: int = 0, n_pages: int = 0, max_tokens: int = 1 << 30,
+                max_pages: int = 1 << 30) -> int:
+    """The status that Batch.set would raise for these lengths and this 2-D page table, 0 if none. Needs no device."""
+    q = np.ascontiguousarray(q_len, dtype=np.int32).reshape(-1)
+    kv = q if kv_len is None else np.ascontiguousarray(kv_len, dtype=np.int32).reshape(-1)
+    table = np.empty((q.size, 0), np.int32) if page_table is None else np.ascontiguousarray(page_table, dtype=np.int32)
+    return int(lib().ggr_batch_check(page_size, n_pages, q.size, q.ctypes.data, kv.ctypes.data, table.ctypes.data if table.size else None,
+                                     table.shape[1], max_tokens, max_pages))
 
 
 def gemma_layer_windows(n_layers: int, window: int, period: int = 6):

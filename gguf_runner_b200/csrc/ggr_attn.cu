@@ -3022,6 +3022,11 @@ PathView path_view(const ggr_attn_ctx* c) {
     return v;
 }
 RopeParams path_rope(const ggr_attn_ctx* c, int layer) { return rope_params(c, layer); }
+bool path_rope_window_kind(const ggr_attn_ctx* c, int layer) { return c->cfg.swa_theta_on_window_layers && is_swa_layer(c, layer); }
+float path_rope_theta(const ggr_attn_ctx* c, bool window_kind) {
+    if (!window_kind) return c->cfg.rope_theta;
+    return c->cfg.rope_theta_swa > 0.0f ? c->cfg.rope_theta_swa : 10000.0f;
+}
 int path_fail(ggr_attn_ctx* c, int status, const std::string& msg) { return fail(c, status, msg); }
 void path_create_error(const std::string& msg) { g_create_err = msg; }
 bool path_capturing(ggr_attn_ctx* c) { return capturing(c); }

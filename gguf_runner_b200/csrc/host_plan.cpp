@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../include/ggr_attn.h"
+#include "batch_check.h"
 
 struct ggr_rope_plan {
     std::vector<std::array<int64_t, 3>> positions;
@@ -132,7 +133,58 @@ int ggr_gemma_layer_windows(int32_t n_layers, int32_t window, int32_t period, in
     return GGR_OK;
 }
 
+int ggr_batch_check(int32_t page_size, int32_t n_pages, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
+                    int32_t table_stride, int32_t max_tokens, int32_t max_pages) {
+    ggr::BatchTotals totals;
+    const char* why;
+    try {
+        return ggr::batch_check(page_size, n_pages, n_seqs, q_len, kv_len, page_table, table_stride, max_tokens, max_pages, &totals, &why);
+    } catch (...) {
+        return GGR_ERR_ALLOC;
+    }
+}
+
 }  // extern "C"
+
+int ggr::batch_check(int32_t page_size, int32_t n_pages, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
+                     int32_t table_stride, int32_t max_tokens, int32_t max_pages, BatchTotals* totals, const char** why) {
+    auto bad = [&](int status, const char* msg) {
+        *why = msg;
+        return status;
+    };
+    *why = "";
+    *totals = {0, 0, 0};
+    if (n_seqs < 0 || page_size < 0) return bad(GGR_ERR_INVALID, "negative batch size");
+    if (n_seqs && (!q_len || !kv_len)) return bad(GGR_ERR_INVALID, "null argument");
+    for (int32_t i = 0; i < n_seqs; ++i) {
+        if (q_len[i] < 0 || kv_len[i] < q_len[i])
+            return bad(GGR_ERR_INVALID, "kv_len counts the new tokens: it must be at least q_len, and q_len not negative");
+        if (!page_size && kv_len[i] != q_len[i]) return bad(GGR_ERR_INVALID, "packed prompts have no cached keys: kv_len must equal q_len");
+        totals->tokens += q_len[i];
+        totals->rows += kv_len[i];
+        if (page_size) {
+            const int64_t n = ((int64_t)kv_len[i] + page_size - 1) / page_size;
+            if (n > table_stride) return bad(GGR_ERR_RANGE, "a sequence has more pages than a row of the page table");
+            totals->entries += n;
+        }
+    }
+    if (totals->tokens > max_tokens) return bad(GGR_ERR_RANGE, "more new tokens than the batch plan holds");
+    if (totals->entries > max_pages) return bad(GGR_ERR_RANGE, "more pages than the batch plan holds");
+    if (totals->rows >= ((int64_t)1 << 31)) return bad(GGR_ERR_RANGE, "more rows than a 32-bit index names");
+    if (totals->entries && !page_table) return bad(GGR_ERR_INVALID, "null page table");
+    // a page takes new rows of one sequence only: two would write the same place
+    std::vector<int32_t> written;
+    for (int32_t i = 0; page_size && i < n_seqs; ++i) {
+        const int32_t* row = page_table + (int64_t)i * table_stride;
+        for (int64_t j = 0; j * page_size < kv_len[i]; ++j) {
+            if (row[j] < 0 || row[j] >= n_pages) return bad(GGR_ERR_RANGE, "page table entry outside the pool");
+            if ((j + 1) * page_size > kv_len[i] - q_len[i] && q_len[i] > 0) written.push_back(row[j]);
+        }
+    }
+    std::sort(written.begin(), written.end());
+    if (std::adjacent_find(written.begin(), written.end()) != written.end()) return bad(GGR_ERR_INVALID, "a page would receive new rows twice");
+    return GGR_OK;
+}
 
 // ---- TurboQuant transform signs (src/engine/runtime/inference.rs:370-395, splitmix64 :673-679) ----
 

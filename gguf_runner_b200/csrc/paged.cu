@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/ggr_attn.h"
+#include "batch_check.h"
 #include "paged.cuh"
 #include "paged_mma.cuh"
 #include "paged_tc.cuh"
@@ -114,6 +115,7 @@ struct ggr_batch {
     bool up_used[2] = {false, false};
     int turn = 0;
     size_t at_counts = 0, at_pos = 0, at_slot = 0, at_entries = 0, at_table = 0, at_items[kMaxLists][kKinds] = {}, bytes = 0;
+    double* d_freqs = nullptr;  // RoPE frequencies in 64 bits: of ordinary layers, of window layers
     float* d_part = nullptr;
     unsigned* d_tickets = nullptr;
     __nv_bfloat16* d_planes = nullptr;  // packed f32 rows: [k, v][3 planes][max_tokens][Hkv * D]
@@ -123,8 +125,6 @@ struct ggr_batch {
     int n_items[kMaxLists][kKinds] = {};
     std::vector<PagedItem> scratch;
     int rows_step = 128;
-    std::vector<int> page_owner;  // stamp of the sequence whose new rows a page receives
-    int stamp = 0;
 
     const int* counts(int list, int kind) const { return reinterpret_cast<const int*>(d_plan + at_counts) + (list * kKinds + kind) * 4; }
     const int* dense_counts() const { return reinterpret_cast<const int*>(d_plan + at_counts) + windows.size() * kKinds * 4; }
@@ -253,7 +253,7 @@ int first_key(int pos, int window) { return window > 0 ? std::max(0, pos + 1 - w
 
 }  // namespace
 
-extern "C" int ggr_pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v, float* k_scale, float* v_scale,
+static int pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v, float* k_scale, float* v_scale,
                                 ggr_pages** out) {
     if (!c) return GGR_ERR_INVALID;
     if (!out) return path_fail(c, GGR_ERR_INVALID, "null argument");
@@ -351,6 +351,7 @@ extern "C" void ggr_batch_destroy(ggr_batch* b) {
         if (b->h_plan[i]) cudaFreeHost(b->h_plan[i]);
     }
     cudaFree(b->d_plan);
+    cudaFree(b->d_freqs);
     cudaFree(b->d_part);
     cudaFree(b->d_tickets);
     cudaFree(b->d_planes);
@@ -361,7 +362,7 @@ extern "C" void ggr_batch_destroy(ggr_batch* b) {
     delete b;
 }
 
-extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens, int32_t max_pages, ggr_batch** out) {
+static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens, int32_t max_pages, ggr_batch** out) {
     if (!c) return GGR_ERR_INVALID;
     if (!out) return path_fail(c, GGR_ERR_INVALID, "null argument");
     *out = nullptr;
@@ -451,55 +452,33 @@ extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype
         cudaMemsetAsync(b->d_tickets, 0, b->part_tiles * p.Hkv * sizeof(unsigned), p.stream) != cudaSuccess ||
         (b->tc && cudaMemsetAsync(b->d_sched, 0, 2 * sizeof(int), p.stream) != cudaSuccess))
         return path_fail(c, GGR_ERR_CUDA, "unable to clear the batch plan");
-    if (pages) b->page_owner.assign(pages->v.n_pages, 0);
+    if (pages) {
+        const int half = p.rope_dim / 2;
+        std::vector<double> freqs(2 * half);
+        for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < half; ++i) freqs[k * half + i] = std::pow((double)path_rope_theta(c, k != 0), -(double)(2 * i) / p.rope_dim);
+        if (cudaMalloc((void**)&b->d_freqs, freqs.size() * sizeof(double)) != cudaSuccess) {
+            cudaGetLastError();
+            return path_fail(c, GGR_ERR_ALLOC, "unable to allocate the batch plan");
+        }
+        PAGED_TRY(c, cudaMemcpyAsync(b->d_freqs, freqs.data(), freqs.size() * sizeof(double), cudaMemcpyHostToDevice, p.stream));
+        PAGED_TRY(c, cudaStreamSynchronize(p.stream));
+    }
     *out = b.release();
     return GGR_OK;
 }
 
-extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table, int32_t table_stride) {
+static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table, int32_t table_stride) {
     if (!b) return GGR_ERR_INVALID;
     ggr_attn_ctx* c = b->ctx;
     const PathView p = path_view(c);
-    if (n_seqs < 0 || n_seqs > b->max_seqs) return path_fail(c, GGR_ERR_RANGE, "more sequences than the batch plan holds");
-    if (n_seqs && (!q_len || !kv_len)) return path_fail(c, GGR_ERR_INVALID, "null argument");
+    if (n_seqs > b->max_seqs) return path_fail(c, GGR_ERR_RANGE, "more sequences than the batch plan holds");
     const int ps = b->pages ? b->pages->page_size : 0;
-    int64_t tokens = 0, entries = 0, rows = 0;
-    for (int i = 0; i < n_seqs; ++i) {
-        if (q_len[i] < 0 || kv_len[i] < q_len[i]) return path_fail(c, GGR_ERR_INVALID, "kv_len counts the new tokens: it must be at least q_len, and q_len not negative");
-        if (!b->pages && kv_len[i] != q_len[i]) return path_fail(c, GGR_ERR_INVALID, "packed prompts have no cached keys: kv_len must equal q_len");
-        tokens += q_len[i];
-        rows += kv_len[i];
-        if (b->pages) {
-            const int n = (int)(((int64_t)kv_len[i] + ps - 1) / ps);
-            if (n > table_stride) return path_fail(c, GGR_ERR_RANGE, "a sequence has more pages than a row of the page table");
-            entries += n;
-        }
-    }
-    if (tokens > b->max_tokens) return path_fail(c, GGR_ERR_RANGE, "more new tokens than the batch plan holds");
-    if (entries > b->max_pages) return path_fail(c, GGR_ERR_RANGE, "more pages than the batch plan holds");
-    if (rows >= ((int64_t)1 << 31)) return path_fail(c, GGR_ERR_RANGE, "more rows than a 32-bit index names");
-    if (entries && !page_table) return path_fail(c, GGR_ERR_INVALID, "null page table");
-    if (b->pages) {
-        // a page takes new rows of one sequence only: two would write the same place
-        if (b->stamp > (1 << 30)) {
-            std::fill(b->page_owner.begin(), b->page_owner.end(), 0);
-            b->stamp = 0;
-        }
-        const int stamp0 = b->stamp;
-        b->stamp += n_seqs;
-        for (int i = 0; i < n_seqs; ++i) {
-            const int32_t* row = page_table + (int64_t)i * table_stride;
-            const int n = (kv_len[i] + ps - 1) / ps;
-            for (int j = 0; j < n; ++j) {
-                if (row[j] < 0 || row[j] >= b->pages->v.n_pages) return path_fail(c, GGR_ERR_RANGE, "page table entry outside the pool");
-                if ((int64_t)(j + 1) * ps > kv_len[i] - q_len[i] && q_len[i] > 0) {
-                    int& owner = b->page_owner[row[j]];
-                    if (owner > stamp0) return path_fail(c, GGR_ERR_INVALID, "a page would receive new rows twice");
-                    owner = stamp0 + 1 + i;
-                }
-            }
-        }
-    }
+    BatchTotals totals;
+    const char* why;
+    if (const int rc = batch_check(ps, b->pages ? b->pages->v.n_pages : 0, n_seqs, q_len, kv_len, page_table, table_stride, b->max_tokens, b->max_pages, &totals, &why))
+        return path_fail(c, rc, why);
+    const int64_t tokens = totals.tokens, entries = totals.entries, rows = totals.rows;
     Guard guard(b->device);
     if (path_capturing(c)) return path_fail(c, GGR_ERR_INVALID, "a batch plan cannot be set while its stream is captured");
     const int turn = b->turn;
@@ -708,6 +687,8 @@ extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len,
     PAGED_TRY(c, copy(b->at_table, entries * sizeof(int)));
     for (size_t l = 0; l < b->windows.size(); ++l)
         for (int k = 0; k < kKinds; ++k) PAGED_TRY(c, copy(b->at_items[l][k], b->n_items[l][k] * sizeof(PagedItem)));
+    // (all zero already, unless a launch that ran into a time limit left before its merges)
+    PAGED_TRY(c, cudaMemsetAsync(b->d_tickets, 0, b->part_tiles * b->Hkv * sizeof(unsigned), p.stream));
     PAGED_TRY(c, cudaEventRecord(b->up[turn], p.stream));
     b->up_used[turn] = true;
     b->turn = turn ^ 1;
@@ -915,7 +896,7 @@ PagedAttnArgs attention_args(const PathView& p, const ggr_batch* b, int layer) {
 
 }  // namespace
 
-extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t rotate, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+static int paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t rotate, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                                 const void* v, int64_t v_stride, void* q_out) {
     if (!c) return GGR_ERR_INVALID;
     int rc = check_call(c, b, layer, true);
@@ -943,6 +924,7 @@ extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, in
     AppendArgs a{};
     a.pages = b->pages->v;
     a.rope = path_rope(c, layer);
+    a.freqs = b->d_freqs + (path_rope_window_kind(c, layer) ? p.rope_dim / 2 : 0);
     a.counts = b->counts(0, 0);
     a.tok_pos = reinterpret_cast<const int*>(b->d_plan + b->at_pos);
     a.tok_slot = reinterpret_cast<const int*>(b->d_plan + b->at_slot);
@@ -980,7 +962,7 @@ extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, in
     return GGR_OK;
 }
 
-extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride) {
+static int paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride) {
     if (!c) return GGR_ERR_INVALID;
     int rc = check_call(c, b, layer, true);
     if (rc) return rc;
@@ -1024,7 +1006,7 @@ extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int3
     return GGR_OK;
 }
 
-extern "C" int ggr_paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, void* out, int64_t out_stride) {
+static int paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, void* out, int64_t out_stride) {
     if (!c) return GGR_ERR_INVALID;
     int rc = check_call(c, b, layer, true);
     if (rc) return rc;
@@ -1051,7 +1033,7 @@ extern "C" int ggr_paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer,
     return f32 ? launch_by_dim<kKvQ8Head, true>(c, p, b, list, m, a, rows, capturing) : launch_by_dim<kKvQ8Head, false>(c, p, b, list, m, a, rows, capturing);
 }
 
-extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+static int packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                     int64_t v_stride, void* out, int64_t out_stride) {
     if (!c) return GGR_ERR_INVALID;
     int rc = check_call(c, b, layer, false);
@@ -1103,4 +1085,43 @@ extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer
         !make_map3(&tv128, false, v, b->D, b->Hkv, rows, sy, (uint64_t)v_stride * 2, 64, 1, tc_key_tile(b->D)))
         return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
     return launch_by_dim<KV_BF16, false>(c, p, b, list, m, a, rows, capturing);
+}
+
+// ---- C entries: nothing that the standard library throws leaves them -------------------------------
+
+template <typename F>
+static int guarded(F&& f) {
+    try {
+        return f();
+    } catch (...) {
+        return GGR_ERR_ALLOC;  // (only allocations of the host throw here)
+    }
+}
+
+extern "C" int ggr_pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v, float* k_scale, float* v_scale, ggr_pages** out) {
+    return guarded([&] { return pages_create(c, n_pages, page_size, kv_format, k, v, k_scale, v_scale, out); });
+}
+
+extern "C" int ggr_batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens, int32_t max_pages, ggr_batch** out) {
+    return guarded([&] { return batch_create(c, pages, dtype, max_seqs, max_tokens, max_pages, out); });
+}
+
+extern "C" int ggr_batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table, int32_t table_stride) {
+    return guarded([&] { return batch_set(b, n_seqs, q_len, kv_len, page_table, table_stride); });
+}
+
+extern "C" int ggr_paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t rotate, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out) {
+    return guarded([&] { return paged_append(c, b, layer, rotate, q, q_stride, k, k_stride, v, v_stride, q_out); });
+}
+
+extern "C" int ggr_paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride) {
+    return guarded([&] { return paged_read(c, b, layer, out_dtype, k_out, k_stride, v_out, v_stride); });
+}
+
+extern "C" int ggr_paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, void* out, int64_t out_stride) {
+    return guarded([&] { return paged_attention(c, b, layer, q, q_stride, out, out_stride); });
+}
+
+extern "C" int ggr_packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride) {
+    return guarded([&] { return packed_attention(c, b, layer, q, q_stride, k, k_stride, v, v_stride, out, out_stride); });
 }

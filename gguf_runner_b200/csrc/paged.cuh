@@ -58,6 +58,7 @@ struct PlanView {
 struct AppendArgs {
     PageView pages;
     RopeParams rope;
+    const double* freqs;     // of the layer's kind, in 64 bits
     const int* counts;       // [2] tokens
     const int* tok_pos;      // position of every new token
     const int* tok_slot;     // page * page_size + row in the page
@@ -104,7 +105,7 @@ __device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const float (&x)[E]
     }
 }
 
-// RoPE and append of a few tokens per CTA. A lane has E elements of the lower half of a head and E of the upper, 16 bytes each,
+// RoPE (by cache position, in 64-bit angles) and append of a few tokens per CTA. A lane has E elements of the lower half of a head and E of the upper, 16 bytes each,
 // so that both kinds of RoPE pairs of a fully rotated head lie in one lane, a warp's loads are whole lines, and the head's
 // largest element takes log2(D / 2E) shuffles. Bound by the bytes of the rows; one token per CTA while tokens are few (a token
 // step is latency: the angles of a token, one load, one store), several when there are more CTAs than SMs to hold them. A
@@ -152,8 +153,11 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(AppendArgs a) {
     if (a.rotate) {
         for (int i = threadIdx.x; i < n * half; i += 256) {
             const int t = i / half, f = i - t * half;
-            const float angle = __fmul_rn(__fmul_rn((float)a.tok_pos[t0 + t], a.rope.freqs[f]), a.rope.fscale);
-            sincosf(angle, &sn[i], &cs[i]);
+            // The angle of a far position in 32 bits is off by its position times 2^-24 (2e-4 at 3000, against 6e-8 of the
+            // rotation itself): it is taken in 64 bits and brought into one turn before it becomes an f32.
+            const double angle = (double)a.tok_pos[t0 + t] * a.freqs[f] * (double)a.rope.fscale;
+            const double turns = rint(angle * 0.15915494309189535);
+            sincosf((float)fma(turns, -6.283185307179586, angle), &sn[i], &cs[i]);
         }
         __syncthreads();
     }

@@ -27,6 +27,9 @@ struct PathView {
 
 PathView path_view(const ggr_attn_ctx* c);
 RopeParams path_rope(const ggr_attn_ctx* c, int layer);
+// theta of a layer's frequencies, and of the other kind of layer
+float path_rope_theta(const ggr_attn_ctx* c, bool window_kind);
+bool path_rope_window_kind(const ggr_attn_ctx* c, int layer);
 int path_fail(ggr_attn_ctx* c, int status, const std::string& msg);
 void path_create_error(const std::string& msg);
 bool path_capturing(ggr_attn_ctx* c);

@@ -426,7 +426,7 @@ void ggr_batch_destroy(ggr_batch* batch);
 int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
                   int32_t table_stride);
 /*
- * Stores the new tokens' rows of k and v in their pages. rotate: RoPE by cache position on q and k first (and the layer's
+ * Stores the new tokens' rows of k and v in their pages. rotate: RoPE by cache position (angles in 64 bits) on q and k first (and the layer's
  * bias / QK-norm fixups, dense rows only, before that), rotated (and, in GGR_SCALE_Q_PRESCALED mode, scaled) q to q_out
  * [tokens][q_dim], which may be q itself when heads are rotated as a whole. rotate 0: k is stored as it is, q and q_out are
  * null.
@@ -498,6 +498,9 @@ int ggr_media_plan_validate(const int64_t* start_len, int32_t n, int64_t prompt_
 /* MediaAttentionPlan::chunk_end (src/engine/runtime/attention.rs:43-70): end position or a negative status */
 int64_t ggr_media_chunk_end(const int64_t* start_len, int32_t n, int64_t prompt_tokens, int64_t start,
                             int64_t limit, int64_t chunk);
+/* What ggr_batch_set would say to these lengths and this page table (page_size 0: packed prompts), without a device. */
+int ggr_batch_check(int32_t page_size, int32_t n_pages, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len,
+                    const int32_t* page_table, int32_t table_stride, int32_t max_tokens, int32_t max_pages);
 /* Gemma3 window list from (window, period) (src/vendors/gemma.rs:92-100) */
 int ggr_gemma_layer_windows(int32_t n_layers, int32_t window, int32_t period, int32_t* out);
 

@@ -196,6 +196,8 @@ extern "C" {
     pub fn ggr_batch_destroy(batch: *mut GgrBatch);
     pub fn ggr_batch_set(batch: *mut GgrBatch, n_seqs: i32, q_len: *const i32, kv_len: *const i32,
         page_table: *const i32, table_stride: i32) -> i32;
+    pub fn ggr_batch_check(page_size: i32, n_pages: i32, n_seqs: i32, q_len: *const i32, kv_len: *const i32,
+        page_table: *const i32, table_stride: i32, max_tokens: i32, max_pages: i32) -> i32;
     pub fn ggr_paged_append(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, rotate: i32, q: *const c_void,
         q_stride: i64, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, q_out: *mut c_void) -> i32;
     pub fn ggr_paged_read(ctx: *mut GgrAttnCtx, batch: *mut GgrBatch, layer: i32, out_dtype: i32, k_out: *mut c_void,

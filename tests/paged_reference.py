@@ -5,9 +5,9 @@ import torch
 
 
 def rope(x, pos, d, adjacent, theta):
-    """x [tokens][heads][d] rotated as a whole, in 64 bits; frequencies and angles rounded to 32 bits as the contexts keep them."""
-    freq = (1.0 / torch.tensor([theta], dtype=torch.float64) ** (torch.arange(0, d, 2, dtype=torch.float64) / d)).float().to(x.device)
-    angle = (pos.float().view(-1, 1) * freq).double().view(-1, 1, d // 2)
+    """x [tokens][heads][d] rotated as a whole, in 64 bits."""
+    freq = theta ** -(torch.arange(0, d, 2, dtype=torch.float64, device=x.device) / d)
+    angle = (pos.double().view(-1, 1) * freq).view(-1, 1, d // 2)
     c, s, z, out = angle.cos(), angle.sin(), x.double(), torch.empty_like(x, dtype=torch.float64)
     if adjacent:
         a, b = z[..., 0::2], z[..., 1::2]

@@ -126,11 +126,12 @@ def test_long_contexts(dtype, kv, d):
 
 @pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f32", "bf16"), ("bf16", "q8_head")])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_what_is_not_seen_does_not_count(bad, dtype, kv):
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_what_is_not_seen_does_not_count(d, bad, dtype, kv):
     """A later token of the chunk with values that are not finite leaves the rows before it as they are."""
     q_len, kv_len = [40, 200], [40, 260]
-    clean = Case(8, 4, 128, kv, dtype, 16, q_len, kv_len, seed=5)
-    c = Case(8, 4, 128, kv, dtype, 16, q_len, kv_len, seed=5)
+    clean = Case(8, 4, d, kv, dtype, 16, q_len, kv_len, seed=5)
+    c = Case(8, 4, d, kv, dtype, 16, q_len, kv_len, seed=5)
     at = [21, 199]  # of sequence 0 and 1
     for b, p in enumerate(at):
         page, row = c.table[b][p // 16], p % 16
@@ -145,7 +146,7 @@ def test_what_is_not_seen_does_not_count(bad, dtype, kv):
     hit = torch.where(rows < q_len[0], pos >= at[0], pos >= at[1])
     heads = torch.arange(8, device="cuda") // 2 == 1
     spoilt = hit.view(-1, 1, 1) & heads.view(1, 8, 1)
-    view_a, view_b = a.view(-1, 8, 128), b.view(-1, 8, 128)
+    view_a, view_b = a.view(-1, 8, d), b.view(-1, 8, d)
     untouched = ~spoilt.expand_as(view_a)
     # (rows that were computed again differ in their order of sums: their own error bound)
     c.rows = clean.rows
@@ -160,11 +161,11 @@ def test_what_is_not_seen_does_not_count(bad, dtype, kv):
 @pytest.mark.parametrize("d,adjacent,rope_dim", [(128, False, 0), (128, True, 0), (64, False, 0), (256, False, 0), (128, False, 64)])
 def test_append_rotates_and_stores(d, adjacent, rope_dim, kv, dtype):
     hq, hkv, page = 6, 2, 16
-    q_len, kv_len = [1, 0, 19, 3], [40, 16, 19, 900]
+    q_len, kv_len = [1, 0, 19, 3], [40, 16, 19, 6000]
     ctx = context(hq, hkv, d, layers=2, rope_style=ROPE_ADJACENT if adjacent else ROPE_NEOX, rope_dim=rope_dim)
     table, n_pages = tables(kv_len, page)
     pages = g.Pages(ctx, n_pages, page, kv)
-    batch = g.Batch(ctx, pages, dtype, 4, 32, 200)
+    batch = g.Batch(ctx, pages, dtype, 4, 32, 400)
     batch.set(q_len, kv_len, table)
     gen = torch.Generator(device="cuda").manual_seed(6)
     n, (qd, kd) = sum(q_len), (hq * d, hkv * d)
@@ -181,10 +182,9 @@ def test_append_rotates_and_stores(d, adjacent, rope_dim, kv, dtype):
         x = x.reshape(n, heads, d)
         return torch.cat([ref.rope(x[..., :rd], pos, rd, adjacent, 1e6), x[..., rd:].double()], -1)
 
-    # Rotation in f32 of pairs of length at most 8: sincos, products and sums are off by 2^-20 of that in all. An angle is
-    # pos * theta^-e with e rounded to f32 (times ln theta < 14: 14 * 2^-25), the power, its inverse and two products rounded
-    # (2^-23 + 3 * 2^-24): off by less than pos * 2^-21, and the pair turns by that much.
-    slack = 8 * (2.0 ** -20 + pos.double().view(-1, 1) * 2.0 ** -21)
+    # Rotation of pairs of length at most 8 in f32, by angles brought into one turn in 64 bits: the angle, its sine and cosine, two
+    # products and a sum are off by 2^-22 of that length at most each, 2^-20 in all.
+    slack = torch.full((n, 1), 8 * 2.0 ** -20, dtype=torch.float64, device="cuda")
     want_q, half = turned(q, hq).view(n, qd), 2.0 ** (-8 if dtype == "bf16" else -24)
     assert bool(((out[:n].double() - want_q).abs() <= half * want_q.abs() + slack).all())
     got_k, got_v = ctx.paged_read(batch, 1, "f32")
@@ -350,6 +350,161 @@ def test_captured_steps_follow_the_plan():
         with pytest.raises(GgrError):
             with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
                 batch.set([1, 1, 1], lens[0], big.table)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8_head"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_cut_chunks(d, kv):
+    """Few rows and many keys: items are cut along the keys and merged; one row of a piece is not finite."""
+    c = Case(8, 2, d, kv, "bf16", 64, [70, 1, 33], [7000, 50, 3001], seed=16)
+    c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+    first = c.ctx.paged_attention(c.batch, 0, c.q).clone()
+    for _ in range(3):
+        assert torch.equal(c.ctx.paged_attention(c.batch, 0, c.q), first)
+
+
+def test_8_bit_rows_beyond_f16():
+    """Values that the f16 operands of a chunk cannot hold: those rows are computed again in f32."""
+    c = Case(8, 2, 128, "q8_head", "bf16", 16, [40], [90], seed=17)
+    for i, by in enumerate((3e4, 5e3)):
+        page, row = c.table[0][60 // 16], 60 % 16
+        c.scales[i][0, page, 1, row] *= by
+        c.rows[0][i][60, 1] *= float(torch.tensor(by, dtype=torch.float32))
+    got = c.ctx.paged_attention(c.batch, 0, c.q)
+    out, size, reach = c.want()
+    # (scores of up to 1e5: only the largest weight counts, and an f32 score is off by 2^-20 of its reach)
+    allowed = ref.bound(c.dtype, out, size, reach)
+    assert bool(((got.double() - out).abs() <= allowed).all())
+
+
+def test_many_sequences():
+    lens = [1 + (i * 37) % 60 for i in range(300)]
+    q_len = [min(n, 1 + i % 3) for i, n in enumerate(lens)]
+    for kv, dtype in (("bf16", "bf16"), ("q8_head", "f32")):
+        c = Case(4, 2, 64, kv, dtype, 16, q_len, lens, seed=18)
+        c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+
+
+def test_plans_and_streams_do_not_meet():
+    """Two plans of one context in turn, one of them on a side stream: nothing is shared but the pool."""
+    c = Case(32, 8, 128, "bf16", "bf16", 16, [1, 40], [3000, 700], seed=19)
+    want = c.ctx.paged_attention(c.batch, 0, c.q).clone()
+    other = g.Batch(c.ctx, c.pages, "bf16", 2, 41, 300)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        other.set([1, 1], [900, 600], c.table)
+    small = c.q[:2].contiguous()
+    torch.cuda.synchronize()
+    ref_small = None
+    for _ in range(3):
+        a = c.ctx.paged_attention(c.batch, 0, c.q)
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            b = c.ctx.paged_attention(other, 0, small)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want)
+        ref_small = b.clone() if ref_small is None else ref_small
+        assert torch.equal(b, ref_small)
+
+
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("bf16", "q8_head"), ("f32", "q8_head")])
+def test_captured_plans_keep_to_their_kernels(dtype, kv):
+    """A plan with captured token steps still serves chunks (with the kernels of the steps); captured chunks are replayed with
+    single tokens, other lengths and cuts."""
+    for start, later in (([1, 1], [40, 150]), ([40, 150], [1, 2])):
+        c = Case(8, 2, 128, kv, dtype, 16, [40, 150], [2000, 700], seed=20)
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        out = torch.empty_like(c.q)
+        with torch.cuda.stream(side):
+            c.batch.set(start, c.kv_len, c.table)
+            c.ctx.paged_attention(c.batch, 0, c.q, out=out)
+            side.synchronize()
+            with torch.cuda.graph(graph, stream=side):
+                c.ctx.paged_attention(c.batch, 0, c.q, out=out)
+            for q_len in (later, start):
+                c.batch.set(q_len, c.kv_len, c.table)
+                n = sum(q_len)
+                all_q, c.q_len = c.q, q_len
+                graph.replay()
+                side.synchronize()
+                c.q = all_q[:n]
+                c.check(out[:n])
+                c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+                side.synchronize()
+                c.q = all_q
+        with pytest.raises(GgrError), torch.cuda.stream(side):  # nothing to capture
+            c.batch.set([0, 0], c.kv_len, c.table)
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                c.ctx.paged_attention(c.batch, 0, c.q, out=out)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_captured_packed_prompts(dtype):
+    t, ctx = TYPES[dtype], context(8, 2, 128)
+    batch = g.Batch(ctx, None, dtype, 4, 300)
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    q, k, v = (torch.randn(300, h * 128, generator=gen, device="cuda").to(t) for h in (8, 2, 2))
+    out = torch.empty_like(q)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        batch.set([100, 60])
+        ctx.packed_attention(batch, 0, q, k, v, out=out)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            ctx.packed_attention(batch, 0, q, k, v, out=out)
+        with pytest.raises(ValueError):  # a replay may find more rows than this
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                ctx.packed_attention(batch, 0, q[:160], k, v, out=out)
+        for lens in ([7, 250, 1, 42], [3], [150, 150]):
+            batch.set(lens)
+            out.fill_(7.0)
+            graph.replay()
+            side.synchronize()
+            n = sum(lens)
+            assert bool((out[n:] == 7.0).all())
+            fresh = g.Batch(ctx, None, dtype, 4, 300)
+            fresh.set(lens)
+            want = ctx.packed_attention(fresh, 0, q, k, v)[:n]
+            side.synchronize()
+            assert float((out[:n].float() - want.float()).abs().max()) <= (2.0 ** -7 * 4 if dtype == "bf16" else 1e-5)
+
+
+def test_window_layers_rotate_by_their_own_theta():
+    ctx = g.AttnContext(AttnConfig(n_layers=2, n_heads=4, n_kv_heads=2, head_dim=128, seq_len=8, kv_format=KV_BF16, rope_theta=1e6,
+                                   rope_theta_swa=1e4, swa_theta_on_window_layers=1, layer_windows=(64, 0)))
+    pages = g.Pages(ctx, 8, 16)
+    batch = g.Batch(ctx, pages, "f32", 1, 10, 8)
+    batch.set([10], [100], [list(range(7))])
+    q, k, v = (torch.randn(10, h * 128, device="cuda") for h in (4, 2, 2))
+    pos = torch.arange(90, 100, device="cuda")
+    for layer, theta in ((0, 1e4), (1, 1e6)):
+        got = ctx.paged_append(batch, layer, k, v, q=q)
+        want = ref.rope(q.view(10, 4, 128), pos, 128, False, theta).view(10, 512)
+        assert float((got.double() - want).abs().max()) < 8 * 2.0 ** -20
+        same = q.clone()
+        assert ctx.paged_append(batch, layer, k, v, q=same, q_out=same) is same and torch.equal(same, got)
+
+
+def test_pools_beyond_32_bit_offsets():
+    """Pages whose rows lie more than 2^32 elements into the pool."""
+    n_pages, page, hkv, d = 20000, 256, 8, 128
+    pool = [torch.empty(1, n_pages, hkv, page, d, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ctx = context(8, hkv, d)
+    pages = g.Pages(ctx, n_pages, page, "bf16", *pool)
+    batch = g.Batch(ctx, pages, "bf16", 2, 400, 10)
+    q_len, kv_len = [300, 1], [300, 1]
+    table = [[19999, 0], [19000]]
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    q, k, v = (torch.randn(301, h * d, generator=gen, device="cuda").bfloat16() for h in (8, hkv, hkv))
+    batch.set(q_len, kv_len, table)
+    ctx.paged_append(batch, 0, k, v)
+    assert torch.equal(pool[0][0, 19999, :, :256].transpose(0, 1).reshape(256, -1), k[:256])
+    got_k, got_v = ctx.paged_read(batch, 0, "bf16")
+    assert torch.equal(got_k, k) and torch.equal(got_v, v)
+    got = ctx.paged_attention(batch, 0, q)
+    out, size, reach = (x.view(300, -1) for x in ref.attention(q[:300].view(300, 8, d), k[:300].view(300, hkv, d), v[:300].view(300, hkv, d), 0, 0, d ** -0.5))
+    assert bool(((got[:300].double() - out).abs() <= ref.bound(torch.bfloat16, out, size, reach)).all())
+    assert torch.equal(got[300], v[300].view(hkv, d).reshape(-1))
 
 
 def test_results_repeat_bit_for_bit():
