@@ -612,8 +612,9 @@ struct PagedSplitKShape {
     static constexpr int NST = FMT == kKvQ8Head ? (D == 64 ? 6 : (D == 128 ? 4 : 2)) : (D == 64 ? 4 : (BUSY || D == 256 ? 2 : 3));
     static constexpr int LD = D + 8;
     static constexpr uint32_t RING = W * NST * M::TILE;
+    static constexpr uint32_t SCALES = FMT == kKvQ8Head ? W * NST * 128 : 0;
     static constexpr uint32_t MERGE = W * R * LD * 4;
-    static constexpr uint32_t DATA = RING > MERGE ? RING : MERGE;  // the merge reuses the rings
+    static constexpr uint32_t DATA = RING + SCALES > MERGE ? RING + SCALES : MERGE;  // the merge reuses the rings
     static constexpr uint32_t SMEM = DATA + M::QBYTES + 1024;
 };
 
@@ -637,6 +638,8 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     const uint32_t ring = base + warp * NST * M::TILE;
+    const uint32_t scales = base + S::RING + warp * NST * 128;
+    const float* scales_p = reinterpret_cast<const float*>(base_p + S::RING + warp * NST * 128);
     float* acc = reinterpret_cast<float*>(base_p);  // [W][R][LD] after the rings have drained
     volatile int* abortp = &s_abort;
     if (a.lets_in) grid_allow_dependents();
@@ -660,26 +663,32 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int tok_lo = w.row0 / a.G, tok_hi = (w.row0 + w.rows - 1) / a.G;
         const int any_lo = paged_first_key(w.pos0 + tok_lo, a.window), any_hi = w.pos0 + tok_hi + 1;
         const int all_lo = paged_first_key(w.pos0 + tok_hi, a.window), all_hi = w.pos0 + tok_lo + 1;
-        auto issue = [&](int t) {
+        // Pages of this warp's tiles, 32 at a time: lane i has the one of tile 32 k + i (of the block in use, and of the next)
+        auto pages_from = [&](int t) {
+            const int key = w.key0 + (warp + (t + lane) * W) * 16;
+            return a.paged && t + lane < mine ? a.plan.table[w.src + (key >> a.pages.page_log2)] : 0;
+        };
+        int pages_now = pages_from(0), pages_next = pages_from(32);
+        auto issue = [&](int t) {  // (by the whole warp)
             const uint32_t u = used + t, stage = u % NST;
             const int key = w.key0 + (warp + t * W) * 16;
             const uint32_t bar = smem_u32(&s_full[warp][stage]);
-            const int page = a.paged ? a.plan.table[w.src + (key >> a.pages.page_log2)] : 0;
-            mbar_expect_tx(bar, M::TILE);
-            M::request(a, &tmK, &tmV, w, kvh, key, page, ring + stage * M::TILE, bar);
-        };
-        // Scales come by ordinary loads, one tile ahead: as copies of 64 bytes each they cost the copy engine as much as the codes
-        typename M::Scales sc_now, sc_next;
-        auto fetch_scales = [&](int t) {
-            if constexpr (M::Q8) {
-                const int key = w.key0 + (warp + t * W) * 16;
-                const int64_t row = a.pages.row(a.layer, a.plan.table[w.src + (key >> a.pages.page_log2)], kvh, key & ((1 << a.pages.page_log2) - 1));
-                sc_next.load(a.pages.ks + row, a.pages.vs + row, tq);
+            if (t > 0 && (t & 31) == 0) {
+                pages_now = pages_next;
+                pages_next = pages_from(t + 32);
+            }
+            const int page = __shfl_sync(0xffffffffu, pages_now, t & 31);
+            if (lane == 0) {
+                mbar_expect_tx(bar, M::TILE + (M::Q8 ? 128 : 0));
+                M::request(a, &tmK, &tmV, w, kvh, key, page, ring + stage * M::TILE, bar);
+                if constexpr (M::Q8) {
+                    const int64_t row = a.pages.row(a.layer, page, kvh, key & ((1 << a.pages.page_log2) - 1));
+                    bulk_load(scales + stage * 128, a.pages.ks + row, 64, bar);
+                    bulk_load(scales + stage * 128 + 64, a.pages.vs + row, 64, bar);
+                }
             }
         };
-        if (mine > 0) fetch_scales(0);
-        if (lane == 0)
-            for (int t = 0; t < NST - 1 && t < mine; ++t) issue(t);
+        for (int t = 0; t < NST - 1 && t < mine; ++t) issue(t);
         M x;
         x.start();
         x.load_q(a, w, kvh, w.row0, w.row0 + w.rows, lane, base + S::DATA);
@@ -688,8 +697,6 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int lo0 = paged_first_key(p0, a.window), lo1 = paged_first_key(p1, a.window);
         for (int t = 0; t < mine; ++t) {
             const uint32_t u = used + t, stage = u % NST;
-            sc_now = sc_next;
-            if (t + 1 < mine) fetch_scales(t + 1);
             if (!mbar_wait_warp(smem_u32(&s_full[warp][stage]), (u / NST) & 1u, abortp)) break;
             const int key = w.key0 + (warp + t * W) * 16;
             const uint32_t kt = ring + stage * M::TILE;
@@ -698,10 +705,12 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 M::clear(kt, any_lo - key, any_hi - key, lane);
                 __syncwarp();
             }
-            x.step(kt, sc_now, whole, lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, lane);
+            typename M::Scales sc;
+            if constexpr (M::Q8) sc.load(scales_p + stage * 32, scales_p + stage * 32 + 16, tq);
+            x.step(kt, sc, whole, lo0 - key, p0 + 1 - key, lo1 - key, p1 + 1 - key, lane);
             __syncwarp();
-            if (lane == 0 && t + NST - 1 < mine) {
-                fence_smem_to_async_proxy();
+            if (t + NST - 1 < mine) {
+                if (lane == 0) fence_smem_to_async_proxy();
                 issue(t + NST - 1);
             }
         }
