@@ -728,12 +728,12 @@ struct Maps {
 };
 
 template <int FMT, int D>
-void launch_read(const ReadArgs& a, bool bf16, int grid, cudaStream_t stream) {
-    if (bf16)
-        paged_read_kernel<FMT, D, kReadBf16><<<grid, 256, 0, stream>>>(a);
-    else
-        paged_read_kernel<FMT, D, kReadF32><<<grid, 256, 0, stream>>>(a);
+cudaError_t launch_read(const ReadArgs& a, bool bf16, bool chained, int grid, cudaStream_t stream) {
+    return launch_chained(chained, bf16 ? paged_read_kernel<FMT, D, kReadBf16> : paged_read_kernel<FMT, D, kReadF32>, dim3(grid), 256, 0, stream, a);
 }
+
+// Launches are programmatic (launch_chained) except in a capture, whose edges are full ones, and between event pairs.
+bool chain(const ggr_attn_ctx* c, bool capturing) { return !capturing && !path_timing(c); }
 
 int read_grid(const ggr_batch* b, int64_t entries) {
     const int64_t blocks = entries * (b->pages->page_size / 16) * b->Hkv;
@@ -759,9 +759,9 @@ int launch_dense_rows(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, const Pa
         r.q_dim = b->Hq * D;
         {
             PathTimer t(c, 1);
-            paged_read_kernel<kKvQ8Head, D, kReadHalf><<<read_grid(b, capturing ? b->max_pages : b->n_dense), 256, 0, p.stream>>>(r);
+            PAGED_TRY(c, launch_chained(chain(c, capturing), paged_read_kernel<kKvQ8Head, D, kReadHalf>, dim3(read_grid(b, capturing ? b->max_pages : b->n_dense)), 256, 0,
+                                        p.stream, r));
         }
-        PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
     }
     return GGR_OK;
@@ -791,7 +791,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         t.q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
         t.q_rows_stride = q8 ? b->Hq * D : args.q_stride;
         PathTimer timer(c, 0);
-        PAGED_TRY(c, launch_chained(behind, paged_tc_wide_kernel<q8>, dim3(capturing ? (int)b->item_cap[kTc] : n), kPwThreads, kPwSmem, p.stream, tk, tv, t));
+        PAGED_TRY(c, launch_chained(chain(c, capturing), paged_tc_wide_kernel<q8>, dim3(capturing ? (int)b->item_cap[kTc] : n), kPwThreads, kPwSmem, p.stream, tk, tv, t));
     } else {
         const void* q_rows = q8 ? static_cast<const void*>(b->d_q16) : args.q;
         CUtensorMap tq;
@@ -800,7 +800,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
         static KernelSmemSetup setup;
         PAGED_TRY(c, setup.ensure(paged_tc_kernel<D, q8>, p.device, p.smem_optin, (int)kPtSmem<D>));
         PathTimer timer(c, 0);
-        PAGED_TRY(c, launch_chained(behind, paged_tc_kernel<D, q8>, dim3(capturing ? b->sm_count : std::min(b->sm_count, n)), kPtThreads, kPtSmem<D>, p.stream, tq, tk, tv, t));
+        PAGED_TRY(c, launch_chained(chain(c, capturing), paged_tc_kernel<D, q8>, dim3(capturing ? b->sm_count : std::min(b->sm_count, n)), kPtThreads, kPtSmem<D>, p.stream, tq, tk, tv, t));
     }
     PAGED_TRY(c, cudaGetLastError());
     path_launched(c);
@@ -811,7 +811,7 @@ int launch_tc(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list, const 
     {
         PathTimer timer(c, 2);
         const int grid = std::min(cut * (D == 256 ? 16 : D / 4), 16 * b->sm_count);
-        PAGED_TRY(c, launch_chained(!capturing && !timer.stop, paged_tc_merge_kernel<D>, dim3(grid), 256, 0, p.stream, t));
+        PAGED_TRY(c, launch_chained(chain(c, capturing), paged_tc_merge_kernel<D>, dim3(grid), 256, 0, p.stream, t));
     }
     path_launched(c);
     return GGR_OK;
@@ -833,9 +833,7 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
     for (int k = 0; k < kTc; ++k) {
         const int n = b->n_items[list][k];
         if (!n) continue;
-        // (not between event pairs, and not in a capture, whose edges are full ones; with both kinds the first one is waited for)
-        a.lets_in = tc && !capturing && !path_timing(c) && (k == kRows || !b->n_items[list][kRows]);
-        behind = a.lets_in;
+        behind = chain(c, capturing);
         a.plan.counts = b->counts(list, k);
         a.plan.items = b->items(list, k);
         const dim3 grid(b->Hkv, capturing ? most : std::min(n, 65535));
@@ -846,14 +844,14 @@ int launch_attention(ggr_attn_ctx* c, const PathView& p, ggr_batch* b, int list,
                 static KernelSmemSetup setup;
                 PAGED_TRY(c, setup.ensure(paged_splitk_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
                 PathTimer t(c, 0);
-                paged_splitk_kernel<D, FMT, F32><<<grid, S::W * 32, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
+                PAGED_TRY(c, launch_chained(chain(c, capturing), paged_splitk_kernel<D, FMT, F32>, grid, S::W * 32, S::SMEM, p.stream, *m.k16, *m.v16, a));
             }
         } else {
             using S = PagedRowsShape<D, FMT, F32>;
             static KernelSmemSetup setup;
             PAGED_TRY(c, setup.ensure(paged_rows_kernel<D, FMT, F32>, p.device, p.smem_optin, (int)S::SMEM));
             PathTimer t(c, 0);
-            paged_rows_kernel<D, FMT, F32><<<grid, S::THREADS, S::SMEM, p.stream>>>(*m.k16, *m.v16, a);
+            PAGED_TRY(c, launch_chained(chain(c, capturing), paged_rows_kernel<D, FMT, F32>, grid, S::THREADS, S::SMEM, p.stream, *m.k16, *m.v16, a));
         }
         PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
@@ -952,12 +950,8 @@ static int paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t ro
     const size_t smem = rotate ? (size_t)2 * a.tokens_per_cta * a.rope.rope_half * sizeof(float) : 0;
     {
         PathTimer t(c, 1);
-        if (in_bf16)
-            paged_append_kernel<true><<<grid, 256, smem, p.stream>>>(a);
-        else
-            paged_append_kernel<false><<<grid, 256, smem, p.stream>>>(a);
+        PAGED_TRY(c, launch_chained(chain(c, capturing), in_bf16 ? paged_append_kernel<true> : paged_append_kernel<false>, dim3(grid), 256, smem, p.stream, a));
     }
-    PAGED_TRY(c, cudaGetLastError());
     path_launched(c);
     return GGR_OK;
 }
@@ -987,21 +981,13 @@ static int paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_
     const bool bf16 = out_dtype == GGR_DTYPE_BF16;
     {
         PathTimer t(c, 1);
-        if (b->pages->v.fmt == GGR_KV_BF16) {
-            switch (b->D) {
-                case 64: launch_read<KV_BF16, 64>(a, bf16, grid, p.stream); break;
-                case 128: launch_read<KV_BF16, 128>(a, bf16, grid, p.stream); break;
-                default: launch_read<KV_BF16, 256>(a, bf16, grid, p.stream);
-            }
-        } else {
-            switch (b->D) {
-                case 64: launch_read<kKvQ8Head, 64>(a, bf16, grid, p.stream); break;
-                case 128: launch_read<kKvQ8Head, 128>(a, bf16, grid, p.stream); break;
-                default: launch_read<kKvQ8Head, 256>(a, bf16, grid, p.stream);
-            }
+        const bool chained = chain(c, capturing), q8 = b->pages->v.fmt == GGR_KV_Q8_HEAD;
+        switch (b->D) {
+            case 64: PAGED_TRY(c, (q8 ? launch_read<kKvQ8Head, 64> : launch_read<KV_BF16, 64>)(a, bf16, chained, grid, p.stream)); break;
+            case 128: PAGED_TRY(c, (q8 ? launch_read<kKvQ8Head, 128> : launch_read<KV_BF16, 128>)(a, bf16, chained, grid, p.stream)); break;
+            default: PAGED_TRY(c, (q8 ? launch_read<kKvQ8Head, 256> : launch_read<KV_BF16, 256>)(a, bf16, chained, grid, p.stream));
         }
     }
-    PAGED_TRY(c, cudaGetLastError());
     path_launched(c);
     return GGR_OK;
 }
@@ -1071,10 +1057,9 @@ static int packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const 
             return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the packed rows");
         {
             PathTimer t(c, 1);
-            paged_planes_kernel<<<dim3((unsigned)(((int64_t)rows * kv_dim / 4 + 255) / 256), 2), 256, 0, p.stream>>>(
-                static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, b->counts(0, 0), kv_dim, kp, vp, plane);
+            PAGED_TRY(c, launch_chained(chain(c, capturing), paged_planes_kernel, dim3((unsigned)(((int64_t)rows * kv_dim / 4 + 255) / 256), 2), 256, 0, p.stream,
+                                        static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, b->counts(0, 0), kv_dim, kp, vp, plane));
         }
-        PAGED_TRY(c, cudaGetLastError());
         path_launched(c);
         return launch_by_dim<KV_F32, true>(c, p, b, list, m, a, rows, capturing);
     }

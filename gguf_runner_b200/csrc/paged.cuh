@@ -146,8 +146,6 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(AppendArgs a) {
         lo = load_raw<BF16>(k.src, k.at + k.j * E);
         hi = load_raw<BF16>(k.src, k.at + D / 2 + k.j * E);
     };
-#pragma unroll
-    for (int u = 0; u < UN; ++u) fetch(threadIdx.x + u * 256, x[u], y[u]);
     float* cs = sm;
     float* sn = sm + a.tokens_per_cta * half;
     if (a.rotate) {
@@ -159,8 +157,13 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(AppendArgs a) {
             const double turns = rint(angle * 0.15915494309189535);
             sincosf((float)fma(turns, -6.283185307179586, angle), &sn[i], &cs[i]);
         }
-        __syncthreads();
     }
+    // (so far only the plan was read; the rows may be the work of the launch in front)
+    grid_wait();
+    grid_allow_dependents();
+#pragma unroll
+    for (int u = 0; u < UN; ++u) fetch(threadIdx.x + u * 256, x[u], y[u]);
+    __syncthreads();
     auto finish = [&](const Task& k, const uint4& raw_x, const uint4& raw_y) {
         float x[E], y[E];
         unpack_raw<BF16, E>(raw_x, x);
@@ -309,6 +312,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
     const int sub_log2 = a.pages.page_log2 - 4, Hkv = a.pages.Hkv;
     const int tid = threadIdx.x % used_threads, r0 = tid / per_row, e = (tid % per_row) * E;
     const bool idle = threadIdx.x >= used_threads;
+    grid_wait();
+    grid_allow_dependents();
     const int64_t blocks = ((int64_t)a.counts[1] << sub_log2) * Hkv;
     for (int64_t b0 = (int64_t)blockIdx.x * UN; b0 < blocks; b0 += (int64_t)gridDim.x * UN) {
         int slot[UN], dense[UN], used[UN], head[UN];  // of a block's first row: where it lies in the pool and in the output

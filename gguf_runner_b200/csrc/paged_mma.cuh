@@ -49,11 +49,6 @@ struct PagedAttnArgs {
     float* part;             // states of key splits: per (tile, KV head) [rows][D], then [rows] (m, l)
     unsigned* tickets;       // zero between launches
     int* err;
-    // A step that has sequences for the tcgen05 kernel as well: that one is launched programmatically behind this one and reads
-    // nothing that it writes, so that its CTAs take the SMs as this one's leave them. Whatever came before this launch has
-    // completed by then (it is itself an ordinary launch); the tcgen05 kernel waits for this one before it ends, which keeps the
-    // order for all that follows.
-    int lets_in;
 };
 
 __device__ __forceinline__ int paged_first_key(int pos, int window) { return window > 0 ? max(0, pos + 1 - window) : 0; }
@@ -642,7 +637,6 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const float* scales_p = reinterpret_cast<const float*>(base_p + S::RING + warp * NST * 128);
     float* acc = reinterpret_cast<float*>(base_p);  // [W][R][LD] after the rings have drained
     volatile int* abortp = &s_abort;
-    if (a.lets_in) grid_allow_dependents();
     // The first item and the number of items are requested together (the list is longer than any grid), and travel while the
     // barriers are set up: what a token step of one conversation takes is a chain of such round trips.
     int item = blockIdx.y;
@@ -655,6 +649,13 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     __syncthreads();
 
+    // Launches of the library follow one another programmatically (launch_chained). Up to here, and for the pages of the first
+    // item, only the plan is read, which no kernel writes.
+    bool waited = false;
+    if (item >= n_items) {
+        grid_wait();
+        grid_allow_dependents();
+    }
     uint32_t used = 0;  // tiles this warp has been through: ring position and phase
     for (; item < n_items; item += gridDim.y) {
         if (item != (int)blockIdx.y) w = a.plan.items[item];
@@ -669,6 +670,11 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             return a.paged && t + lane < mine ? a.plan.table[w.src + (key >> a.pages.page_log2)] : 0;
         };
         int pages_now = pages_from(0), pages_next = pages_from(32);
+        if (!waited) {
+            waited = true;
+            grid_wait();
+            grid_allow_dependents();
+        }
         auto issue = [&](int t) {  // (by the whole warp)
             const uint32_t u = used + t, stage = u % NST;
             const int key = w.key0 + (warp + t * W) * 16;
@@ -876,7 +882,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
     volatile int* abortp = &s_abort;
-    if (a.lets_in) grid_allow_dependents();
     if (tid == 0) {
         s_abort = 0;
         for (int s = 0; s < NST; ++s) {
@@ -888,6 +893,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     __syncthreads();
     const int n_items = a.plan.counts[0];
+    grid_wait();
+    grid_allow_dependents();
     uint32_t used = 0;  // stages gone through: ring position and phase
     // keys that some row of an item sees
     auto any_lo_of = [&](const PagedItem& w) { return paged_first_key(w.pos0 + w.row0 / a.G, a.window); };
@@ -1017,6 +1024,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 // f32 rows of k or v as three bf16 planes: x = h + m + l. Rows of `dim` elements, four per thread; `counts` holds the rows in use.
 __global__ void __launch_bounds__(256) paged_planes_kernel(const float* k, const float* v, int64_t k_stride, int64_t v_stride, const int* counts, int dim,
                                                            __nv_bfloat16* kp, __nv_bfloat16* vp, int64_t plane) {
+    grid_wait();
+    grid_allow_dependents();
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= (int64_t)counts[2] * dim) return;
     const int64_t r = i / dim, d = i - r * dim;

@@ -30,7 +30,10 @@ struct PagedTcArgs {
     const void* q_rows;      // head_dim 256: the 16-bit rows of q that are multiplied (of 8-bit pages the f16 ones)
     int64_t q_rows_stride;
     float out_scale;   // of the merged rows: 1 / kReadVScale for f16 rows
-    int behind;        // launched programmatically behind the warp-level kernel of the same call (PagedAttnArgs::lets_in)
+    // Launched programmatically behind the warp-level kernel of the same call, of which it reads nothing: that one lets it in
+    // when it has itself waited for all that came before, so that this kernel's CTAs take the SMs as that one's leave them. It
+    // waits for it before it ends, which keeps the order for all that follows.
+    int behind;
     int* sched;        // [0] items handed out beyond the first wave, [1] CTAs that have left
     float* part;       // states of pieces: [256][D], then [256] (m, l)
 };
@@ -144,6 +147,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t tmem = s_tmem_base;
     volatile int* abortp = &s_abort;
     volatile int* livep = s_live;
+    if (!p.behind) grid_wait();
 
     if (warp >= 8) {
         reg_release<kPtCtrlRegs>();

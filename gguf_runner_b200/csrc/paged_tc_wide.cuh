@@ -81,6 +81,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     fence_after_sync();
     const uint32_t tmem = s_tmem_base;
     volatile int* abortp = &s_abort;
+    if (!p.behind) grid_wait();
 
     if (warp == 4) {
         // ---------------- TMA producer: the whole warp, a lane per copy ----------------

@@ -507,6 +507,41 @@ def test_pools_beyond_32_bit_offsets():
     assert torch.equal(got[300], v[300].view(hkv, d).reshape(-1))
 
 
+@pytest.mark.parametrize("d,kv,dtype", [(128, "bf16", "bf16"), (128, "q8_head", "bf16"), (64, "q8_head", "f32"), (256, "bf16", "bf16")])
+def test_launches_keep_their_order(d, kv, dtype):
+    """Appends over the same pages, attention, reads and foreign kernels behind each other, against the same step by step."""
+    c = Case(8, 2, d, kv, dtype, 16, [1, 60, 2], [900, 300, 33], seed=23)
+    gen = torch.Generator(device="cuda").manual_seed(24)
+    steps = [torch.randn(3, 63, 8 * d, generator=gen, device="cuda").to(c.dtype) for _ in range(6)]
+
+    def play(wait):
+        got = []
+        for x in steps:
+            q = x[0] * 1.0  # a kernel of torch's in front
+            k, v = x[1, :, :2 * d] * 1.0, x[2, :, :2 * d] * 1.0
+            wait()
+            turned = c.ctx.paged_append(c.batch, 0, k, v, q=q)
+            wait()
+            out = c.ctx.paged_attention(c.batch, 0, turned)
+            wait()
+            c.ctx.paged_append(c.batch, 0, v, k)  # over the rows that were just read
+            wait()
+            rows = c.ctx.paged_read(c.batch, 0, dtype)
+            wait()
+            again = c.ctx.paged_attention(c.batch, 0, turned)
+            wait()
+            turned.zero_()
+            c.batch.set(c.q_len, c.kv_len, c.table)
+            got += [out, again, *(r[torch.isfinite(r)] for r in rows)]
+        torch.cuda.synchronize()
+        return got
+
+    want = play(torch.cuda.synchronize)
+    for _ in range(3):
+        for a, b in zip(play(lambda: None), want):
+            assert torch.equal(a, b)
+
+
 def test_results_repeat_bit_for_bit():
     c = Case(32, 4, 128, "bf16", "bf16", 32, [1] * 5 + [60], [5000, 40, 900, 2500, 1, 300], seed=14)
     first = c.ctx.paged_attention(c.batch, 0, c.q).clone()
