@@ -39,9 +39,6 @@ struct ggr_pages {
 
 namespace {
 
-// Packed rows (new tokens times query heads of a KV head) of a sequence above which it goes to the tcgen05 kernel, and above
-// which (32-bit precision, head_dim 256) to the kernel whose warps share the keys.
-constexpr int kTcMinRows = 64, kRowsMinRows = 64;
 // Keys of a tile of the tcgen05 kernels, query tiles of an item
 constexpr int tc_key_tile(int D) { return D == 256 ? kPwBN : 128; }
 constexpr int tc_item_tiles(int D) { return D == 256 ? 1 : 2; }
@@ -197,7 +194,7 @@ int choose_piece(const std::vector<Tile>& tiles, int Hkv, int slots, double tile
 // items. Items are taken longest first by whichever SM is free, so that only the longest and the last ones matter: those
 // above some length or after some whole wave are cut, so far that the SMs end together. A step over a tile takes 2.1 us, an item 3 us besides (its start, its
 // epilogue; at head_dim 256 0.75 per 64-key tile and 6), a piece's rows one more, and the merge 4 and 0.03 per piece. Returns how many pairs stay whole; *piece: the size of the others' pieces.
-int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, bool wide, int* piece) {
+int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t max_pieces, bool wide, int* piece, double* cost_us) {
     const double t = wide ? 0.75 : 2.1, t0 = wide ? 6.0 : 3.0;
     const int n = (int)tiles.size();
     int best_whole = n;
@@ -233,10 +230,17 @@ int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t m
         }
     };
     *piece = 1;
-    if (!n || (int64_t)n * Hkv > 8 * sm_count) return n;
+    *cost_us = 0.0;
+    if (!n) return n;
+    if ((int64_t)n * Hkv > 8 * sm_count) {  // many items: they even out by themselves
+        double sum = 0.0;
+        for (int x : tiles) sum += (t0 + x * t) * Hkv;
+        *cost_us = sum / sm_count + 0.5 * (t0 + tiles[0] * t);
+        return n;
+    }
     consider(n, 1);
     // the longest ones, wherever they stand (ragged lengths)
-    for (double f : {0.85, 0.7, 0.5, 0.34, 0.25, 0.17})
+    for (double f : {0.85, 0.7, 0.5, 0.34, 0.25, 0.17, 0.11, 0.07})
         if (tiles[0] * f >= 2.0) consider(0, (int)std::ceil(tiles[0] * f));
     // and the last wave of equal ones
     const int waves = (int)((int64_t)n * Hkv / sm_count);
@@ -246,10 +250,82 @@ int choose_tc_cut(const std::vector<int>& tiles, int Hkv, int sm_count, size_t m
         for (int k : {2, 3, 4, 6, 8, 12})
             if (tiles[whole] / k >= 2) consider(whole, (tiles[whole] + k - 1) / k);
     }
+    *cost_us = best_cost;
     return best_whole;
 }
 
 int first_key(int pos, int window) { return window > 0 ? std::max(0, pos + 1 - window) : 0; }
+
+// Which sequences leave the split-K kernel: those with more packed rows (new tokens times query heads of a KV head) than the
+// result. It streams the keys once per 16 (f32: 8) rows, the others once per 128 or 256 but with fewer CTAs and a longer start,
+// so the border depends on how many sequences there are and how long they are. Estimated for a few borders, smallest taken.
+// Measured, us of the split-K kernel / the other one, 32/8 heads of 128, bf16, by rows: 1 sequence of 1000 keys, 256 rows: 11 / 18;
+// 1 of 8000, 32: 15 / 30, 128: 32 / 30, 256: 49 / 33; 8 of 2000, 32: 17 / 32, 64: 33 / 32, 128: 64 / 34; 32 of 1000, 16: 30 / 43, 32: 54 /
+// 43, 64: 94 / 43. f32: 1 of 8000, 256: 167 / 609; 8 of 2000, 64: 92 / 124, 128: 160 / 158; 32 of 1000, 16: 69 / 128, 64: 235 / 129.
+// 8/4 heads of 256, bf16: 1 of 8000, 4: 18 / 23, 16: 36 / 24; 8 of 2000, 4: 18 / 16.
+struct BatchShape {
+    int D, G, Hkv, sm_count;
+    bool tc, q8;
+    int split_rows, rows_step, item_tokens, key_tile;  // rows of a tile of the warp-level kernels, tokens of an item and keys of a tile of tcgen05
+    size_t max_pieces;
+    double split_step_us;  // a 16-key tile of the split-K kernel, per SM
+};
+struct Work {
+    int rows, keys;  // of a sequence: packed rows, keys that they walk
+};
+int choose_border(const std::vector<Work>& seqs, const BatchShape& s) {
+    int borders[9], n_borders = 0;
+    // whoever has at most one tile's rows stays, unless head_dim 256 has the tcgen05 kernel; long prompts go
+    const int lo = s.tc && s.D == 256 ? 0 : (s.tc ? 16 : 8), hi = s.tc ? 256 : 4096;
+    bool open = false;
+    for (const Work& w : seqs) open |= w.rows > lo && w.rows <= hi;
+    if (!open) return lo;
+    borders[n_borders++] = lo;
+    for (int b = lo ? 2 * lo : 8; b <= hi && n_borders < 8; b *= s.tc ? 2 : 3) borders[n_borders++] = b;
+    borders[n_borders++] = hi;
+    int best = lo;
+    double best_cost = -1.0;
+    std::vector<int> tiles;
+    for (int k = 0; k < n_borders; ++k) {
+        const int border = borders[k];
+        double steps = 0.0, ctas = 0.0, items = 0.0, sum = 0.0, longest = 0.0, rows = 0.0, most = 0.0;
+        tiles.clear();
+        for (const Work& w : seqs) {
+            if (w.rows == 0) continue;
+            if (w.rows <= border) {
+                const int n = (w.rows + s.split_rows - 1) / s.split_rows;
+                steps += (double)n * ((w.keys + 15) / 16) * s.Hkv;
+                ctas += (double)n * s.Hkv;
+                most = std::max(most, std::min(16.0, (double)w.rows));
+            } else if (s.tc) {
+                const int per = s.item_tokens * s.G;
+                for (int r = 0; r < w.rows; r += per) tiles.push_back((w.keys + s.key_tile - 1) / s.key_tile);
+                rows += w.keys;
+            } else {
+                const int n = (w.rows + s.rows_step - 1) / s.rows_step;
+                const double one = (double)((w.keys + 15) / 16) * (w.rows > s.rows_step / 2 ? 1.2 : 0.95) * s.D / 128;
+                items += (double)n * s.Hkv;
+                sum += n * one * s.Hkv;
+                longest = std::max(longest, one);
+            }
+        }
+        double cost = 0.0;
+        if (ctas > 0.0) cost += 5.0 + (steps * s.split_step_us + std::max(ctas, (double)s.sm_count) * 4.5) / s.sm_count + (s.D == 256 ? 0.8 * most : 0.0);
+        if (items > 0.0) cost += 8.0 + (items <= s.sm_count ? longest : sum / s.sm_count + 0.5 * longest);
+        if (!tiles.empty()) {
+            std::sort(tiles.begin(), tiles.end(), std::greater<int>());
+            int piece;
+            double tc;
+            choose_tc_cut(tiles, s.Hkv, s.sm_count, s.max_pieces, s.D == 256, &piece, &tc);
+            cost += tc + (s.D == 256 ? 0.0 : 4.0) + (s.q8 ? 5.0 + rows * s.Hkv * s.D * 1e-6 : 0.0);
+        }
+        if (best_cost < 0.0 || cost < best_cost) {
+            best_cost = cost;
+            best = border;
+        }
+    }
+    return best;
+}
 
 }  // namespace
 
@@ -516,10 +592,24 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
     std::vector<int> kind(n_seqs, kSplitK), lin(n_seqs, 0);
     auto allowed = [&](int k) { return !b->captured || (b->captured >> k & 1); };
     int64_t dense = 0;
+    int border = 0;
+    if (b->pages || !f32) {
+        const int widest = *std::min_element(b->windows.begin(), b->windows.end()) == 0 ? 0 : *std::max_element(b->windows.begin(), b->windows.end());
+        std::vector<Work> work(n_seqs);
+        for (int i = 0; i < n_seqs; ++i)
+            work[i] = {(int)std::min<int64_t>((int64_t)q_len[i] * b->G, 1 << 30), kv_len[i] - first_key(kv_len[i] - q_len[i], widest)};
+        BatchShape s{};
+        s.D = b->D, s.G = b->G, s.Hkv = b->Hkv, s.sm_count = b->sm_count;
+        s.tc = b->tc, s.q8 = q8;
+        s.split_rows = f32 ? 8 : 16, s.rows_step = b->rows_step;
+        s.item_tokens = b->tc ? tc_item_tiles(b->D) * b->tc_tokens : 0, s.key_tile = tc_key_tile(b->D);
+        s.max_pieces = b->tc_parts;
+        s.split_step_us = (f32 ? 0.19 : (q8 ? 0.13 : 0.1)) * (b->D == 256 ? (f32 ? 2.0 : 4.0) : b->D / 128.0);
+        border = choose_border(work, s);
+    }
     for (int i = 0; i < n_seqs; ++i) {
         const int64_t n_rows = (int64_t)q_len[i] * b->G;
-        int k = b->tc && n_rows > kTcMinRows ? kTc : (!b->pages || n_rows > kRowsMinRows ? kRows : kSplitK);
-        if (!b->pages && f32) k = kRows;
+        int k = n_rows <= border ? kSplitK : (b->tc ? kTc : kRows);
         if (!allowed(k)) k = allowed(kRows) ? kRows : (allowed(kSplitK) ? kSplitK : kTc);
         kind[i] = k;
         if (k == kTc && q8 && q_len[i] > 0) {
@@ -636,7 +726,8 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
             std::stable_sort(tiles[kTc].begin(), tiles[kTc].end(), [&](const Tile& x, const Tile& y) { return n_tiles(x) > n_tiles(y); });
             for (const Tile& t : tiles[kTc]) pair_tiles.push_back(n_tiles(t));
             int n = 0, n_merge = 0, part = 0, piece = 1;
-            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, b->D == 256, &piece);
+            double cost_us;
+            const int whole = choose_tc_cut(pair_tiles, b->Hkv, b->sm_count, b->tc_parts, b->D == 256, &piece, &cost_us);
             b->scratch.clear();
             for (const Tile& t : tiles[kTc]) {
                 const bool cut = &t - tiles[kTc].data() >= whole;
