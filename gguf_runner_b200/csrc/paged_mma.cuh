@@ -592,14 +592,16 @@ __device__ __forceinline__ void paged_store4(const PagedAttnArgs& a, int64_t at,
 __device__ __forceinline__ bool finite4(float4 x) { return isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w); }
 
 constexpr int paged_splitk_warps(int D, int fmt, bool f32) {
-    return D == 256 ? (fmt == kKvQ8Head ? 8 : 6) : (f32 || fmt == kKvQ8Head ? 12 : 8);
+    return D == 256 ? (fmt == kKvQ8Head ? 8 : 6) : ((D == 64 && fmt == kKvQ8Head) || (f32 && fmt != kKvQ8Head) ? 12 : 8);
 }
 
 template <int D, int FMT, bool F32>
 struct PagedSplitKShape {
-    // Warps and ring stages. bf16 on bf16 streams at the memory's rate with eight warps; the others are bound by the latency of a
-    // warp's chain (load, expand codes, multiply, softmax, multiply), so that more warps count for more than deeper rings or
-    // fragments in registers. (16 conversations of 1310 to 20000 keys, 32/4 heads of 128, int8, f32 rows: WARPS_NOTE.)
+    // Warps and ring stages. bf16 on bf16 streams at nine tenths of the memory's rate with eight warps. Where a tile is more
+    // arithmetic, twelve warps hide more of each other's chains (load, multiply, softmax, multiply), if their registers last: 16
+    // conversations of 1310 to 20000 keys, eight warps -> twelve: f32 over bf16 pages, 32/4 heads of 128, 54.7 -> 50.1 us; int8,
+    // 32/8 heads of 64, 55.3 -> 48.5; int8 at head_dim 128 is even (38.4 and 38.5), and one conversation of 700 keys 9.1 -> 9.8, so
+    // that stays at eight.
     static constexpr bool BUSY = F32 || FMT == kKvQ8Head;
     using M = PagedMma<D, FMT, F32, F32, D == 256 || (D == 128 && F32 && FMT == KV_BF16)>;
     static constexpr int R = M::ROWS;
