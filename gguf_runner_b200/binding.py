@@ -316,6 +316,14 @@ def _ptr(x, want_dtype=None):
     return C.c_void_p(a.ctypes.data), PTR_HOST
 
 
+def _int32(name: str, x) -> np.ndarray:
+    """x as contiguous int32, refused where that would change a value."""
+    a = np.asarray(x)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+        raise ValueError(f"{name} must hold 32-bit integers")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 def _raw_stream(device: int) -> int:
     """The cudaStream_t of torch's current stream on a device."""
     import torch
@@ -397,16 +405,18 @@ class Batch:
 
     def set(self, q_len, kv_len=None, page_table=None):
         """page_table: a row of page ids per sequence (a list of lists, or a 2-D array padded with anything)."""
-        q = np.ascontiguousarray(q_len, dtype=np.int32).reshape(-1)
-        kv = q if kv_len is None else np.ascontiguousarray(kv_len, dtype=np.int32).reshape(-1)
+        if not self.ctx._h or not self._h:
+            raise ValueError("the plan or its context has been closed")
+        q = _int32("q_len", q_len).reshape(-1)
+        kv = q if kv_len is None else _int32("kv_len", kv_len).reshape(-1)
         if q.shape != kv.shape:
             raise ValueError("q_len and kv_len have different lengths")
         if page_table is None:
             table = np.empty((q.size, 0), np.int32)
         elif isinstance(page_table, np.ndarray):
-            table = np.ascontiguousarray(page_table, dtype=np.int32)
+            table = _int32("page_table", page_table)
         else:
-            rows = [np.asarray(r, dtype=np.int32).reshape(-1) for r in page_table]
+            rows = [_int32("page_table", r).reshape(-1) for r in page_table]
             table = np.zeros((len(rows), max((r.size for r in rows), default=0)), np.int32)
             for i, r in enumerate(rows):
                 if self.pages is not None and i < kv.size and r.size * self.pages.page_size < kv[i]:
@@ -764,10 +774,10 @@ class AttnContext:
         if _is_torch(x) and x.dtype is dtype and x.is_cuda and x.get_device() == self.config.device and x.dim() == 2:
             rows, cols = x.shape
             step, one = x.stride()
-            if rows >= n and cols == dim and one == 1 and (rows >= most or not _capturing()):
+            if rows >= n and cols == dim and one == 1 and (step >= dim or rows < 2) and (rows >= most or not _capturing()):
                 return x.data_ptr(), step if rows > 1 else dim
         self._check_tensor(name, x, str(dtype)[6:])
-        raise ValueError(f"{name} must have at least {n} rows of {dim} elements, each row contiguous"
+        raise ValueError(f"{name} must have at least {n} rows of {dim} elements, each row contiguous and apart from the others"
                          + (f", and {most} under stream capture" if most > n else ""))
 
     def _row_out(self, like, n, dim, dtype):
@@ -979,9 +989,9 @@ def rope_axis(layout: int, frequency: int, sections: Sequence[int]) -> int:
 def batch_check(q_len, kv_len=None, page_table=None, page_size: int = 0, n_pages: int = 0, max_tokens: int = 1 << 30,
                 max_pages: int = 1 << 30) -> int:
     """The status that Batch.set would raise for these lengths and this 2-D page table, 0 if none. Needs no device."""
-    q = np.ascontiguousarray(q_len, dtype=np.int32).reshape(-1)
-    kv = q if kv_len is None else np.ascontiguousarray(kv_len, dtype=np.int32).reshape(-1)
-    table = np.empty((q.size, 0), np.int32) if page_table is None else np.ascontiguousarray(page_table, dtype=np.int32)
+    q = _int32("q_len", q_len).reshape(-1)
+    kv = q if kv_len is None else _int32("kv_len", kv_len).reshape(-1)
+    table = np.empty((q.size, 0), np.int32) if page_table is None else _int32("page_table", page_table)
     return int(lib().ggr_batch_check(page_size, n_pages, q.size, q.ctypes.data, kv.ctypes.data, table.ctypes.data if table.size else None,
                                      table.shape[1], max_tokens, max_pages))
 

@@ -448,7 +448,7 @@ static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_
     if (max_seqs <= 0 || max_tokens <= 0 || max_pages < (pages ? 1 : 0)) return path_fail(c, GGR_ERR_INVALID, "a batch plan needs room for a sequence, a token and a page");
     if (p.D != 64 && p.D != 128 && p.D != 256) return path_fail(c, GGR_ERR_UNSUPPORTED, "batch plans are built for head_dim 64, 128 and 256");
     if (p.sharded) return path_fail(c, GGR_ERR_UNSUPPORTED, "a context that holds a shard of the positions has no batch plans");
-    if ((int64_t)max_tokens * p.Hq * p.D >= ((int64_t)1 << 40)) return path_fail(c, GGR_ERR_RANGE, "max_tokens is out of range");
+    if ((int64_t)max_tokens * p.G >= ((int64_t)1 << 31)) return path_fail(c, GGR_ERR_RANGE, "max_tokens is out of range");
     Guard guard(p.device);
     std::unique_ptr<ggr_batch, void (*)(ggr_batch*)> b(new (std::nothrow) ggr_batch(), ggr_batch_destroy);
     if (!b) return path_fail(c, GGR_ERR_ALLOC, "out of host memory");

@@ -434,18 +434,18 @@ int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const 
 int ggr_paged_append(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t rotate, const void* q, int64_t q_stride,
                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out);
 /* All kv_len rows of all sequences, sequence after sequence, dequantised into k_out and v_out [rows][kv_dim] (out_dtype, row
- * strides in elements). */
+ * strides in elements). A captured call's buffers have to hold the rows of the longest step that its replays find. */
 int ggr_paged_read(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride,
                    void* v_out, int64_t v_stride);
 /*
  * out[t] = attention of new token t (rotated q) over the visible cached rows of its sequence, its own and those of the
  * chunk's tokens before it included. What a token does not see (later tokens, other sequences, rows that were never written)
- * does not touch its result, whatever it holds.
+ * does not touch its result, whatever it holds. out overlaps neither q nor the pages.
  */
 int ggr_paged_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, void* out,
                         int64_t out_stride);
 /*
- * Causal attention of whole prompts straight from their rotated q, k and v rows, no cache involved.
+ * Causal attention of whole prompts straight from their rotated q, k and v rows, no cache involved. out overlaps none of them.
  */
 int ggr_packed_attention(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, const void* q, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride);

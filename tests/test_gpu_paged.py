@@ -514,9 +514,17 @@ def test_launches_keep_their_order(d, kv, dtype):
     gen = torch.Generator(device="cuda").manual_seed(24)
     steps = [torch.randn(3, 63, 8 * d, generator=gen, device="cuda").to(c.dtype) for _ in range(6)]
 
+    arrays = [x for x in c.pool + c.scales if x is not None]
+    start = [x.clone() for x in arrays]
+
     def play(wait):
         got = []
-        for x in steps:
+        for x, s in zip(arrays, start):
+            x.copy_(s)
+        for i, x in enumerate(steps):
+            # a plan of its own for every step: nothing may be read of the one before
+            kv_len = [c.kv_len[0] - 61 * i, c.kv_len[1] - 17 * i, c.kv_len[2] - i]
+            c.batch.set(c.q_len, kv_len, c.table)
             q = x[0] * 1.0  # a kernel of torch's in front
             k, v = x[1, :, :2 * d] * 1.0, x[2, :, :2 * d] * 1.0
             wait()
@@ -531,7 +539,6 @@ def test_launches_keep_their_order(d, kv, dtype):
             again = c.ctx.paged_attention(c.batch, 0, turned)
             wait()
             turned.zero_()
-            c.batch.set(c.q_len, c.kv_len, c.table)
             got += [out, again, *(r[torch.isfinite(r)] for r in rows)]
         torch.cuda.synchronize()
         return got
@@ -547,6 +554,20 @@ def test_results_repeat_bit_for_bit():
     first = c.ctx.paged_attention(c.batch, 0, c.q).clone()
     for _ in range(5):
         assert torch.equal(c.ctx.paged_attention(c.batch, 0, c.q), first)
+
+
+def test_more_heads_than_a_query_tile_has_rows():
+    c = Case(160, 1, 64, "bf16", "bf16", 16, [1, 9], [70, 300], seed=25)
+    c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+
+
+def test_closed_handles_are_refused():
+    c = Case(4, 2, 64, "bf16", "bf16", 16, [1], [5])
+    c.ctx.close()
+    with pytest.raises(ValueError):
+        c.batch.set([1], [5], c.table)
+    with pytest.raises(GgrError):
+        c.ctx.paged_attention(c.batch, 0, c.q)
 
 
 def test_prescaled_queries():
@@ -601,6 +622,12 @@ def test_refusals():
         ctx.paged_attention(batch, 0, q[:2])
     with pytest.raises(ValueError):
         ctx.paged_attention(batch, 0, q.T.contiguous().T)
+    with pytest.raises(ValueError):  # one row for all tokens
+        ctx.paged_attention(batch, 0, q[:1].expand(20, 1024))
+    with pytest.raises(ValueError):
+        batch.set([1], [1], [[2 ** 32]])
+    with pytest.raises(ValueError):
+        batch.set([1.5], [2], [[0]])
     with pytest.raises(GgrError):  # rows off the 16-byte grid
         ctx.paged_attention(batch, 0, torch.zeros(20, 1025, device="cuda", dtype=torch.bfloat16)[:, 1:])
     packed = g.Batch(ctx, None, "bf16", 2, 20)
