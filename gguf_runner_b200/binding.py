@@ -324,11 +324,17 @@ def _int32(name: str, x) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.int32)
 
 
+_RAW_STREAM = None
+
+
 def _raw_stream(device: int) -> int:
     """The cudaStream_t of torch's current stream on a device."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (without a Stream object: 0.2 us instead of 1.2)
-    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+    global _RAW_STREAM
+    if _RAW_STREAM is None:
+        import torch
+        # (without a Stream object: 0.2 us instead of 1.2)
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _RAW_STREAM(device)
 
 
 def _capturing() -> bool:
@@ -457,6 +463,7 @@ class AttnContext:
             raise GgrError(st, self._L.ggr_attn_create_error().decode())
         self._h = handle
         self._stream = None
+        self._device, self._q_dim, self._kv_dim = config.device, config.q_dim, config.kv_dim
 
     def _follow_torch_stream(self, *tensors):
         """Device-pointer calls are enqueued on torch's current stream, so they are
@@ -771,9 +778,12 @@ class AttnContext:
     def _rows(self, name, x, dtype, n, dim, most=0):
         """Address and row stride of `n` rows (a [rows][dim] tensor whose elements of a row lie together). A captured call needs
         `most` rows: replays may find a longer plan. (A token step is a few of these calls: the checks take 0.6 us.)"""
-        if _is_torch(x) and x.dtype is dtype and x.is_cuda and x.get_device() == self.config.device and x.dim() == 2:
-            rows, cols = x.shape
-            step, one = x.stride()
+        try:
+            same = x.dtype is dtype and x.get_device() == self._device
+            (rows, cols), (step, one) = x.shape, x.stride()
+        except (AttributeError, TypeError, ValueError):
+            same = False
+        if same:
             if rows >= n and cols == dim and one == 1 and (step >= dim or rows < 2) and (rows >= most or not _capturing()):
                 return x.data_ptr(), step if rows > 1 else dim
         self._check_tensor(name, x, str(dtype)[6:])
@@ -786,20 +796,20 @@ class AttnContext:
 
     def paged_append(self, batch: Batch, layer: int, k, v, q=None, q_out=None):
         """Rows of k and v into the pages of the batch's new tokens. With q: RoPE on q and k first; returns rotated q."""
-        c, n, dt, most = self.config, batch.n_tokens, batch.torch_dtype, batch.max_tokens
-        kp, ks = self._rows("k", k, dt, n, c.kv_dim, most)
-        vp, vs = self._rows("v", v, dt, n, c.kv_dim, most)
+        n, dt, most, q_dim, kv_dim = batch.n_tokens, batch.torch_dtype, batch.max_tokens, self._q_dim, self._kv_dim
+        kp, ks = self._rows("k", k, dt, n, kv_dim, most)
+        vp, vs = self._rows("v", v, dt, n, kv_dim, most)
         qp, qs, op = None, 0, None
         if q is not None:
             if q_out is None:
-                q_out = self._row_out(q, most if _capturing() else n, c.q_dim, dt)
-            qp, qs = self._rows("q", q, dt, n, c.q_dim, most)
-            op, os_ = self._rows("q_out", q_out, dt, n, c.q_dim, most)
-            if os_ != c.q_dim:
+                q_out = self._row_out(q, most if _capturing() else n, q_dim, dt)
+            qp, qs = self._rows("q", q, dt, n, q_dim, most)
+            op, os_ = self._rows("q_out", q_out, dt, n, q_dim, most)
+            if os_ != q_dim:
                 raise ValueError("q_out must be dense")
         elif q_out is not None:
             raise ValueError("q_out without q")
-        self._follow_torch_stream(k)
+        self._follow_torch_stream_of_device()
         self._check(self._L.ggr_paged_append(self._h, batch._h, layer, 0 if q is None else 1, qp, qs, kp, ks, vp, vs, op))
         return q_out
 
@@ -814,18 +824,18 @@ class AttnContext:
             k_out, v_out = (torch.empty((n, c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
         kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim)
         vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim)
-        self._follow_torch_stream(k_out)
+        self._follow_torch_stream_of_device()
         self._check(self._L.ggr_paged_read(self._h, batch._h, layer, DTYPES[dtype], kp, ks, vp, vs))
         return k_out, v_out
 
     def paged_attention(self, batch: Batch, layer: int, q, out=None):
         """Attention of the batch's new tokens (rotated q) over their sequences' pages."""
-        c, n, dt, most = self.config, batch.n_tokens, batch.torch_dtype, batch.max_tokens
+        n, dt, most, q_dim = batch.n_tokens, batch.torch_dtype, batch.max_tokens, self._q_dim
         if out is None:
-            out = self._row_out(q, most if _capturing() else n, c.q_dim, dt)
-        qp, qs = self._rows("q", q, dt, n, c.q_dim, most)
-        op, os_ = self._rows("out", out, dt, n, c.q_dim, most)
-        self._follow_torch_stream(q)
+            out = self._row_out(q, most if _capturing() else n, q_dim, dt)
+        qp, qs = self._rows("q", q, dt, n, q_dim, most)
+        op, os_ = self._rows("out", out, dt, n, q_dim, most)
+        self._follow_torch_stream_of_device()
         self._check(self._L.ggr_paged_attention(self._h, batch._h, layer, qp, qs, op, os_))
         return out
 
