@@ -4,7 +4,7 @@
 //     o = sum_j p_j v_j / sum_j p_j,   p_j = 2^((s_j - m) c),   s_j = q . k_j,   c = scale * log2 e.
 //
 // Two forms of one tile step (16 rows x 16 keys, PagedMma::step):
-//  - paged_splitk_kernel: the eight (head_dim 256: four) warps of a CTA share 16 rows and split the keys between them, each
+//  - paged_splitk_kernel: the six to twelve warps of a CTA share 16 rows and split the keys between them, each
 //    with a ring of its own that TMA fills; states are merged in shared memory, and over CTAs by the last one to finish a row
 //    tile. Bound by the bytes of the cache: for a few tokens times G heads every cache byte is read once.
 //  - paged_rows_kernel: eight warps with 16 rows each walk the same keys through one ring, which a ninth warp fills.
@@ -272,7 +272,7 @@ struct PagedMma {
     }
 
     // A tile's share of four elements of o. The tensor core adds into its accumulator by truncation, which over hundreds of tiles
-    // goes one way (3e-9 of o per tile measured): in f32 a tile is summed from zero and then added, rounded to nearest.
+    // goes one way (1.4e-6 of o after 37 tiles): in f32 a tile is summed from zero and then added, rounded to nearest.
     struct Sum {
         float c[4];
         __device__ __forceinline__ explicit Sum(const float (&o)[4]) {
