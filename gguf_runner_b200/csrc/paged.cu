@@ -512,9 +512,7 @@ static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_
               cudaMalloc((void**)&b->d_tickets, b->part_tiles * p.Hkv * sizeof(unsigned)) == cudaSuccess;
     if (ok && !pages && dtype == GGR_DTYPE_F32)
         ok = cudaMalloc((void**)&b->d_planes, (size_t)6 * max_tokens * p.Hkv * p.D * sizeof(__nv_bfloat16)) == cudaSuccess;
-    if (ok && b->tc)
-        ok = cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 128 * tc_item_tiles(p.D) * (p.D + 2) * sizeof(float)) == cudaSuccess &&
-             cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
+    if (ok && b->tc) ok = cudaMalloc((void**)&b->d_sched, 2 * sizeof(int)) == cudaSuccess;
     if (ok && b->tc && pages && pages->v.fmt == GGR_KV_Q8_HEAD)
         ok = cudaMalloc((void**)&b->d_q16, (size_t)max_tokens * p.Hq * p.D * sizeof(__half)) == cudaSuccess;
     for (int i = 0; ok && i < 2; ++i)
@@ -618,6 +616,12 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
         } else if (k == kTc && !b->pages) {
             lin[i] = seqs[i].tok0;
         }
+    }
+    // (39 MB that a plan of token steps never needs)
+    if (!b->d_tc_part && std::find(kind.begin(), kind.end(), (int)kTc) != kind.end() &&
+        cudaMalloc((void**)&b->d_tc_part, b->tc_parts * 128 * tc_item_tiles(b->D) * (b->D + 2) * sizeof(float)) != cudaSuccess) {
+        cudaGetLastError();
+        return path_fail(c, GGR_ERR_ALLOC, "unable to allocate the partial states of a batch plan");
     }
     if (dense > (int64_t)b->dense_rows) {
         if (!b->captured || !b->d_dense) {
