@@ -385,12 +385,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 for (int cidx = 0; cidx < 4; ++cidx)
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        mxa = max3(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
-                        mxb = max3(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
-                        mxc = max3(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
-                        mxd = max3(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
+                        mxa = max3_nan(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
+                        mxb = max3_nan(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
+                        mxc = max3_nan(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
+                        mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                     }
-                const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+                const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
                 const bool need = mx > m_used + thr;
                 float alpha = 1.0f;
                 if (need) {
@@ -408,7 +408,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         tmem_st32(tO + cidx * 32, orow);
                     }
                 }
-                l *= alpha;
+                // (a NaN score: the polynomial, which clamps its argument, would give that key weight 0, so it goes into the sum here)
+                l = mx == mx ? l * alpha : mx;
                 const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
                 const float neg = -mref * c;
                 const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
@@ -464,6 +465,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             cs += n_t;
             if (!(ok = mbar_wait(o_final(t), it & 1, abortp))) break;
             fence_after_sync();
+            if (m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
             const bool split = w.part >= 0;
             float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPtState<D>;
             if (split) __stcg(reinterpret_cast<float2*>(state + 256 * D) + t * 128 + row, make_float2(n_t > 0 ? m_used : -INFINITY, n_t > 0 ? l : 0.0f));

@@ -248,12 +248,12 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             for (int cidx = 0; cidx < 2; ++cidx)
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
-                    mxa = max3(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
-                    mxb = max3(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
-                    mxc = max3(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
-                    mxd = max3(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
+                    mxa = max3_nan(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
+                    mxb = max3_nan(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
+                    mxc = max3_nan(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
+                    mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                 }
-            const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+            const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
             const bool need = mx > m_used + thr;
             float alpha = 1.0f;
             if (need) {
@@ -275,7 +275,8 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     tmem_st32(tO + cidx * 32, orow);
                 }
             }
-            l *= alpha;
+            // (a NaN score: see paged_tc.cuh)
+            l = mx == mx ? l * alpha : mx;
             const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
             const float neg = -mref * c;
             const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
@@ -327,6 +328,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             if (n > 0 && !rescale_now && !(ok = mbar_wait(pv_done((n - 1) & 1), ((n - 1) >> 1) & 1, abortp))) break;
         }
         if (ok && hi > lo) ok = mbar_wait(o_final, 0, abortp);
+        if (m_used == INFINITY) l = NAN;  // (see paged_tc.cuh)
         const bool split = w.part >= 0;
         float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPwState;
         if (ok && split && valid) __stcg(reinterpret_cast<float2*>(state + 128 * D) + row, make_float2(hi > lo ? m_used : -INFINITY, hi > lo ? l : 0.0f));

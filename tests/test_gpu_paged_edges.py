@@ -1,0 +1,69 @@
+"""Where the paged operators can go wrong: values that are not finite, rows and scales at the ends of their ranges, empty steps,
+plans that are refused, closed or captured, against plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+import gguf_runner_b200 as g
+from gguf_runner_b200.binding import GgrError
+from tests import paged_reference as ref
+from tests.test_gpu_paged import TYPES, Case, context, tables
+
+pytestmark = pytest.mark.gpu
+
+
+def without(case, seq, key):
+    """The 64-bit result, as `ref.attention` gives it, of sequence `seq` with key `key`, which all its rows see, left out."""
+    at, n = sum(case.q_len[:seq]), case.q_len[seq]
+    k, v = (torch.cat([x[:key], x[key + 1:]]) for x in case.rows[seq])
+    return ref.attention(case.q[at:at + n].view(n, case.hq, case.d), k, v, case.kv_len[seq] - n - 1, 0, case.scale)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv,bad", [("bf16", math.nan), ("bf16", math.inf), ("bf16", -math.inf), ("q8_head", math.nan)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_key_that_is_not_finite_counts_wherever_it_stands(d, kv, bad, dtype):
+    """One element of one key of KV head 1, at every residue of 8: a score of NaN or +inf makes the rows of its heads NaN, one of
+    -inf has weight 0; the other KV head is left as it is."""
+    c = Case(4, 2, d, kv, dtype, 16, [150] * 8, [300] * 8, seed=31)
+    c.q.view(-1, 4, d)[:, :, 0] = 1.0
+    for b in range(8):
+        page, row = c.table[b][(96 + b) // 16], (96 + b) % 16
+        if kv == "bf16":
+            c.pool[0][0, page, 1, row, 0] = bad
+        else:
+            c.scales[0][0, page, 1, row] = bad
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(8, 150, 4, d)
+    out, size, reach = (x.view(8, 150, 4, d) for x in c.want())
+    off = (got.double() - out).abs() <= ref.bound(c.dtype, out, size, reach)
+    assert bool(off[:, :, :2].all())
+    for b in range(8):
+        mine = got[b, :, 2:]
+        if bad != -math.inf:
+            assert bool(mine.isnan().all()), (b, float(mine.isnan().double().mean()))
+        else:
+            w, size, reach = without(c, b, 96 + b)
+            ok = (got[b].double() - w).abs() <= ref.bound(c.dtype, w, size, reach)
+            assert bool(ok[:, 2:].all()), b
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_nan_key_of_packed_prompts_counts_wherever_it_stands(d, dtype):
+    lens, t = [200] * 8, TYPES[dtype]
+    ctx = context(4, 2, d)
+    batch = g.Batch(ctx, None, dtype, 8, 1600)
+    batch.set(lens)
+    gen = torch.Generator(device="cuda").manual_seed(32)
+    q, k, v = (torch.randn(1600, h, d, generator=gen, device="cuda").to(t) for h in (4, 2, 2))
+    spoilt = k.clone()
+    for b in range(8):
+        spoilt[200 * b + 96 + b, 1, 5] = math.nan
+    got = ctx.packed_attention(batch, 0, q.view(1600, -1), spoilt.view(1600, -1), v.view(1600, -1)).view(8, 200, 4, d)
+    for b in range(8):
+        s = slice(200 * b, 200 * b + 200)
+        out, size, reach = ref.attention(q[s], k[s], v[s], 0, 0, 1 / math.sqrt(d))
+        ok = (got[b].double() - out).abs() <= ref.bound(t, out, size, reach)
+        assert bool(ok[:, :2].all()) and bool(ok[:96 + b].all())
+        assert bool(got[b, 96 + b:, 2:].isnan().all()), b
