@@ -84,7 +84,8 @@ __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const Paged
         float s = 0.0f;
         for (int i = 0; i < E; ++i) s = fmaf(q[i], at(a.pk, a.pk_stride, a.pages.k, a.pages.ks, j, lane + 32 * i), s);
         s = warp_sum(s) * a.c;
-        const float top = fmaxf(m, s), f = m == top ? 1.0f : exp2f(m - top), p = exp2f(s - top);
+        // (a score of -inf has weight 0, also while there is no larger one to measure it by)
+        const float top = fmaxf(m, s), f = m == top ? 1.0f : exp2f(m - top), p = s == -INFINITY ? 0.0f : exp2f(s - top);
         m = top;
         l = l * f + p;
         for (int i = 0; i < E; ++i) o[i] = o[i] * f + p * at(a.pv, a.pv_stride, a.pages.v, a.pages.vs, j, lane + 32 * i);

@@ -67,3 +67,24 @@ def test_a_nan_key_of_packed_prompts_counts_wherever_it_stands(d, dtype):
         ok = (got[b].double() - out).abs() <= ref.bound(t, out, size, reach)
         assert bool(ok[:, :2].all()) and bool(ok[:96 + b].all())
         assert bool(got[b, 96 + b:, 2:].isnan().all()), b
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_first_score_of_minus_infinity(d, n, dtype):
+    """The first key scores -inf and a later token's value is not finite: the rows in between see the one with weight 0 and the
+    other not at all."""
+    c = Case(4, 2, d, "bf16", dtype, 16, [n], [n], seed=33)
+    c.q.view(n, 4, d)[:, :, 0] = 1.0
+    c.pool[0][0, c.table[0][0], 1, 0, 0] = -math.inf
+    c.pool[1][0, c.table[0][1], 1, 5, 3] = math.nan  # position 21
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(n, 4, d)
+    k, v = (x[1:] for x in c.rows[0])
+    out, size, reach = ref.attention(c.q.view(n, 4, d)[1:], k, v, 0, 0, c.scale)
+    ok = (got[1:].double() - out).abs() <= ref.bound(c.dtype, out, size, reach)
+    heads = got[:, 2:]
+    assert bool(ok[:20, 2:].all()), float(heads[1:21].isnan().double().mean())
+    assert bool(heads[21:, :, 3].isnan().all())
+    ok[:, :, 3] = True
+    assert bool(ok[20:, 2:].all())
