@@ -467,6 +467,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             fence_after_sync();
             if (m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
             const bool split = w.part >= 0;
+            if (m_used == -INFINITY && l == l) l = split ? 0.0f : NAN;  // only scores of -inf: no softmax; a piece without weight
             float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPtState<D>;
             if (split) __stcg(reinterpret_cast<float2*>(state + 256 * D) + t * 128 + row, make_float2(n_t > 0 ? m_used : -INFINITY, n_t > 0 ? l : 0.0f));
             bool bad = false;

@@ -330,6 +330,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         if (ok && hi > lo) ok = mbar_wait(o_final, 0, abortp);
         if (m_used == INFINITY) l = NAN;  // (see paged_tc.cuh)
         const bool split = w.part >= 0;
+        if (m_used == -INFINITY && l == l) l = split ? 0.0f : NAN;
         float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPwState;
         if (ok && split && valid) __stcg(reinterpret_cast<float2*>(state + 128 * D) + row, make_float2(hi > lo ? m_used : -INFINITY, hi > lo ? l : 0.0f));
         bool bad = false;

@@ -88,3 +88,30 @@ def test_a_first_score_of_minus_infinity(d, n, dtype):
     assert bool(heads[21:, :, 3].isnan().all())
     ok[:, :, 3] = True
     assert bool(ok[20:, 2:].all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [20, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_whose_scores_are_all_minus_infinity(d, n, dtype):
+    """No key has a weight: 0 / 0, as the softmax of such a row is, and not the mean or zero."""
+    c = Case(4, 2, d, "bf16", dtype, 16, [n], [n], seed=39)
+    c.q.view(n, 4, d)[:, :, 0] = 1.0
+    c.pool[0][0, c.table[0][0], 1, :9, 0] = -math.inf
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(n, 4, d)
+    out, size, reach = ref.attention(c.q.view(n, 4, d)[9:], *(x[9:] for x in c.rows[0]), 0, 0, c.scale)
+    assert bool(got[:9, 2:].isnan().all())
+    assert bool(((got[9:].double() - out).abs() <= ref.bound(c.dtype, out, size, reach))[:, 2:].all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_pieces_whose_scores_are_all_minus_infinity(d, dtype):
+    """Few rows and many keys, cut along the keys: what lies in the first half has no weight."""
+    c = Case(4, 2, d, "bf16", dtype, 64, [70], [7000], seed=40)
+    c.q.view(70, 4, d)[:, :, 0] = 1.0
+    for p in range(0, 3520, 64):
+        c.pool[0][0, c.table[0][p // 64], 1, :, 0] = -math.inf
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(70, 4, d)
+    out, size, reach = ref.attention(c.q.view(70, 4, d), *(x[3520:] for x in c.rows[0]), 6930 - 3520, 0, c.scale)
+    assert bool(((got.double() - out).abs() <= ref.bound(c.dtype, out, size, reach))[:, 2:].all())
