@@ -544,6 +544,8 @@ static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_
 
 static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table, int32_t table_stride) {
     if (!b) return GGR_ERR_INVALID;
+    // a step that is refused is not the one before: the caller's rows are no longer that step's
+    b->set = false;
     ggr_attn_ctx* c = b->ctx;
     const PathView p = path_view(c);
     if (n_seqs > b->max_seqs) return path_fail(c, GGR_ERR_RANGE, "more sequences than the batch plan holds");
@@ -558,7 +560,6 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
     const int turn = b->turn;
     unsigned char* h = b->h_plan[turn];
     if (b->up_used[turn]) PAGED_TRY(c, cudaEventSynchronize(b->up[turn]));
-    b->set = false;
     int* tok_pos = reinterpret_cast<int*>(h + b->at_pos);
     int* tok_slot = reinterpret_cast<int*>(h + b->at_slot);
     int2* entry = reinterpret_cast<int2*>(h + b->at_entries);

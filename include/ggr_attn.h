@@ -421,7 +421,8 @@ void ggr_batch_destroy(ggr_batch* batch);
  * reused: their entries only have to name a page. The call copies its arrays and enqueues their upload; it does not belong into a
  * stream capture, but captured launches of the plan follow it when they are replayed behind it. A captured call has to be
  * given buffers of max_tokens rows, as replays may find a longer step; it holds the kernels of the step it was captured with,
- * and the plan keeps to those from then on: token steps that are replayed are best given a plan of their own.
+ * and the plan keeps to those from then on: token steps that are replayed are best given a plan of their own. After a call that
+ * fails the plan has no step: the calls below refuse it until one has been set.
  */
 int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const int32_t* kv_len, const int32_t* page_table,
                   int32_t table_stride);

@@ -115,3 +115,26 @@ def test_pieces_whose_scores_are_all_minus_infinity(d, dtype):
     got = c.ctx.paged_attention(c.batch, 0, c.q).view(70, 4, d)
     out, size, reach = ref.attention(c.q.view(70, 4, d), *(x[3520:] for x in c.rows[0]), 6930 - 3520, 0, c.scale)
     assert bool(((got.double() - out).abs() <= ref.bound(c.dtype, out, size, reach))[:, 2:].all())
+
+
+@pytest.mark.parametrize("step", [dict(q_len=[9, 1], kv_len=[9, 1]), dict(q_len=[1] * 3, kv_len=[1] * 3), dict(q_len=[-1, 1], kv_len=[1, 1]),
+                                  dict(q_len=[1, 1], kv_len=[1, 1], page_table=[[99], [0]])])
+def test_a_refused_step_does_not_leave_the_one_before_in_force(step):
+    """Whoever goes on has other rows than those of the step before: every call is refused until a step has been set."""
+    c = Case(4, 2, 64, "bf16", "bf16", 16, [2, 3], [20, 40], seed=41)
+    want = c.ctx.paged_attention(c.batch, 0, c.q)
+    packed = g.Batch(c.ctx, None, "bf16", 2, 5)
+    packed.set([2, 3])
+    k = torch.zeros(5, 128, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(GgrError):
+        c.batch.set(**{"page_table": [[0], [1], [2]][:len(step["q_len"])], **step})
+    if "page_table" not in step:
+        with pytest.raises(GgrError):
+            packed.set(step["q_len"])
+        with pytest.raises(GgrError):
+            c.ctx.packed_attention(packed, 0, c.q, k, k)
+    for call in (lambda: c.ctx.paged_attention(c.batch, 0, c.q), lambda: c.ctx.paged_append(c.batch, 0, k, k), lambda: c.ctx.paged_read(c.batch, 0)):
+        with pytest.raises(GgrError):
+            call()
+    c.batch.set(c.q_len, c.kv_len, c.table)
+    assert torch.equal(c.ctx.paged_attention(c.batch, 0, c.q), want)
