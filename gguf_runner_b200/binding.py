@@ -401,6 +401,8 @@ class Batch:
     def __init__(self, ctx: "AttnContext", pages: Optional[Pages], dtype: str, max_seqs: int, max_tokens: int, max_pages: int = 0):
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
+        if pages is not None and not pages._h:
+            raise ValueError("the page pool has been closed")
         self._L, self.ctx, self.pages, self.dtype = lib(), ctx, pages, dtype
         self.max_tokens, self.n_tokens, self.n_rows = max_tokens, 0, 0
         self.torch_dtype = _torch_dtype(dtype)
@@ -413,6 +415,8 @@ class Batch:
         """page_table: a row of page ids per sequence (a list of lists, or a 2-D array padded with anything)."""
         if not self.ctx._h or not self._h:
             raise ValueError("the plan or its context has been closed")
+        if self.pages is not None and not self.pages._h:
+            raise ValueError("the page pool of the plan has been closed")
         q = _int32("q_len", q_len).reshape(-1)
         kv = q if kv_len is None else _int32("kv_len", kv_len).reshape(-1)
         if q.shape != kv.shape:

@@ -33,6 +33,8 @@ struct ggr_pages {
     int device, n_layers, page_size;
     PageView v{};
     void* owned[4] = {nullptr, nullptr, nullptr, nullptr};
+    int users = 0;         // batch plans on the pool, which read it: the last of them gives a destroyed pool's memory back
+    bool destroyed = false;
     CUtensorMap tmK16, tmV16;    // 16 rows of a page, one 64- or 128-byte block of columns
     CUtensorMap tmK128, tmV128;  // bf16: min(page_size, 128) rows (head_dim 256: at most 64)
 };
@@ -43,6 +45,7 @@ namespace {
 constexpr int tc_key_tile(int D) { return D == 256 ? kPwBN : 128; }
 constexpr int tc_item_tiles(int D) { return D == 256 ? 1 : 2; }
 constexpr int kMaxLists = 4;  // distinct windows of a model's layers
+constexpr char kPagesGone[] = "the page pool of the batch plan has been destroyed";
 // lists of a plan: items of the three attention kernels, and the pairs of query tiles whose pieces are merged
 enum Kind { kSplitK = 0, kRows = 1, kTc = 2, kMerge = 3, kKinds = 4 };
 
@@ -400,11 +403,16 @@ static int pages_create(ggr_attn_ctx* c, int32_t n_pages, int32_t page_size, int
     return GGR_OK;
 }
 
-extern "C" void ggr_pages_destroy(ggr_pages* pages) {
-    if (!pages) return;
+static void pages_free(ggr_pages* pages) {
     Guard guard(pages->device);
     for (void* x : pages->owned) cudaFree(x);  // (cudaFree waits for the work that uses it)
     delete pages;
+}
+
+extern "C" void ggr_pages_destroy(ggr_pages* pages) {
+    if (!pages || pages->destroyed) return;
+    pages->destroyed = true;
+    if (!pages->users) pages_free(pages);
 }
 
 extern "C" int ggr_pages_device_ptrs(const ggr_pages* pages, void** k, void** v, float** k_scale, float** v_scale, uint64_t* array_bytes) {
@@ -435,6 +443,7 @@ extern "C" void ggr_batch_destroy(ggr_batch* b) {
     cudaFree(b->d_sched);
     cudaFree(b->d_dense);
     cudaFree(b->d_q16);
+    if (b->pages && --b->pages->users == 0 && b->pages->destroyed) pages_free(b->pages);
     delete b;
 }
 
@@ -444,6 +453,7 @@ static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_
     *out = nullptr;
     const PathView p = path_view(c);
     if (pages && pages->ctx != c) return path_fail(c, GGR_ERR_INVALID, "the pages belong to another context");
+    if (pages && pages->destroyed) return path_fail(c, GGR_ERR_INVALID, kPagesGone);
     if (dtype != GGR_DTYPE_F32 && dtype != GGR_DTYPE_BF16) return path_fail(c, GGR_ERR_INVALID, "unknown dtype");
     if (max_seqs <= 0 || max_tokens <= 0 || max_pages < (pages ? 1 : 0)) return path_fail(c, GGR_ERR_INVALID, "a batch plan needs room for a sequence, a token and a page");
     if (p.D != 64 && p.D != 128 && p.D != 256) return path_fail(c, GGR_ERR_UNSUPPORTED, "batch plans are built for head_dim 64, 128 and 256");
@@ -454,6 +464,7 @@ static int batch_create(ggr_attn_ctx* c, ggr_pages* pages, int32_t dtype, int32_
     if (!b) return path_fail(c, GGR_ERR_ALLOC, "out of host memory");
     b->ctx = c;
     b->pages = pages;
+    if (pages) ++pages->users;
     b->device = p.device;
     b->dtype = dtype;
     b->max_seqs = max_seqs;
@@ -548,6 +559,7 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
     b->set = false;
     ggr_attn_ctx* c = b->ctx;
     const PathView p = path_view(c);
+    if (b->pages && b->pages->destroyed) return path_fail(c, GGR_ERR_INVALID, kPagesGone);
     if (n_seqs > b->max_seqs) return path_fail(c, GGR_ERR_RANGE, "more sequences than the batch plan holds");
     const int ps = b->pages ? b->pages->page_size : 0;
     BatchTotals totals;
@@ -801,6 +813,7 @@ namespace {
 
 int check_call(ggr_attn_ctx* c, ggr_batch* b, int layer, bool wants_pages) {
     if (!b || b->ctx != c) return path_fail(c, GGR_ERR_INVALID, "the batch plan belongs to another context");
+    if (b->pages && b->pages->destroyed) return path_fail(c, GGR_ERR_INVALID, kPagesGone);
     if (!b->set) return path_fail(c, GGR_ERR_INVALID, "the batch plan has not been set");
     if (layer < 0 || layer >= b->n_layers) return path_fail(c, GGR_ERR_RANGE, "layer outside the cache");
     if (wants_pages && !b->pages) return path_fail(c, GGR_ERR_INVALID, "the batch plan has no pages");

@@ -399,7 +399,7 @@ typedef struct ggr_batch ggr_batch;
  */
 int ggr_pages_create(ggr_attn_ctx* ctx, int32_t n_pages, int32_t page_size, int32_t kv_format, void* k, void* v,
                      float* k_scale, float* v_scale, ggr_pages** out);
-/* After the batch plans that use the pool. */
+/* Batch plans on the pool are refused from then on; its memory goes back with the last of them. */
 void ggr_pages_destroy(ggr_pages* pages);
 int ggr_pages_device_ptrs(const ggr_pages* pages, void** k, void** v, float** k_scale, float** v_scale,
                           uint64_t* array_bytes);

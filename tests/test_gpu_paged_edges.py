@@ -138,3 +138,31 @@ def test_a_refused_step_does_not_leave_the_one_before_in_force(step):
             call()
     c.batch.set(c.q_len, c.kv_len, c.table)
     assert torch.equal(c.ctx.paged_attention(c.batch, 0, c.q), want)
+
+
+def test_a_pool_outlives_the_plans_on_it():
+    """A closed pool's plans are refused by every call; its memory is there until the last of them is closed."""
+    ctx = context(8, 8, 128, layers=4)
+    start = torch.cuda.mem_get_info()[0]
+    pages = g.Pages(ctx, 1000, 256)  # 2 x 2 GB
+    plans = [g.Batch(ctx, pages, "bf16", 1, 4, 2) for _ in range(2)]
+    k, q = (torch.zeros(4, h * 128, dtype=torch.bfloat16, device="cuda") for h in (8, 8))
+    for p in plans:
+        p.set([4], [4], [[7]])
+        ctx.paged_append(p, 0, k, k)
+    pages.close()
+    pages.close()
+    for call in (lambda p: p.set([4], [4], [[7]]), lambda p: ctx.paged_append(p, 0, k, k), lambda p: ctx.paged_attention(p, 0, q),
+                 lambda p: ctx.paged_read(p, 0)):
+        for p in plans:
+            with pytest.raises((ValueError, GgrError)):
+                call(p)
+    with pytest.raises(ValueError):
+        g.Batch(ctx, pages, "bf16", 1, 4, 2)
+    with pytest.raises(GgrError):
+        pages.device_ptrs()
+    torch.cuda.synchronize()
+    plans[0].close()
+    assert start - torch.cuda.mem_get_info()[0] > 2 << 30
+    plans[1].close()
+    assert start - torch.cuda.mem_get_info()[0] < 1 << 30
