@@ -405,6 +405,7 @@ class Batch:
             raise ValueError("the page pool has been closed")
         self._L, self.ctx, self.pages, self.dtype = lib(), ctx, pages, dtype
         self.max_tokens, self.n_tokens, self.n_rows = max_tokens, 0, 0
+        self.max_rows = 0 if pages is None else max_pages * pages.page_size
         self.torch_dtype = _torch_dtype(dtype)
         h = C.c_void_p()
         ctx._check(self._L.ggr_batch_create(ctx._h, None if pages is None else pages._h, DTYPES[dtype], max_seqs, max_tokens, max_pages,
@@ -818,16 +819,16 @@ class AttnContext:
         return q_out
 
     def paged_read(self, batch: Batch, layer: int, dtype: str = "bf16", k_out=None, v_out=None):
-        """All cached rows of all sequences of the batch, dequantised: (k, v), each [sum of kv_len][kv_dim]. (A captured call
-        is not told how long later plans are: its tensors have to hold the longest.)"""
+        """All cached rows of all sequences of the batch, dequantised: (k, v), each [sum of kv_len][kv_dim]. (Replays of a
+        captured call may find a longer plan: its tensors have the rows of all pages that the plan may name.)"""
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
-        dt, c, n = _torch_dtype(dtype), self.config, batch.n_rows
+        dt, c, n, most = _torch_dtype(dtype), self.config, batch.n_rows, batch.max_rows
         if k_out is None or v_out is None:
             import torch
-            k_out, v_out = (torch.empty((n, c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
-        kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim)
-        vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim)
+            k_out, v_out = (torch.empty((most if _capturing() else n, c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
+        kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim, most)
+        vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim, most)
         self._follow_torch_stream_of_device()
         self._check(self._L.ggr_paged_read(self._h, batch._h, layer, DTYPES[dtype], kp, ks, vp, vs))
         return k_out, v_out

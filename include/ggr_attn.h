@@ -435,7 +435,7 @@ int ggr_batch_set(ggr_batch* batch, int32_t n_seqs, const int32_t* q_len, const 
 int ggr_paged_append(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t rotate, const void* q, int64_t q_stride,
                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out);
 /* All kv_len rows of all sequences, sequence after sequence, dequantised into k_out and v_out [rows][kv_dim] (out_dtype, row
- * strides in elements). A captured call's buffers have to hold the rows of the longest step that its replays find. */
+ * strides in elements). A captured call's buffers have max_pages * page_size rows: replays may find a longer step. */
 int ggr_paged_read(ggr_attn_ctx* ctx, ggr_batch* batch, int32_t layer, int32_t out_dtype, void* k_out, int64_t k_stride,
                    void* v_out, int64_t v_stride);
 /*

@@ -166,3 +166,27 @@ def test_a_pool_outlives_the_plans_on_it():
     assert start - torch.cuda.mem_get_info()[0] > 2 << 30
     plans[1].close()
     assert start - torch.cuda.mem_get_info()[0] < 1 << 30
+
+
+def test_a_captured_read_has_room_for_the_longest_step():
+    c = Case(4, 2, 64, "bf16", "bf16", 16, [1, 1], [20, 40], seed=36)
+    most = 5 * 16  # the plan has room for five pages
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    small, large = (torch.zeros(2, n, 128, device="cuda") for n in (60, most))
+    with torch.cuda.stream(side):
+        c.batch.set([0, 0], [20, 10], c.table)
+        c.ctx.paged_read(c.batch, 0, "f32", *small)
+        side.synchronize()
+        with pytest.raises(ValueError):  # a replay may find more rows than this
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                c.ctx.paged_read(c.batch, 0, "f32", *small)
+        with torch.cuda.graph(graph, stream=side):
+            k, v = c.ctx.paged_read(c.batch, 0, "f32", *large)
+            own = c.ctx.paged_read(c.batch, 0, "f32")
+        assert own[0].shape == own[1].shape == (most, 128)
+        c.batch.set([1, 1], [20, 40], c.table)
+        graph.replay()
+        side.synchronize()
+        for i, got in enumerate((k, v)):
+            want = torch.cat([r[i] for r in c.rows]).view(60, 128)
+            assert torch.equal(got[:60].double(), want) and not bool(got[60:].any()) and torch.equal(own[i][:60], got[:60])
