@@ -60,42 +60,113 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// One row again, key by key in f32, by a warp: what is not seen is not touched. Only rows whose fast result is not finite.
-template <int D, bool F32>
+// N consecutive elements of a row of keys or values, from element `at` on, in f32 (codes of 8-bit pages: without their scale).
+template <int N, int FMT>
+__device__ __forceinline__ void paged_elems(const void* rows, int64_t at, float (&x)[N]) {
+    if constexpr (FMT == kKvQ8Head) {
+        uint32_t u[(N + 3) / 4];
+        const unsigned char* p = static_cast<const unsigned char*>(rows) + at;
+        if constexpr (N == 8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(p);
+            u[0] = w.x, u[1] = w.y;
+        } else if constexpr (N == 4) {
+            u[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            u[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = (float)(int)(signed char)(u[i >> 2] >> (8 * (i & 3)));
+    } else if constexpr (FMT == KV_F32) {
+        const float* p = static_cast<const float*>(rows) + at;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 u = *reinterpret_cast<const float2*>(p + i);
+            x[i] = u.x, x[i + 1] = u.y;
+        }
+    } else {
+        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(rows) + at;
+        if constexpr (N == 8) {
+            unpack8(*reinterpret_cast<const uint4*>(p), x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const uint32_t u = *reinterpret_cast<const uint32_t*>(p + i);
+                x[i] = __uint_as_float(u << 16), x[i + 1] = __uint_as_float(u & 0xffff0000u);
+            }
+        }
+    }
+}
+
+// One row again in f32, by a warp: what is not seen is not touched. Only rows whose fast result is not finite, and not known to be
+// right as it is (a bf16 row's sum of weights is NaN when one of its scores is, whatever the values are). 32 keys at a time: a lane
+// takes q times one of them, then every lane D / 32 elements of their values. A row that has met a NaN score is NaN, and is left
+// there; of 8-bit pages the scales tell before anything else is read.
+template <int D, int FMT, bool F32>
 __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const PagedItem& w, int kvh, int r, int lane) {
     constexpr int E = D / 32;
-    const int tok = r / a.G, h = kvh * a.G + r % a.G, pos = w.pos0 + tok;
-    const int64_t qo = (w.tok0 + tok) * a.q_stride + (int64_t)h * D;
+    const int tok = r / a.G, h = kvh * a.G + r % a.G, pos = w.pos0 + tok, first = paged_first_key(pos, a.window);
+    const int64_t qo = (w.tok0 + tok) * a.q_stride + (int64_t)h * D + lane * E;
+    constexpr bool q8 = FMT == kKvQ8Head;
     float q[E], o[E], m = -INFINITY, l = 0.0f;
+#pragma unroll
     for (int i = 0; i < E; ++i) {
-        q[i] = F32 ? static_cast<const float*>(a.q)[qo + lane + 32 * i] : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qo + lane + 32 * i]);
+        q[i] = F32 ? static_cast<const float*>(a.q)[qo + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qo + i]);
         o[i] = 0.0f;
     }
-    auto at = [&](const void* packed, int64_t stride, const unsigned char* pool, const float* scales, int j, int d) -> float {
-        if (!a.paged) {
-            const int64_t i = (int64_t)(w.src + j) * stride + (int64_t)kvh * D + d;
-            return F32 ? static_cast<const float*>(packed)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(packed)[i]);
-        }
-        const int64_t row = a.pages.row(a.layer, a.plan.table[w.src + (j >> a.pages.page_log2)], kvh, j & ((1 << a.pages.page_log2) - 1));
-        if (a.pages.fmt == KV_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(pool)[row * D + d]);
-        return (float)reinterpret_cast<const signed char*>(pool)[row * D + d] * scales[row];
+    auto row_of = [&](int j) -> int64_t {
+        if (!a.paged) return w.src + j;
+        return a.pages.row(a.layer, a.plan.table[w.src + (j >> a.pages.page_log2)], kvh, j & ((1 << a.pages.page_log2) - 1));
     };
-    for (int j = paged_first_key(pos, a.window); j <= pos; ++j) {
-        float s = 0.0f;
-        for (int i = 0; i < E; ++i) s = fmaf(q[i], at(a.pk, a.pk_stride, a.pages.k, a.pages.ks, j, lane + 32 * i), s);
-        s = warp_sum(s) * a.c;
-        // (a score of -inf has weight 0, also while there is no larger one to measure it by)
-        const float top = fmaxf(m, s), f = m == top ? 1.0f : exp2f(m - top), p = s == -INFINITY ? 0.0f : exp2f(s - top);
-        m = top;
-        l = l * f + p;
-        for (int i = 0; i < E; ++i) o[i] = o[i] * f + p * at(a.pv, a.pv_stride, a.pages.v, a.pages.vs, j, lane + 32 * i);
+    if constexpr (q8) {
+        bool odd = false;
+#pragma unroll 4
+        for (int j = first + lane; j <= pos; j += 32) {
+            const int64_t row = row_of(j);
+            odd |= isnan(a.pages.ks[row]) | isnan(a.pages.vs[row]);
+        }
+        if (__any_sync(0xffffffffu, odd)) l = NAN;
     }
-    const int64_t oo = (w.tok0 + tok) * a.o_stride + (int64_t)h * D;
+    const void* keys = a.paged ? static_cast<const void*>(a.pages.k) : a.pk;
+    const void* vals = a.paged ? static_cast<const void*>(a.pages.v) : a.pv;
+    const int64_t k_step = a.paged ? D : a.pk_stride, v_step = a.paged ? D : a.pv_stride, head = a.paged ? 0 : (int64_t)kvh * D;
+    for (int j0 = first; j0 <= pos && l == l; j0 += 32) {
+        const int n = min(32, pos + 1 - j0);
+        const int64_t row = row_of(j0 + min(lane, n - 1));
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int d = 0; d < D; d += 8) {
+            float x[8];
+            paged_elems<8, FMT>(keys, row * k_step + head + d, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[e & 3] = fmaf(__shfl_sync(0xffffffffu, q[e % E], (d + e) / E), x[e], part[e & 3]);
+        }
+        float s = ((part[0] + part[1]) + (part[2] + part[3])) * a.c;
+        if constexpr (q8) s *= a.pages.ks[row];
+        if (lane >= n) s = -INFINITY;
+        // (a score of -inf has weight 0, also while there is no larger one to measure it by)
+        const float top = fmaxf(m, warp_max(s)), f = m == top ? 1.0f : exp2f(m - top);
+        float p = s == -INFINITY ? 0.0f : exp2f(s - top);
+        m = top;
+        l = l * f + warp_sum(p);
+        if constexpr (q8) p *= a.pages.vs[row];
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] *= f;
+#pragma unroll 16
+        for (int i = 0; i < n; ++i) {
+            const float pi = __shfl_sync(0xffffffffu, p, i);
+            float x[E];
+            paged_elems<E, FMT>(vals, __shfl_sync(0xffffffffu, row, i) * v_step + head + lane * E, x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(pi, x[e], o[e]);
+        }
+    }
+    const int64_t oo = (w.tok0 + tok) * a.o_stride + (int64_t)h * D + lane * E;
+#pragma unroll
     for (int i = 0; i < E; ++i) {
         if (F32)
-            static_cast<float*>(a.out)[oo + lane + 32 * i] = o[i] / l;
+            static_cast<float*>(a.out)[oo + i] = o[i] / l;
         else
-            static_cast<__nv_bfloat16*>(a.out)[oo + lane + 32 * i] = __float2bfloat16_rn(o[i] / l);
+            static_cast<__nv_bfloat16*>(a.out)[oo + i] = __float2bfloat16_rn(o[i] / l);
     }
 }
 
@@ -629,7 +700,8 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     __shared__ float s_m[W][R], s_l[W][R];  // per warp, then weights of the warps
     __shared__ float s_top[R], s_sum[R];
     __shared__ float s_w[R][kPagedSplitMax];
-    __shared__ int s_abort, s_last, s_bad;
+    __shared__ int s_abort, s_last;
+    __shared__ unsigned s_bad;  // rows of the tile that have to be computed again
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.x;
@@ -790,7 +862,7 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 const int row = w.row0 + r, tok = row / a.G;
                 const float inv = 1.0f / s_sum[r];
                 v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                if (!finite4(v)) s_bad = 1;
+                if (!finite4(v) && (F32 || s_sum[r] == s_sum[r])) atomicOr(&s_bad, 1u << r);
                 paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D + d, v);
             }
         }
@@ -837,14 +909,15 @@ paged_splitk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     const int row = w.row0 + r, tok = row / a.G;
                     const float inv = 1.0f / s_sum[r];
                     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                    if (!finite4(v)) s_bad = 1;
+                    if (!finite4(v) && (F32 || s_sum[r] == s_sum[r])) atomicOr(&s_bad, 1u << r);
                     paged_store4<F32>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D + d, v);
                 }
             }
         }
         __syncthreads();
         if (s_bad) {
-            for (int r = warp; r < w.rows; r += W) paged_row_again<D, F32>(a, w, kvh, w.row0 + r, lane);
+            for (int r = warp; r < w.rows; r += W)
+                if (s_bad >> r & 1u) paged_row_again<D, FMT, F32>(a, w, kvh, w.row0 + r, lane);
             __syncthreads();
         }
         // the next item's copies go where the generic proxy has just written
@@ -986,15 +1059,17 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             if (!mine) continue;
             x.sum_rows();
             const float i0 = 1.0f / x.l0, i1 = 1.0f / x.l1;
-            bool bad = false;
+            unsigned again = 0;  // of the warp's 16 rows
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
+                bool bad = false;
                 const int row = r0 + gq + 8 * half, tok = row / a.G;
-                if (row >= r1) continue;
+                const float sum = half ? x.l1 : x.l0;
                 const int64_t at = (w.tok0 + tok) * a.o_stride + (int64_t)(kvh * a.G + row - tok * a.G) * D;
                 const float inv = half ? i1 : i0;
 #pragma unroll
                 for (int nt = 0; nt < M::NT; ++nt) {
+                    if (row >= r1) break;
                     if constexpr (FMT == kKvQ8Head) {
                         if (nt & 1) continue;
                         const float4 v = make_float4(x.o[nt][2 * half] * inv, x.o[nt + 1][2 * half] * inv, x.o[nt][2 * half + 1] * inv, x.o[nt + 1][2 * half + 1] * inv);
@@ -1010,11 +1085,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                             *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + to) = pack_bf16x2(v0, v1);
                     }
                 }
+                const unsigned lanes = __ballot_sync(0xffffffffu, bad && (F32 || sum == sum));  // four to a row
+#pragma unroll
+                for (int r = 0; r < 8; ++r) again |= (lanes >> (4 * r) & 15u ? 1u : 0u) << (8 * half + r);
             }
-            if (__any_sync(0xffffffffu, bad)) {
-                __syncwarp();
-                for (int r = r0; r < min(r0 + 16, r1); ++r) paged_row_again<D, F32>(a, w, kvh, r, lane);
-            }
+            __syncwarp();
+            for (int r = 0; again >> r; ++r)
+                if (again >> r & 1u) paged_row_again<D, FMT, F32>(a, w, kvh, r0 + r, lane);
         }
     }
     if (s_abort) {

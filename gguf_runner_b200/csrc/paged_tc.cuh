@@ -523,12 +523,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 fence_before_sync();
             }
             mbar_arrive(o_free(t));
-            unsigned again = __ballot_sync(0xffffffffu, bad && valid);
+            unsigned again = __ballot_sync(0xffffffffu, bad && valid && (HALF || l == l));
             while (again) {
                 const int rr = __ffs(again) - 1;
                 again &= again - 1;
                 const int tk = __shfl_sync(0xffffffffu, tok, rr), hd = __shfl_sync(0xffffffffu, head, rr);
-                paged_row_again<D, false>(a, w, w.kvh, tk * a.G + hd, lane);
+                paged_row_again<D, HALF ? kKvQ8Head : KV_BF16, false>(a, w, w.kvh, tk * a.G + hd, lane);
             }
         }
     }
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_consta
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             o[v] = make_float4(o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
-            bad |= valid && !finite4(o[v]);
+            bad |= valid && !finite4(o[v]) && (p.out_scale != 1.0f || l == l);
             if (valid) paged_store4<false>(a, (w.tok0 + tok) * a.o_stride + (int64_t)(w.kvh * a.G + head) * D + (v * L + sub) * 4, o[v]);
         }
         unsigned again = __ballot_sync(0xffffffffu, bad);
@@ -622,7 +622,11 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const __grid_consta
             const int from = __ffs(again) - 1;
             again &= ~((L == 32 ? 0xffffffffu : ((1u << L) - 1)) << (from & ~(L - 1)));
             __syncwarp();
-            paged_row_again<D, false>(a, w, w.kvh, __shfl_sync(0xffffffffu, tok * a.G + head, from), lane);
+            const int row = __shfl_sync(0xffffffffu, tok * a.G + head, from);
+            if (p.out_scale != 1.0f)  // f16 rows: 8-bit pages
+                paged_row_again<D, kKvQ8Head, false>(a, w, w.kvh, row, lane);
+            else
+                paged_row_again<D, KV_BF16, false>(a, w, w.kvh, row, lane);
         }
     }
 }

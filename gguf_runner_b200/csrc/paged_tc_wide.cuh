@@ -374,11 +374,11 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 bulk_store_commit_and_wait();
             }
             __syncwarp();
-            unsigned again = __ballot_sync(0xffffffffu, bad && valid);
+            unsigned again = __ballot_sync(0xffffffffu, bad && valid && (HALF || l == l));
             while (again) {
                 const int rr = __ffs(again) - 1;
                 again &= again - 1;
-                paged_row_again<D, false>(a, w, w.kvh, w.row0 * a.G + warp * 32 + rr, lane);
+                paged_row_again<D, HALF ? kKvQ8Head : KV_BF16, false>(a, w, w.kvh, w.row0 * a.G + warp * 32 + rr, lane);
             }
         }
     }

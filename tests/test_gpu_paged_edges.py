@@ -190,3 +190,52 @@ def test_a_captured_read_has_room_for_the_longest_step():
         for i, got in enumerate((k, v)):
             want = torch.cat([r[i] for r in c.rows]).view(60, 128)
             assert torch.equal(got[:60].double(), want) and not bool(got[60:].any()) and torch.equal(own[i][:60], got[:60])
+
+
+def device_time(call, n=3):
+    """Milliseconds of a call on the device."""
+    call()
+    start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    for _ in range(n):
+        call()
+    stop.record()
+    stop.synchronize()
+    return start.elapsed_time(stop) / n
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv", ["bf16", "q8_head"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_value_that_is_not_finite_in_cut_rows(d, kv, dtype):
+    """Chunks and a single token over long texts, cut along their keys: a later token's value shows in the rows that see it, in the
+    elements that it spoils, and nowhere else."""
+    q_len, kv_len, at = [70, 1, 33], [7000, 9000, 3001], [6950, 8999, 2990]
+    c = Case(8, 2, d, kv, dtype, 64, q_len, kv_len, seed=42)
+    for b, p in enumerate(at):
+        page, row = c.table[b][p // 64], p % 64
+        if kv == "bf16":
+            c.pool[1][0, page, 1, row, 3] = math.nan
+        else:
+            c.scales[1][0, page, 1, row] = math.nan
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(-1, 8, d)
+    out, size, reach = (x.view(-1, 8, d) for x in c.want())
+    ok = (got.double() - out).abs() <= ref.bound(c.dtype, out, size, reach)
+    pos = torch.cat([torch.arange(k - n, k) for n, k in zip(q_len, kv_len)]).cuda()
+    seen = pos >= torch.cat([torch.full((n,), p) for n, p in zip(q_len, at)]).cuda()
+    spoilt = torch.zeros_like(ok)
+    spoilt[seen, 4:, 3 if kv == "bf16" else slice(None)] = True
+    assert bool(ok[~spoilt].all()) and bool(got[spoilt].isnan().all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_values_in_long_texts(d):
+    """Values that the f16 operands of 8-bit chunks cannot hold: the rows that see them are right, and the call ends in its time."""
+    c = Case(8, 2, d, "q8_head", "bf16", 64, [150], [12000], seed=43)
+    usual = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
+    c.scales[1][0, c.table[0][2], 1, 5] *= 2000.0
+    c.rows[0][1][133, 1] *= 2000.0
+    c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+    took = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
+    # (one key after the other, a single row took 14 to 52 ms)
+    assert took < 12.0, (took, usual)
