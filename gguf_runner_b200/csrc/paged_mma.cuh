@@ -60,6 +60,28 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// Bounded waits (see mbar_wait) of kernels in which other warps of the CTA may meanwhile compute rows again, which takes as long as
+// the row's keys are many: flags[0] is raised by whoever gives up, flags[1] counts paged_row_again's steps, some microseconds each,
+// and the limit starts anew as long as it moves. (By the limit alone a CTA would give up its items while a warp has 32 rows of 150000 keys, at 0.25 us a row and key.)
+__device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int* flags) {
+    if (tc::mbar_test(bar, parity)) return true;
+    int seen = 0;
+    for (uint32_t it = 0; it < kTcSpinLimit; ++it) {
+        if (tc::mbar_try(bar, parity, 4000u)) return true;
+        if ((it & 15u) == 15u) {
+            if (flags[0]) return false;
+            const int now = flags[1];
+            if (now != seen) seen = now, it = 0;
+        }
+    }
+    flags[0] = 1;
+    return false;
+}
+__device__ __forceinline__ bool paged_wait_warp(uint32_t bar, uint32_t parity, volatile int* flags) {
+    const bool ok = paged_wait(bar, parity, flags);
+    return __all_sync(0xffffffffu, ok);
+}
+
 // N consecutive elements of a row of keys or values, from element `at` on, in f32 (codes of 8-bit pages: without their scale).
 template <int N, int FMT>
 __device__ __forceinline__ void paged_elems(const void* rows, int64_t at, float (&x)[N]) {
@@ -100,9 +122,9 @@ __device__ __forceinline__ void paged_elems(const void* rows, int64_t at, float 
 // One row again in f32, by a warp: what is not seen is not touched. Only rows whose fast result is not finite, and not known to be
 // right as it is (a bf16 row's sum of weights is NaN when one of its scores is, whatever the values are). 32 keys at a time: a lane
 // takes q times one of them, then every lane D / 32 elements of their values. A row that has met a NaN score is NaN, and is left
-// there; of 8-bit pages the scales tell before anything else is read.
+// there; of 8-bit pages the scales tell before anything else is read. `steps`: in shared memory, see paged_wait.
 template <int D, int FMT, bool F32>
-__device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const PagedItem& w, int kvh, int r, int lane) {
+__device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const PagedItem& w, int kvh, int r, int lane, int* steps = nullptr) {
     constexpr int E = D / 32;
     const int tok = r / a.G, h = kvh * a.G + r % a.G, pos = w.pos0 + tok, first = paged_first_key(pos, a.window);
     const int64_t qo = (w.tok0 + tok) * a.q_stride + (int64_t)h * D + lane * E;
@@ -119,10 +141,13 @@ __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const Paged
     };
     if constexpr (q8) {
         bool odd = false;
+        for (int j0 = first; j0 <= pos; j0 += 1024) {
+            if (steps && lane == 0) atomicAdd(steps, 1);
 #pragma unroll 4
-        for (int j = first + lane; j <= pos; j += 32) {
-            const int64_t row = row_of(j);
-            odd |= isnan(a.pages.ks[row]) | isnan(a.pages.vs[row]);
+            for (int j = j0 + lane; j <= min(pos, j0 + 1023); j += 32) {
+                const int64_t row = row_of(j);
+                odd |= isnan(a.pages.ks[row]) | isnan(a.pages.vs[row]);
+            }
         }
         if (__any_sync(0xffffffffu, odd)) l = NAN;
     }
@@ -130,6 +155,7 @@ __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const Paged
     const void* vals = a.paged ? static_cast<const void*>(a.pages.v) : a.pv;
     const int64_t k_step = a.paged ? D : a.pk_stride, v_step = a.paged ? D : a.pv_stride, head = a.paged ? 0 : (int64_t)kvh * D;
     for (int j0 = first; j0 <= pos && l == l; j0 += 32) {
+        if (steps && lane == 0) atomicAdd(steps, 1);
         const int n = min(32, pos + 1 - j0);
         const int64_t row = row_of(j0 + min(lane, n - 1));
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -952,14 +978,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     constexpr int NST = S::NST, SUB = S::SUB, KT = 16 * SUB;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t s_full[NST], s_empty[NST], s_raw;
-    __shared__ int s_abort;
+    __shared__ int s_flags[2];  // of paged_wait
+    int& s_abort = s_flags[0];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int gq = lane >> 2, tq = lane & 3, kvh = blockIdx.x;
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     unsigned char* base_p = smem + (base - smem_u32(smem));
-    volatile int* abortp = &s_abort;
+    volatile int* abortp = s_flags;
     if (tid == 0) {
-        s_abort = 0;
+        s_flags[0] = s_flags[1] = 0;
         for (int s = 0; s < NST; ++s) {
             mbar_init(smem_u32(&s_full[s]), 1);
             mbar_init(smem_u32(&s_empty[s]), S::W);
@@ -985,7 +1012,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const int n_stages = (w.key1 - w.key0 + KT - 1) / KT, any_lo = any_lo_of(w), any_hi = any_hi_of(w);
             for (int t = 0; t < n_stages; ++t, ++used) {
                 const uint32_t stage = used % NST;
-                if (!(ok = mbar_wait_warp(smem_u32(&s_empty[stage]), ((used / NST) & 1u) ^ 1u, abortp))) break;
+                if (!(ok = paged_wait_warp(smem_u32(&s_empty[stage]), ((used / NST) & 1u) ^ 1u, abortp))) break;
                 const int key = w.key0 + t * KT;
                 const bool edge = key < any_lo || key + KT > any_hi;
                 const uint32_t bar = edge ? smem_u32(&s_raw) : smem_u32(&s_full[stage]);
@@ -1007,7 +1034,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 }
                 __syncwarp();
                 if (edge) {
-                    if (!(ok = mbar_wait_warp(bar, raws & 1u, abortp))) break;
+                    if (!(ok = paged_wait_warp(bar, raws & 1u, abortp))) break;
                     ++raws;
                     for (int i = 0; i < SUB; ++i) M::clear(dst + i * M::TILE, any_lo - key - 16 * i, any_hi - key - 16 * i, lane);
                     fence_smem_to_async_proxy();  // (this stage's next copy comes after the arrivals below and the readers')
@@ -1040,7 +1067,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const int lo0 = paged_first_key(p0, a.window), lo1 = paged_first_key(p1, a.window);
             for (int t = 0; t < n_stages; ++t, ++used) {
                 const uint32_t stage = used % NST;
-                if (!mbar_wait_warp(smem_u32(&s_full[stage]), (used / NST) & 1u, abortp)) break;
+                if (!paged_wait_warp(smem_u32(&s_full[stage]), (used / NST) & 1u, abortp)) break;
 #pragma unroll 1
                 for (int i = 0; i < SUB; ++i) {
                     const int key = w.key0 + t * KT + 16 * i;
@@ -1091,7 +1118,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
             __syncwarp();
             for (int r = 0; again >> r; ++r)
-                if (again >> r & 1u) paged_row_again<D, FMT, F32>(a, w, kvh, r0 + r, lane);
+                if (again >> r & 1u) paged_row_again<D, FMT, F32>(a, w, kvh, r0 + r, lane, &s_flags[1]);
         }
     }
     if (s_abort) {

@@ -95,7 +95,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bars[25];
     __shared__ uint32_t s_tmem_base;
-    __shared__ int s_abort;
+    __shared__ int s_flags[2];  // of paged_wait
+    int& s_abort = s_flags[0];
     __shared__ __align__(16) PagedItem s_item[2];
     __shared__ int s_live[2];
 
@@ -118,7 +119,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     auto item_empty = [&](int s) { return bar0 + 8u * (22 + s); };
 
     if (tid == 0) {
-        s_abort = 0;
+        s_flags[0] = s_flags[1] = 0;
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(raw, 1);
@@ -145,7 +146,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = s_tmem_base;
-    volatile int* abortp = &s_abort;
+    volatile int* abortp = s_flags;
     volatile int* livep = s_live;
     if (!p.behind) grid_wait();
 
@@ -163,7 +164,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             uint32_t raws = 0;
             for (int it = 0;; ++it) {
                 const int slot = it & 1;
-                if (!mbar_wait_warp(item_empty(slot), ((it >> 1) & 1) ^ 1, abortp)) break;
+                if (!paged_wait_warp(item_empty(slot), ((it >> 1) & 1) ^ 1, abortp)) break;
                 int r = 0;
                 if (lane == 0) r = it == 0 ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.sched, 1);
                 r = __shfl_sync(0xffffffffu, r, 0);
@@ -177,7 +178,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const PagedItem w = s_item[slot];
                 const PtRange rg = pt_range(p, w);
                 const bool act0 = rg.hi0 > rg.lo0, act1 = rg.hi1 > rg.lo1;
-                if (!mbar_wait_warp(q_empty, (it & 1) ^ 1, abortp)) break;
+                if (!paged_wait_warp(q_empty, (it & 1) ^ 1, abortp)) break;
                 if (lane == 0) {
                     mbar_expect_tx(q_full, ((act0 ? 1 : 0) + (act1 ? 1 : 0)) * q_bytes);
                     for (int t = 0; t < 2; ++t) {
@@ -203,18 +204,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const int y = p.linear ? w.kvh : key & ((1 << page_log2) - 1);
                     const int z = p.linear ? w.lin + key : (a.layer * a.pages.n_pages + page) * a.pages.Hkv + w.kvh;
                     page = page_of(j + 1);
-                    if (!(ok = mbar_wait_warp(k_empty(s), ph, abortp))) break;
+                    if (!(ok = paged_wait_warp(k_empty(s), ph, abortp))) break;
                     if (lane == 0) mbar_expect_tx(k_full(s), bytes);
                     __syncwarp();
                     if (mine) tma_load_3d(sK + s * TILE + box_at, &tmK, blk * 64, y, z, k_full(s));
-                    if (!(ok = mbar_wait_warp(v_empty(s), ph, abortp))) break;
+                    if (!(ok = paged_wait_warp(v_empty(s), ph, abortp))) break;
                     const bool edge = j * 128 < any_lo || (j + 1) * 128 > any_hi;
                     const uint32_t vbar = edge ? raw : v_full(s);
                     if (lane == 0) mbar_expect_tx(vbar, bytes);
                     __syncwarp();
                     if (mine) tma_load_3d(sV + s * TILE + box_at, &tmV, blk * 64, y, z, vbar);
                     if (edge) {
-                        if (!(ok = mbar_wait_warp(raw, raws & 1u, abortp))) break;
+                        if (!(ok = paged_wait_warp(raw, raws & 1u, abortp))) break;
                         ++raws;
                         for (int i = lane; i < 128 * NBLK * 8; i += 32) {
                             const int row = (i >> 3) & 127, k = j * 128 + row;
@@ -255,7 +256,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             bool ok = true;
             for (int it = 0; ok; ++it) {
                 const int slot = it & 1;
-                if (!(ok = mbar_wait_warp(item_full(slot), (it >> 1) & 1, abortp))) break;
+                if (!(ok = paged_wait_warp(item_full(slot), (it >> 1) & 1, abortp))) break;
                 const int live = __shfl_sync(0xffffffffu, livep[slot], 0);
                 PtRange w = pt_range(p, s_item[slot]);
                 w.lo0 = __shfl_sync(0xffffffffu, w.lo0, 0);
@@ -271,16 +272,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
                     if (w.hi_of(t) <= w.lo_of(t)) {
-                        if (!(ok = mbar_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
+                        if (!(ok = paged_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
                         if (lane == 0) mbar_arrive(o_final(t));
                     }
                 if (!ok) break;
-                if (!(ok = mbar_wait_warp(q_full, it & 1, abortp))) break;
+                if (!(ok = paged_wait_warp(q_full, it & 1, abortp))) break;
                 if (hi == lo) {
                     mma_commit_e(q_empty);
                     continue;
                 }
-                if (!(ok = mbar_wait_warp(k_full(g & 1), (g >> 1) & 1, abortp))) break;
+                if (!(ok = paged_wait_warp(k_full(g & 1), (g >> 1) & 1, abortp))) break;
                 fence_after_sync();
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -293,25 +294,25 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 for (int j = lo; j < hi; ++j, ++g) {
                     const int s = g & 1;
                     const bool has_next = j + 1 < hi;
-                    if (!(ok = mbar_wait_warp(v_full(s), (g >> 1) & 1, abortp))) break;
+                    if (!(ok = paged_wait_warp(v_full(s), (g >> 1) & 1, abortp))) break;
                     bool next_k_ready = false;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int lo_t = w.lo_of(t), hi_t = w.hi_of(t), c_t = t ? c1 : c0;
                         if (j >= lo_t && j < hi_t) {
                             const uint32_t ph = (c_t + j - lo_t) & 1;
-                            if (!(ok = mbar_wait_warp(p_half(t, 0), ph, abortp))) break;
-                            if (j == lo_t && !(ok = mbar_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
+                            if (!(ok = paged_wait_warp(p_half(t, 0), ph, abortp))) break;
+                            if (j == lo_t && !(ok = paged_wait_warp(o_free(t), (it & 1) ^ 1, abortp))) break;
                             fence_after_sync();
                             issue_pv_half(t, s, 0, j > lo_t);
-                            if (!(ok = mbar_wait_warp(p_half(t, 1), ph, abortp))) break;
+                            if (!(ok = paged_wait_warp(p_half(t, 1), ph, abortp))) break;
                             fence_after_sync();
                             issue_pv_half(t, s, 1, true);
                             if (j == hi_t - 1) mma_commit_e(o_final(t));
                         }
                         if (has_next && j + 1 >= lo_t && j + 1 < hi_t) {
                             if (!next_k_ready) {
-                                if (!(ok = mbar_wait_warp(k_full(s ^ 1), ((g + 1) >> 1) & 1, abortp))) break;
+                                if (!(ok = paged_wait_warp(k_full(s ^ 1), ((g + 1) >> 1) & 1, abortp))) break;
                                 fence_after_sync();
                                 next_k_ready = true;
                             }
@@ -342,7 +343,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         int cs = 0;
         for (int it = 0; ok; ++it) {
             const int slot = it & 1;
-            if (!(ok = mbar_wait(item_full(slot), (it >> 1) & 1, abortp))) break;
+            if (!(ok = paged_wait(item_full(slot), (it >> 1) & 1, abortp))) break;
             const int live = livep[slot];
             const PagedItem w = s_item[slot];
             __syncwarp();
@@ -363,7 +364,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             float m_used = -INFINITY, l = 0.0f;
             for (int j = lo_t; j < hi_t; ++j) {
                 const int k = j - lo_t;
-                if (!(ok = mbar_wait(s_full(t), (cs + k) & 1, abortp))) break;
+                if (!(ok = paged_wait(s_full(t), (cs + k) & 1, abortp))) break;
                 fence_after_sync();
                 uint32_t sr[4][32];
 #pragma unroll
@@ -463,7 +464,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             }
             if (!ok) break;
             cs += n_t;
-            if (!(ok = mbar_wait(o_final(t), it & 1, abortp))) break;
+            if (!(ok = paged_wait(o_final(t), it & 1, abortp))) break;
             fence_after_sync();
             if (m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
             const bool split = w.part >= 0;
@@ -528,7 +529,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const int rr = __ffs(again) - 1;
                 again &= again - 1;
                 const int tk = __shfl_sync(0xffffffffu, tok, rr), hd = __shfl_sync(0xffffffffu, head, rr);
-                paged_row_again<D, HALF ? kKvQ8Head : KV_BF16, false>(a, w, w.kvh, tk * a.G + hd, lane);
+                paged_row_again<D, HALF ? kKvQ8Head : KV_BF16, false>(a, w, w.kvh, tk * a.G + hd, lane, &s_flags[1]);
             }
         }
     }

@@ -239,3 +239,33 @@ def test_large_values_in_long_texts(d):
     took = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
     # (one key after the other, a single row took 14 to 52 ms)
     assert took < 12.0, (took, usual)
+
+
+def test_waits_outlast_rows_that_are_computed_again():
+    """A chunk behind 300000 8-bit keys with one value beyond f16, in front of a long prompt: its rows take longer than any wait of
+    their CTA is allowed to, and neither they nor the prompt's rows, whose items come behind them, are lost."""
+    heads, d, page, q_len, kv_len = 8, 64, 256, [300, 38144], [300000, 38144]
+    ctx = context(heads, heads, d)
+    used = [-(-n // page) for n in kv_len]
+    gen = torch.Generator(device="cuda").manual_seed(44)
+    pool = [torch.randint(-127, 128, (1, sum(used), heads, page, d), generator=gen, device="cuda", dtype=torch.int8) for _ in range(2)]
+    scales = [torch.full((1, sum(used), heads, page), 1 / 64, device="cuda") for _ in range(2)]
+    scales[1][0, 0, 1, 7] = 20.0
+    pages = g.Pages(ctx, sum(used), page, "q8_head", *pool, *scales)
+    batch = g.Batch(ctx, pages, "bf16", 2, sum(q_len), sum(used))
+    batch.set(q_len, kv_len, [list(range(used[0])), list(range(used[0], sum(used)))])
+    q = torch.randn(sum(q_len), heads * d, generator=gen, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    ctx.paged_attention(batch, 0, q, out=out)
+    took = device_time(lambda: ctx.paged_attention(batch, 0, q, out=out), 1)
+    for b, toks in ((0, (0, 100, 299)), (1, (0, 255, 256, 20000, 38143))):
+        of = slice(0, used[0]) if b == 0 else slice(used[0], None)
+        for h in (0, 1, 7):
+            k, v = (pool[i][0, of, h].reshape(-1, 1, d).double() * scales[i][0, of, h].reshape(-1, 1, 1).double() for i in range(2))
+            for t in toks:
+                n, row = kv_len[b] - q_len[b] + t + 1, t + b * q_len[0]
+                want, size, reach = ref.attention(q[row].view(1, heads, d)[:, h:h + 1], k[:n], v[:n], n - 1, 0, 1 / math.sqrt(d))
+                got = out[row].view(heads, d)[h].double()
+                assert bool(((got - want[0, 0]).abs() <= ref.bound(torch.bfloat16, want, size, reach)[0, 0]).all()), (b, h, t)
+    assert bool(torch.isfinite(out).all()) and not bool((out.view(-1, heads, d) == 7.0).all(-1).any())
+    assert took > 1000.0, took  # (long enough to show it)
