@@ -823,10 +823,10 @@ class AttnContext:
         captured call may find a longer plan: its tensors have the rows of all pages that the plan may name.)"""
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
-        dt, c, n, most = _torch_dtype(dtype), self.config, batch.n_rows, batch.max_rows
+        dt, c, n, most = _torch_dtype(dtype), self.config, batch.n_rows, batch.max_rows if _capturing() else 0
         if k_out is None or v_out is None:
             import torch
-            k_out, v_out = (torch.empty((most if _capturing() else n, c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
+            k_out, v_out = (torch.empty((max(n, most), c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
         kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim, most)
         vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim, most)
         self._follow_torch_stream_of_device()
