@@ -270,7 +270,9 @@ struct PagedMma {
                     for (int half = 0; half < 2; ++half) top[i] = fmaxf(top[i], fmaxf(fabsf(held[ks][i][half].x), fabsf(held[ks][i][half].y)));
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                by[i] = __uint_as_float(0x7f000000u - (min(max(__float_as_uint(top[i]), 0x00800000u), 0x7e800000u) & 0x7f800000u));
+                // (not below 2^-100, zeros included: the threshold in units of a smaller row's scores would be infinite, its maximum
+                // would never move from -inf, and the merges would take it for a row that has seen nothing)
+                by[i] = __uint_as_float(0x7f000000u - (min(max(__float_as_uint(top[i]), 0x0d800000u), 0x7e800000u) & 0x7f800000u));
             }
         }
         q0 = 1.0f / by[0];

@@ -269,3 +269,16 @@ def test_waits_outlast_rows_that_are_computed_again():
                 assert bool(((got - want[0, 0]).abs() <= ref.bound(torch.bfloat16, want, size, reach)[0, 0]).all()), (b, h, t)
     assert bool(torch.isfinite(out).all()) and not bool((out.view(-1, heads, d) == 7.0).all(-1).any())
     assert took > 1000.0, took  # (long enough to show it)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_of_zeros_over_8_bit_pages(d, dtype):
+    """Rows of q that are zero or next to it, uncut and cut: every key counts the same, and they cost what others cost."""
+    c = Case(8, 2, d, "q8_head", dtype, 16, [3, 1, 2], [40, 12000, 7], seed=34)
+    usual = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
+    rows = c.q.view(6, 8, d)
+    rows[0], rows[3, :3], rows[1, 2], rows[5, 7], rows[3, 5] = 0.0, 0.0, 1e-38, 1e-30, 1e-37
+    c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+    took = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
+    assert took < 5 * usual, (took, usual)  # (one row again, key by key, would take hundreds of times as long)
