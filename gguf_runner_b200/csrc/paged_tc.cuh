@@ -10,9 +10,10 @@
 //  - Items (two query tiles and a stretch of keys) are cut on the host, longest first, and handed out through a counter. Pieces
 //    of a pair of tiles leave un-normalised rows, which paged_tc_merge_kernel weighs in the order of the keys.
 //  - 8-bit pages are read into dense f16 rows first (paged_read_kernel, 34 us of 602 for 2048 tokens behind 14336, 40/8 heads
-//    of 128), q into f16 beside them: eleven bits leave code * scale 2^-12 off, an eighth of what bf16 weights are. bf16 rows would
-//    add two roundings as large as that of the weights (by their variances 3.2e-3 instead of 2.3e-3 from 64 bits), and scales that
-//    the softmax warps multiply into scores and weights are two multiplications and half a shared-memory load per score.
+//    of 128), q into f16 beside them: eleven bits leave code * scale 2^-12 off, an eighth of what bf16 weights are (weights: see
+//    kPtHalfShift). bf16 rows would add two roundings as large as that of the weights (by their variances 3.2e-3 instead of 2.3e-3
+//    from 64 bits), and scales that the softmax warps multiply into scores and weights are two multiplications and half a
+//    shared-memory load per score.
 // Values that nobody in the item sees (behind the sequence's end, before its window) may be anything, and 0 * NaN is NaN: the
 // producer clears them in the first and last tile, before the MMA issuer hears of the tile. Rows that come out not finite are
 // computed again by paged_row_again.
@@ -76,6 +77,10 @@ __device__ __forceinline__ PtRange pt_range(const PagedTcArgs& p, const PagedIte
     return r;
 }
 
+// f16 weights are taken times 2^7, and so is their sum: a weight is at most 2^8 (the lazy reference maximum) and stays in range, and
+// what is 2^-21 of the reference (2^-14 without) still has all eleven bits, 2^-31 a value at all. Thousands of keys at 2^-26 of the
+// largest weight would else drop out of the result while the sum keeps them.
+constexpr float kPtHalfShift = 7.0f;
 template <bool HALF>
 __device__ __forceinline__ uint32_t pt_pack(float x, float y) {
     if constexpr (!HALF) return pack_bf16x2(x, y);
@@ -412,7 +417,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 // (a NaN score: the polynomial, which clamps its argument, would give that key weight 0, so it goes into the sum here)
                 l = mx == mx ? l * alpha : mx;
                 const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
-                const float neg = -mref * c;
+                const float neg = (HALF ? kPtHalfShift : 0.0f) - mref * c;
                 const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
                 uint64_t sum_a = 0ull, sum_b = 0ull;
 #pragma unroll

@@ -278,7 +278,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             // (a NaN score: see paged_tc.cuh)
             l = mx == mx ? l * alpha : mx;
             const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
-            const float neg = -mref * c;
+            const float neg = (HALF ? kPtHalfShift : 0.0f) - mref * c;
             const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
             uint64_t sum_a = 0ull, sum_b = 0ull;
 #pragma unroll

@@ -282,3 +282,23 @@ def test_rows_of_zeros_over_8_bit_pages(d, dtype):
     c.check(c.ctx.paged_attention(c.batch, 0, c.q))
     took = device_time(lambda: c.ctx.paged_attention(c.batch, 0, c.q))
     assert took < 5 * usual, (took, usual)  # (one row again, key by key, would take hundreds of times as long)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_small_weights_over_8_bit_pages(d):
+    """One key has a weight of 1 and 20000 others 2^-26 of it, which together make 3e-4 of the sum, and all of the result."""
+    n, gap = 20150, 26 * math.log(2.0)
+    c = Case(4, 2, d, "q8_head", "bf16", 64, [150], [n], seed=35)
+    c.q.fill_(1.0)
+    high = 2.0
+    low = high - gap / math.sqrt(d)  # q . k / sqrt(d) = sqrt(d) x for a key of elements x
+    rows = torch.full((2, n), low, device="cuda")
+    rows[0, 0], rows[1], rows[1, 0] = high, 1.0, 0.0
+    for i in range(2):
+        for p in range(n):
+            page, row = c.table[0][p // 64], p % 64
+            c.pool[i][0, page, :, row] = 127
+            c.scales[i][0, page, :, row] = rows[i, p] / 127
+        step = (rows[i] / 127).double()
+        c.rows[0][i] = (127 * step).view(n, 1, 1).expand(n, 2, d).contiguous()
+    c.check(c.ctx.paged_attention(c.batch, 0, c.q))
