@@ -1010,8 +1010,11 @@ static int paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t ro
     if (rc) return rc;
     const PathView p = path_view(c);
     const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D, kv_dim = b->Hkv * b->D;
-    if ((rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v", v, &v_stride, kv_dim, es))) return rc;
     if (!rotate && (q || q_out)) return path_fail(c, GGR_ERR_INVALID, "q is taken only to be rotated");
+    Guard guard(p.device);
+    const bool capturing = path_capturing(c);
+    if (!b->n_tokens && !capturing) return GGR_OK;  // (rows of an empty tensor may have no address)
+    if ((rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v", v, &v_stride, kv_dim, es))) return rc;
     int64_t qo_stride = q_dim;
     if (rotate) {
         if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "q_out", q_out, &qo_stride, q_dim, es))) return rc;
@@ -1019,9 +1022,6 @@ static int paged_append(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t ro
         if (q == q_out && (p.rope_dim != b->D || q_stride != qo_stride))
             return path_fail(c, GGR_ERR_INVALID, "q_out may be q itself only for dense rows whose heads are rotated as a whole");
     }
-    Guard guard(p.device);
-    const bool capturing = path_capturing(c);
-    if (!b->n_tokens && !capturing) return GGR_OK;
     int in_bf16 = b->dtype == GGR_DTYPE_BF16;
     if (rotate && path_has_fixups(c, layer)) {
         if (q_stride != q_dim || k_stride != kv_dim || v_stride != kv_dim) return path_fail(c, GGR_ERR_UNSUPPORTED, "bias and QK-norm need dense rows");
@@ -1071,11 +1071,11 @@ static int paged_read(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, int32_t out_
     if (rc) return rc;
     if (out_dtype != GGR_DTYPE_F32 && out_dtype != GGR_DTYPE_BF16) return path_fail(c, GGR_ERR_INVALID, "unknown dtype");
     const int kv_dim = b->Hkv * b->D, es = elem_bytes(out_dtype);
-    if ((rc = check_rows(c, "k_out", k_out, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v_out", v_out, &v_stride, kv_dim, es))) return rc;
     const PathView p = path_view(c);
     Guard guard(p.device);
     const bool capturing = path_capturing(c);
     if (!b->n_entries && !capturing) return GGR_OK;
+    if ((rc = check_rows(c, "k_out", k_out, &k_stride, kv_dim, es)) || (rc = check_rows(c, "v_out", v_out, &v_stride, kv_dim, es))) return rc;
     ReadArgs a{};
     a.pages = b->pages->v;
     a.counts = b->counts(0, 0);
@@ -1107,11 +1107,11 @@ static int paged_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const v
     if (rc) return rc;
     const PathView p = path_view(c);
     const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D;
-    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es))) return rc;
     if (p.image_blocks) return path_fail(c, GGR_ERR_UNSUPPORTED, "bidirectional blocks belong to one generation: batches attend causally");
     Guard guard(p.device);
     const bool capturing = path_capturing(c);
     if (!b->n_tokens && !capturing) return GGR_OK;
+    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es))) return rc;
     PagedAttnArgs a = attention_args(p, b, layer);
     a.paged = 1;
     a.pages = b->pages->v;
@@ -1135,13 +1135,13 @@ static int packed_attention(ggr_attn_ctx* c, ggr_batch* b, int32_t layer, const 
     if (rc) return rc;
     const PathView p = path_view(c);
     const int es = elem_bytes(b->dtype), q_dim = b->Hq * b->D, kv_dim = b->Hkv * b->D;
-    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) ||
-        (rc = check_rows(c, "v", v, &v_stride, kv_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es)))
-        return rc;
     if (p.image_blocks) return path_fail(c, GGR_ERR_UNSUPPORTED, "bidirectional blocks belong to one generation: batches attend causally");
     Guard guard(p.device);
     const bool capturing = path_capturing(c);
     if (!b->n_tokens && !capturing) return GGR_OK;
+    if ((rc = check_rows(c, "q", q, &q_stride, q_dim, es)) || (rc = check_rows(c, "k", k, &k_stride, kv_dim, es)) ||
+        (rc = check_rows(c, "v", v, &v_stride, kv_dim, es)) || (rc = check_rows(c, "out", out, &out_stride, q_dim, es)))
+        return rc;
     const int rows = capturing ? b->max_tokens : b->n_tokens;
     const bool f32 = b->dtype == GGR_DTYPE_F32;
     PagedAttnArgs a = attention_args(p, b, layer);

@@ -302,3 +302,26 @@ def test_many_small_weights_over_8_bit_pages(d):
         step = (rows[i] / 127).double()
         c.rows[0][i] = (127 * step).view(n, 1, 1).expand(n, 2, d).contiguous()
     c.check(c.ctx.paged_attention(c.batch, 0, c.q))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_steps_without_new_tokens(dtype):
+    c = Case(4, 2, 64, "bf16", dtype, 16, [1, 1], [20, 40], seed=37)
+    none = [torch.empty(0, h * 64, dtype=c.dtype, device="cuda") for h in (4, 2, 2)]
+    for q_len, kv_len, table in (([0, 0], [20, 40], c.table), ([0, 0], [0, 0], [[], []]), ([], [], [])):
+        c.batch.set(q_len, kv_len, table)
+        assert c.ctx.paged_append(c.batch, 0, none[1], none[2], q=none[0]).shape == (0, 256)
+        assert c.ctx.paged_append(c.batch, 0, none[1], none[2]) is None
+        assert c.ctx.paged_attention(c.batch, 0, none[0]).shape == (0, 256)
+        k, v = c.ctx.paged_read(c.batch, 0, "f32")
+        assert k.shape == v.shape == (sum(kv_len), 128)
+        if k.shape[0]:
+            assert torch.equal(k.double(), torch.cat([r[0] for r in c.rows]).view(60, 128))
+    packed = g.Batch(c.ctx, None, dtype, 2, 10)
+    for lens in ([0, 0], []):
+        packed.set(lens)
+        assert c.ctx.packed_attention(packed, 0, *none).shape == (0, 256)
+    with pytest.raises(GgrError):  # what is wrong stays so
+        c.ctx.paged_attention(c.batch, 1, none[0])
+    with pytest.raises(ValueError):
+        c.ctx.paged_attention(c.batch, 0, none[1])
