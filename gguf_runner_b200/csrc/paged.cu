@@ -644,9 +644,19 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
                 cudaFree(b->d_dense);
             }
             b->d_dense = nullptr;
+            // twice what it was, so that a prompt that comes in chunks makes room a few times and not at every step; the plan's pages
+            // are the most that can be asked for
+            size_t want = std::min(std::max<size_t>(2 * b->dense_rows, 4096), (size_t)b->max_pages * ps);
+            want = std::max(std::min(want, ((size_t)1 << 31) - 1), (size_t)dense);
             b->dense_rows = 0;
-            const size_t want = (size_t)std::max<int64_t>(dense, 4096);
-            if (want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__half)) == cudaSuccess) {
+            auto make = [&] { return want < ((size_t)1 << 31) && cudaMalloc((void**)&b->d_dense, 2 * want * row * sizeof(__half)) == cudaSuccess; };
+            bool made = make();
+            if (!made && want > (size_t)dense) {
+                cudaGetLastError();
+                want = (size_t)dense;
+                made = make();
+            }
+            if (made) {
                 if (!make_map3(&b->tmKd, false, b->d_dense, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, tc_key_tile(b->D)) ||
                     !make_map3(&b->tmVd, false, b->d_dense + want * row, b->D, b->Hkv, want, (uint64_t)b->D * 2, row * 2, 64, 1, tc_key_tile(b->D)))
                     return path_fail(c, GGR_ERR_CUDA, "cuTensorMapEncodeTiled failed for the dequantised rows");

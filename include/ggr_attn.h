@@ -385,7 +385,9 @@ int ggr_attn_layer_prefill(ggr_attn_ctx* ctx, int32_t layer, int32_t seq, int32_
  * cache is not touched (seq_len 1 keeps it small). head_dim 64, 128 or 256, any number of query heads per KV head. Rows are
  * device memory in the plan's dtype (GGR_DTYPE_BF16: tensor-core arithmetic of bf16 operands; GGR_DTYPE_F32: 32-bit
  * precision), 16-byte aligned, with a row stride in elements (0 = dense; a multiple of 16 bytes), so that q, k and v may be
- * slices of one projection. Outputs have the same dtype. Calls only enqueue work on the context's stream.
+ * slices of one projection. Outputs have the same dtype. Calls only enqueue work on the context's stream,
+ * but for ggr_batch_set when a step needs more scratch than any before it (the first with chunks; 8-bit pages: chunks behind twice as
+ * many tokens): it then waits for the stream and allocates.
  */
 typedef struct ggr_pages ggr_pages;
 typedef struct ggr_batch ggr_batch;

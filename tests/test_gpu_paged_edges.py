@@ -325,3 +325,26 @@ def test_steps_without_new_tokens(dtype):
         c.ctx.paged_attention(c.batch, 1, none[0])
     with pytest.raises(ValueError):
         c.ctx.paged_attention(c.batch, 0, none[1])
+
+
+def test_a_prompt_in_chunks_over_8_bit_pages():
+    """The rows that 8-bit chunks are multiplied as grow with the prompt: the room for them is not made anew at every step."""
+    total, step = 16384, 1024
+    c = Case(16, 8, 128, "q8_head", "bf16", 64, [step], [total], seed=38)
+    c.batch = g.Batch(c.ctx, c.pages, "bf16", 1, step, total // 64)
+    q, free = c.q, []
+    torch.empty(1 << 30, dtype=torch.uint8, device="cuda")  # (what the checks need: from torch's cache)
+    for n in range(step, total + 1, step):
+        c.batch.set([step], [n], c.table)
+        got = c.ctx.paged_attention(c.batch, 0, q)
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+        if n in (step, 5 * step, total):
+            c.kv_len, rows = [n], c.rows
+            c.rows = [[x[:n] for x in rows[0]]]
+            c.q = q[-40:]
+            c.q_len = [40]
+            out, size, reach = c.want()
+            assert bool(((got[-40:].double() - out).abs() <= ref.bound(c.dtype, out, size, reach)).all())
+            c.rows = rows
+    assert len(set(free[1:])) <= 3, free  # 4096 rows, 8192, 16384
