@@ -307,7 +307,8 @@ __device__ __forceinline__ float code_value(uint32_t w, int i) { return __uint_a
 
 // Rows of all sequences out of their pages. A thread has 16 bytes of output at a time (E elements), so that a warp's stores, and
 // its loads, are whole lines; a CTA takes blocks of 16 rows of one KV head of K and of V, UN of them at once: the page ids of
-// all are fetched before the rows of any, and all rows before the first is stored (a block alone is two dependent loads).
+// all are fetched before the rows of any, and all rows before the first is stored (a block alone is two dependent loads). Rows come
+// by plain loads: the launch in front may still write them while this one's CTAs are there already, waiting for it.
 template <int FMT, int D, int OUT>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
     constexpr int E = OUT == kReadF32 ? 4 : 8;
@@ -348,15 +349,15 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
                     const int64_t row = a.pages.row(a.layer, slot[u] >> a.pages.page_log2, head[u], (slot[u] & ((1 << a.pages.page_log2) - 1)) + r);
                     const unsigned char* src = (v ? a.pages.v : a.pages.k) + (row * D + e) * (FMT == KV_BF16 ? 2 : 1);
                     if constexpr (FMT == KV_BF16 && E == 8) {
-                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
+                        const uint4 x = *reinterpret_cast<const uint4*>(src);
                         raw[v][i][0] = x.x, raw[v][i][1] = x.y, raw[v][i][2] = x.z, raw[v][i][3] = x.w;
                     } else if constexpr (FMT == KV_BF16 || E == 8) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(src));
+                        const uint2 x = *reinterpret_cast<const uint2*>(src);
                         raw[v][i][0] = x.x, raw[v][i][1] = x.y;
                     } else {
-                        raw[v][i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+                        raw[v][i][0] = *reinterpret_cast<const uint32_t*>(src);
                     }
-                    if constexpr (FMT != KV_BF16) scale[v][i] = __ldg((v ? a.pages.vs : a.pages.ks) + row);
+                    if constexpr (FMT != KV_BF16) scale[v][i] = (v ? a.pages.vs : a.pages.ks)[row];
                 }
 #pragma unroll
         for (int u = 0; u < UN; ++u)
