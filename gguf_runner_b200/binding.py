@@ -337,14 +337,26 @@ def _raw_stream(device: int) -> int:
     return _RAW_STREAM(device)
 
 
+_IS_CAPTURING = None
+
+
 def _capturing() -> bool:
-    import torch
-    return torch.cuda.is_current_stream_capturing()
+    """Whether torch's current stream is captured."""
+    global _IS_CAPTURING
+    if _IS_CAPTURING is None:
+        import torch
+        _IS_CAPTURING = torch.cuda.is_current_stream_capturing
+    return _IS_CAPTURING()
+
+
+_TORCH_DTYPES = {}
 
 
 def _torch_dtype(name: str):
-    import torch
-    return torch.float32 if name == "f32" else torch.bfloat16
+    if not _TORCH_DTYPES:
+        import torch
+        _TORCH_DTYPES.update(f32=torch.float32, bf16=torch.bfloat16)
+    return _TORCH_DTYPES[name]
 
 
 class Pages:
@@ -406,7 +418,7 @@ class Batch:
         self._L, self.ctx, self.pages, self.dtype = lib(), ctx, pages, dtype
         self.max_tokens, self.n_tokens, self.n_rows = max_tokens, 0, 0
         self.max_rows = 0 if pages is None else max_pages * pages.page_size
-        self.torch_dtype = _torch_dtype(dtype)
+        self.torch_dtype, self._torch_device = _torch_dtype(dtype), None
         h = C.c_void_p()
         ctx._check(self._L.ggr_batch_create(ctx._h, None if pages is None else pages._h, DTYPES[dtype], max_seqs, max_tokens, max_pages,
                                             C.byref(h)))
@@ -823,12 +835,15 @@ class AttnContext:
         captured call may find a longer plan: its tensors have the rows of all pages that the plan may name.)"""
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
-        dt, c, n, most = _torch_dtype(dtype), self.config, batch.n_rows, batch.max_rows if _capturing() else 0
+        dt, n, most = _torch_dtype(dtype), batch.n_rows, batch.max_rows if _capturing() else 0
         if k_out is None or v_out is None:
             import torch
-            k_out, v_out = (torch.empty((max(n, most), c.kv_dim), dtype=dt, device=f"cuda:{c.device}") if o is None else o for o in (k_out, v_out))
-        kp, ks = self._rows("k_out", k_out, dt, n, c.kv_dim, most)
-        vp, vs = self._rows("v_out", v_out, dt, n, c.kv_dim, most)
+            if batch._torch_device is None:  # (an object: torch takes 0.15 us to read a name)
+                batch._torch_device = torch.device("cuda", self._device)
+            rows = (max(n, most), self._kv_dim)
+            k_out, v_out = (torch.empty(rows, dtype=dt, device=batch._torch_device) if o is None else o for o in (k_out, v_out))
+        kp, ks = self._rows("k_out", k_out, dt, n, self._kv_dim, most)
+        vp, vs = self._rows("v_out", v_out, dt, n, self._kv_dim, most)
         self._follow_torch_stream_of_device()
         self._check(self._L.ggr_paged_read(self._h, batch._h, layer, DTYPES[dtype], kp, ks, vp, vs))
         return k_out, v_out
