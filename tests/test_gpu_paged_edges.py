@@ -348,3 +348,114 @@ def test_a_prompt_in_chunks_over_8_bit_pages():
             assert bool(((got[-40:].double() - out).abs() <= ref.bound(c.dtype, out, size, reach)).all())
             c.rows = rows
     assert len(set(free[1:])) <= 3, free  # 4096 rows, 8192, 16384
+
+
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("bf16", "q8_head"), ("f32", "bf16"), ("f32", "q8_head")])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_layers_with_windows_of_their_own(d, kv, dtype):
+    """Window and global layers of one plan: short and long texts, chunks and single tokens, cut and uncut."""
+    windows = (100, 0, 33, 100, 2000)
+    c = Case(8, 2, d, kv, dtype, 32, [1, 70, 3, 150], [9000, 5000, 40, 700], seed=45)
+    pool, scales = ([None if x is None else x.expand(5, *x.shape[1:]).contiguous() for x in arrays] for arrays in (c.pool, c.scales))
+    c.ctx = context(8, 2, d, layers=5, windows=windows)
+    c.pages = g.Pages(c.ctx, c.pages.n_pages, 32, kv, *pool, *scales)
+    c.batch = g.Batch(c.ctx, c.pages, dtype, 4, 224, sum(map(len, c.table)))
+    c.batch.set(c.q_len, c.kv_len, c.table)
+    got = [c.ctx.paged_attention(c.batch, layer, c.q) for layer in range(5)]
+    for layer, window in enumerate(windows):
+        c.window = window
+        if layer != 3:
+            c.check(got[layer])
+    assert torch.equal(got[3], got[0])
+
+
+def test_more_windows_than_a_plan_has_lists_for():
+    ctx = context(4, 2, 64, layers=5, windows=(1, 2, 3, 4, 5))
+    with pytest.raises(GgrError):
+        g.Batch(ctx, None, "bf16", 1, 1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv", ["bf16", "q8_head"])
+def test_captured_steps_rotate_by_the_replayed_plan(kv, dtype):
+    """Rotating append and attention of a token step in a graph, replayed at other lengths, over other pages."""
+    c = Case(8, 2, 128, kv, dtype, 16, [1, 1, 1], [700, 900, 64], seed=46)
+    gen = torch.Generator(device="cuda").manual_seed(47)
+    q, k, v = (torch.randn(3, h * 128, generator=gen, device="cuda").to(c.dtype) for h in (8, 2, 2))
+    turned, out = torch.empty_like(q), torch.empty_like(q)
+    arrays = [x for x in c.pool + c.scales if x is not None]
+    start = [x.clone() for x in arrays]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+
+    def step():
+        c.ctx.paged_append(c.batch, 0, k, v, q=q, q_out=turned)
+        c.ctx.paged_attention(c.batch, 0, turned, out=out)
+
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+        for n, kv_len in ((3, [700, 900, 64]), (3, [12, 1, 17]), (2, [650, 800])):
+            results = []
+            for run in (graph.replay, step):
+                for x, s in zip(arrays, start):
+                    x.copy_(s)
+                turned.fill_(7.0)
+                out.fill_(7.0)
+                c.batch.set([1] * n, kv_len, c.table[:n])
+                run()
+                side.synchronize()
+                results.append([x.clone() for x in (turned, out, *arrays)])
+            for a, b in zip(*results):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            assert bool((results[0][0][n:] == 7.0).all()) and bool((results[0][1][n:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv", ["bf16", "q8_head"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_with_strides(d, kv, dtype):
+    """q as a slice of a projection's output, results into a slice of another buffer, over single tokens and chunks."""
+    c = Case(8, 4, d, kv, dtype, 16, [1, 150, 20], [400, 300, 21], seed=48)
+    n, dim = c.q.shape
+    wide = torch.full((n, dim + 64), math.nan, dtype=c.dtype, device="cuda")
+    wide[:, 32:32 + dim] = c.q
+    into = torch.full((n + 1, dim + 128), 7.0, dtype=c.dtype, device="cuda")
+    c.ctx.paged_attention(c.batch, 0, wide[:, 32:32 + dim], out=into[:, 64:64 + dim])
+    c.check(into[:n, 64:64 + dim])
+    into[:n, 64:64 + dim] = 7.0
+    assert bool((into == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("bf16", "q8_head"), ("f32", "q8_head")])
+def test_contexts_on_two_streams_at_once(dtype, kv):
+    """Two contexts, one in a replayed graph, with launches that run beside each other: the results are those of each alone."""
+    cases = [Case(8, 2, 128, kv, dtype, 16, q_len, kv_len, seed=49 + i) for i, (q_len, kv_len) in
+             enumerate((([1, 200, 3], [6000, 4000, 90]), ([1, 70, 1], [9000, 3000, 1])))]
+    want = [c.ctx.paged_attention(c.batch, 0, c.q).clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [torch.empty_like(c.q) for c in cases]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        cases[0].ctx.paged_attention(cases[0].batch, 0, cases[0].q, out=outs[0])
+        streams[0].synchronize()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            cases[0].ctx.paged_attention(cases[0].batch, 0, cases[0].q, out=outs[0])
+        graph.replay()
+        streams[0].synchronize()
+    first = outs[0].clone()
+    cases[0].check(first)
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            with torch.cuda.stream(streams[0]):
+                graph.replay()
+            with torch.cuda.stream(streams[1]):
+                cases[1].ctx.paged_attention(cases[1].batch, 0, cases[1].q, out=outs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], first) and torch.equal(outs[1], want[1])
