@@ -170,7 +170,8 @@ int ggr::batch_check(int32_t page_size, int32_t n_pages, int32_t n_seqs, const i
     }
     if (totals->tokens > max_tokens) return bad(GGR_ERR_RANGE, "more new tokens than the batch plan holds");
     if (totals->entries > max_pages) return bad(GGR_ERR_RANGE, "more pages than the batch plan holds");
-    if (totals->rows >= ((int64_t)1 << 31)) return bad(GGR_ERR_RANGE, "more rows than a 32-bit index names");
+    // (the kernels reach up to a few tiles of keys past the last one before they compare)
+    if (totals->rows >= ((int64_t)1 << 31) - 1024) return bad(GGR_ERR_RANGE, "more rows than a 32-bit index names");
     if (totals->entries && !page_table) return bad(GGR_ERR_INVALID, "null page table");
     // a page takes new rows of one sequence only: two would write the same place
     std::vector<int32_t> written;

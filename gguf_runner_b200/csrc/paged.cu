@@ -740,7 +740,7 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
                 for (int s = 0; s < it.n_split; ++s) {
                     it.split = s;
                     it.key0 = t.key0 + s * each * 16;
-                    it.key1 = std::min(t.key1, it.key0 + each * 16);
+                    it.key1 = (int)std::min<int64_t>(t.key1, it.key0 + (int64_t)each * 16);
                     items[n++] = it;
                 }
             }
@@ -776,7 +776,7 @@ static int batch_set(ggr_batch* b, int32_t n_seqs, const int32_t* q_len, const i
                     for (int s = 0; s < it.n_split; ++s) {
                         it.split = s;
                         it.key0 = t.key0 + s * each * kt;
-                        it.key1 = std::min(t.key1, it.key0 + each * kt);
+                        it.key1 = (int)std::min<int64_t>(t.key1, it.key0 + (int64_t)each * kt);
                         b->scratch.push_back(it);
                         if (s == 0 && it.n_split > 1) merge[n_merge++] = it;
                     }

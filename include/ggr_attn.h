@@ -406,10 +406,10 @@ void ggr_pages_destroy(ggr_pages* pages);
 int ggr_pages_device_ptrs(const ggr_pages* pages, void** k, void** v, float** k_scale, float** v_scale,
                           uint64_t* array_bytes);
 /*
- * A batch plan with room for max_seqs sequences, max_tokens new tokens and max_pages page table entries in all. pages null:
- * a plan for ggr_packed_attention (max_pages 0). A plan owns the scratch of its launches: launches of one plan have to be
- * ordered (one stream, or events between), different plans are independent. Destroy a plan before its context; work that
- * uses it is waited for.
+ * A batch plan with room for max_seqs sequences, max_tokens new tokens and max_pages page table entries in all (a step has
+ * fewer than 2^31 - 1024 tokens, cached ones included). pages null: a plan for ggr_packed_attention (max_pages 0). A plan owns
+ * the scratch of its launches: launches of one plan have to be ordered (one stream, or events between), different plans are
+ * independent. Destroy a plan before its context; work that uses it is waited for.
  */
 int ggr_batch_create(ggr_attn_ctx* ctx, ggr_pages* pages, int32_t dtype, int32_t max_seqs, int32_t max_tokens,
                      int32_t max_pages, ggr_batch** out);
