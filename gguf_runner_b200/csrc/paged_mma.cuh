@@ -159,15 +159,15 @@ __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const Paged
         const int n = min(32, pos + 1 - j0);
         const int64_t row = row_of(j0 + min(lane, n - 1));
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float step = q8 ? a.pages.ks[row] : 1.0f;
 #pragma unroll 8
         for (int d = 0; d < D; d += 8) {
             float x[8];
             paged_elems<8, FMT>(keys, row * k_step + head + d, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[e & 3] = fmaf(__shfl_sync(0xffffffffu, q[e % E], (d + e) / E), x[e], part[e & 3]);
+            for (int e = 0; e < 8; ++e) part[e & 3] = fmaf(__shfl_sync(0xffffffffu, q[e % E], (d + e) / E), q8 ? x[e] * step : x[e], part[e & 3]);
         }
         float s = ((part[0] + part[1]) + (part[2] + part[3])) * a.c;
-        if constexpr (q8) s *= a.pages.ks[row];
         if (lane >= n) s = -INFINITY;
         // (a score of -inf has weight 0, also while there is no larger one to measure it by)
         const float top = fmaxf(m, warp_max(s)), f = m == top ? 1.0f : exp2f(m - top);
