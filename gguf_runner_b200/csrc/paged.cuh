@@ -289,9 +289,9 @@ struct ReadArgs {
     int q_dim;
 };
 
-// kReadHalf: f16 operands of the tcgen05 kernel. V is taken times 64, so that values of 6e-8 to 1000 keep the precision of a
-// bf16 row or better; what f16 cannot hold (or was not finite) becomes NaN, and rows that meet it are computed again from the
-// pages in f32.
+// kReadHalf: f16 operands of the tcgen05 kernel. V is taken times 64, so that values of 1.2e-7 to 1023 keep the precision of a
+// bf16 row or better (smaller ones are off by at most 2^-31); what f16 cannot hold (or was not finite) becomes NaN, and rows that
+// meet it are computed again from the pages in f32.
 enum ReadOut { kReadF32 = 0, kReadBf16 = 1, kReadHalf = 2 };
 constexpr float kReadVScale = 64.0f;
 

@@ -21,8 +21,9 @@
 // instructions per product instead of two or three, and both halves of a row lie in one lane.
 //
 // Keys that only some rows of a tile see get weight 0, and 0 times an infinity or NaN in a value would spoil the other rows:
-// a row whose result is not finite is computed again, key by key, by paged_row_again. Rows of a tile that nobody sees
-// (behind the sequence's end, before its window: never written, freed or another sequence's) are cleared in shared memory.
+// a row whose result is not finite is computed again, by a warp of its own, by paged_row_again (unless it must be NaN: see there).
+// Rows of a tile that nobody sees (behind the sequence's end, before its window: never written, freed or another sequence's) are
+// cleared in shared memory.
 #pragma once
 
 #include "mma_utils.cuh"
@@ -122,7 +123,8 @@ __device__ __forceinline__ void paged_elems(const void* rows, int64_t at, float 
 // One row again in f32, by a warp: what is not seen is not touched. Only rows whose fast result is not finite, and not known to be
 // right as it is (a bf16 row's sum of weights is NaN when one of its scores is, whatever the values are). 32 keys at a time: a lane
 // takes q times one of them, then every lane D / 32 elements of their values. A row that has met a NaN score is NaN, and is left
-// there; of 8-bit pages the scales tell before anything else is read. `steps`: in shared memory, see paged_wait.
+// there; of 8-bit pages the scales tell before anything else is read. Bound by the latency of each 32 keys' loads, 0.25 us a key at
+// head_dim 64 and 128, 0.45 at 256 (one key after the other: 1.2, 2.2 and 4.4). `steps`: in shared memory, see paged_wait.
 template <int D, int FMT, bool F32>
 __device__ __noinline__ void paged_row_again(const PagedAttnArgs& a, const PagedItem& w, int kvh, int r, int lane, int* steps = nullptr) {
     constexpr int E = D / 32;

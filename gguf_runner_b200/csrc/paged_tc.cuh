@@ -9,7 +9,7 @@
 //    of the producer warp side by side; each lane looks its page up one tile ahead.
 //  - Items (two query tiles and a stretch of keys) are cut on the host, longest first, and handed out through a counter. Pieces
 //    of a pair of tiles leave un-normalised rows, which paged_tc_merge_kernel weighs in the order of the keys.
-//  - 8-bit pages are read into dense f16 rows first (paged_read_kernel, 34 us of 602 for 2048 tokens behind 14336, 40/8 heads
+//  - 8-bit pages are read into dense f16 rows first (paged_read_kernel, 34 us of 680 for 2048 tokens behind 14336, 40/8 heads
 //    of 128), q into f16 beside them: eleven bits leave code * scale 2^-12 off, an eighth of what bf16 weights are (weights: see
 //    kPtHalfShift). bf16 rows would add two roundings as large as that of the weights (by their variances 3.2e-3 instead of 2.3e-3
 //    from 64 bits), and scales that the softmax warps multiply into scores and weights are two multiplications and half a

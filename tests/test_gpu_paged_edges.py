@@ -459,3 +459,21 @@ def test_contexts_on_two_streams_at_once(dtype, kv):
                 cases[1].ctx.paged_attention(cases[1].batch, 0, cases[1].q, out=outs[1])
         torch.cuda.synchronize()
         assert torch.equal(outs[0], first) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv", ["bf16", "q8_head"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_of_q_that_are_not_finite_or_large(d, kv, dtype):
+    """A row of q with a NaN is a row of NaNs, and the rows beside it in its tile are right; so is a row that f16 does not hold."""
+    c = Case(8, 2, d, kv, dtype, 32, [1, 150, 4], [900, 333, 60], seed=51)
+    rows = c.q.view(155, 8, d)
+    rows[0, 3, 7] = rows[20, 5, 0] = rows[152, 0, d - 1] = math.nan
+    rows[0, 4] *= 1e5
+    rows[30, 2] *= 1e5
+    got = c.ctx.paged_attention(c.batch, 0, c.q).view(155, 8, d)
+    spoilt = rows.isnan().any(-1)
+    assert bool(got[spoilt].isnan().all())
+    out, size, reach = (x.view(155, 8, d) for x in c.want())
+    ok = (got.double() - out).abs() <= ref.bound(c.dtype, out, size, reach)
+    assert bool(ok[~spoilt].all())
