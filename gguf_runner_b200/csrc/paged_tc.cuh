@@ -367,6 +367,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 vs = paged_first_key(w.pos0 + tok, a.window);
             }
             float m_used = -INFINITY, l = 0.0f;
+            bool odd = false;
             for (int j = lo_t; j < hi_t; ++j) {
                 const int k = j - lo_t;
                 if (!(ok = paged_wait(s_full(t), (cs + k) & 1, abortp))) break;
@@ -397,6 +398,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                     }
                 const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
+                // (a NaN score: the polynomial, which clamps its argument, would give that key weight 0)
+                odd |= mx != mx;
                 const bool need = mx > m_used + thr;
                 float alpha = 1.0f;
                 if (need) {
@@ -414,8 +417,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         tmem_st32(tO + cidx * 32, orow);
                     }
                 }
-                // (a NaN score: the polynomial, which clamps its argument, would give that key weight 0, so it goes into the sum here)
-                l = mx == mx ? l * alpha : mx;
+                l *= alpha;
                 const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
                 const float neg = (HALF ? kPtHalfShift : 0.0f) - mref * c;
                 const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
@@ -471,7 +473,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             cs += n_t;
             if (!(ok = paged_wait(o_final(t), it & 1, abortp))) break;
             fence_after_sync();
-            if (m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
+            if (odd || m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
             const bool split = w.part >= 0;
             if (m_used == -INFINITY && l == l) l = split ? 0.0f : NAN;  // only scores of -inf: no softmax; a piece without weight
             float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPtState<D>;

@@ -198,6 +198,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const uint32_t tO = tmem + lane_addr + O_COL0;
         const float c = a.c, thr = 8.0f / c;
         float m_used = -INFINITY, l = 0.0f;
+        bool odd = false;
         bool ok = true;
         const int64_t tok_row = w.tok0 + w.row0 + tok;
         if (hi > lo) {
@@ -254,6 +255,8 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                 }
             const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
+            // (a NaN score: see paged_tc.cuh)
+            odd |= mx != mx;
             const bool need = mx > m_used + thr;
             float alpha = 1.0f;
             if (need) {
@@ -275,8 +278,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     tmem_st32(tO + cidx * 32, orow);
                 }
             }
-            // (a NaN score: see paged_tc.cuh)
-            l = mx == mx ? l * alpha : mx;
+            l *= alpha;
             const float mref = (m_used == -INFINITY) ? 0.0f : m_used;
             const float neg = (HALF ? kPtHalfShift : 0.0f) - mref * c;
             const uint64_t c2 = pack_f32x2(c, c), neg2 = pack_f32x2(neg, neg);
@@ -328,7 +330,7 @@ paged_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             if (n > 0 && !rescale_now && !(ok = mbar_wait(pv_done((n - 1) & 1), ((n - 1) >> 1) & 1, abortp))) break;
         }
         if (ok && hi > lo) ok = mbar_wait(o_final, 0, abortp);
-        if (m_used == INFINITY) l = NAN;  // (see paged_tc.cuh)
+        if (odd || m_used == INFINITY) l = NAN;  // (see paged_tc.cuh)
         const bool split = w.part >= 0;
         if (m_used == -INFINITY && l == l) l = split ? 0.0f : NAN;
         float* state = p.part + (int64_t)(split ? w.part + w.split : 0) * kPwState;

@@ -462,6 +462,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             int vs = 0, ve = 0;
             if (valid) a.vis.range(a.base_pos + qi, vs, ve);
             float m_used = -INFINITY, l = 0.0f;
+            bool odd = false;
             for (int j = lo_t; j < hi_t; ++j) {
                 const int k = j - lo_t;
                 TRACE_MARK();
@@ -490,15 +491,17 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 for (int cidx = 0; cidx < 4; ++cidx)
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        mxa = max3(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
-                        mxb = max3(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
-                        mxc = max3(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
-                        mxd = max3(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
+                        mxa = max3_nan(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
+                        mxb = max3_nan(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
+                        mxc = max3_nan(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
+                        mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                     }
-                const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+                const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
                 TRACE_ADD(ts_max);
                 if ((warp & 3) == 0) TRACE_EVT(j - lo, 10 + t * 8);
                 // lazy rescale of the running output
+                // (a NaN score: the polynomial, which clamps its argument, would give that key weight 0)
+                odd |= mx != mx;
                 const bool need = mx > m_used + thr;
                 float alpha = 1.0f;
                 if (need) {
@@ -577,6 +580,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (!(ok = mbar_wait(o_final(t), it & 1, abortp))) break;
             TRACE_ADD(ts_ofin);
             fence_after_sync();
+            if (odd || m_used == INFINITY) l = NAN;  // a score of +inf, whose weight the polynomial would also make 0
             float* orow0 = a.out;
             if constexpr (SPLIT) {
                 orow0 = a.part + (int64_t)w.split * a.m * Hq * D;
@@ -588,7 +592,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 // warp hit different banks; the warp then reads the area back four rows at a time and stores
                 // whole 128-byte lines. One thread per row storing 16-byte pieces 16 KB apart cost a cache-line
                 // wavefront per lane and instruction, 3-4 us per item during which the tile's pipeline stood still.
-                const float inv = SPLIT ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
+                const float inv = SPLIT ? 1.0f : (l <= 0.0f ? 0.0f : 1.0f / l);  // (NaN stays one)
                 const void* grow = nullptr;
                 if (!SPLIT && a.gate && valid)
                     grow = static_cast<const unsigned char*>(a.gate) +
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(PrefillTcArgs a) {
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s = 0; s < a.n_split; ++s) {
         const float2 ml = __ldcg(&a.ml[s * rows + row]);
-        if (ml.x == -INFINITY) continue;
+        if (ml.x == -INFINITY && ml.y == ml.y) continue;
         const float f = exp2f((ml.x - top) * a.score_scale);
         const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part + (s * rows + row) * D + d));
         l = fmaf(f, ml.y, l);
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(PrefillTcArgs a) {
         o.z = fmaf(f, x.z, o.z);
         o.w = fmaf(f, x.w, o.w);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l <= 0.0f ? 0.0f : 1.0f / l;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (a.gate)
         o = prefill_gate4(o, static_cast<const unsigned char*>(a.gate) + row * a.gate_head_stride * (a.gate_bf16 ? 2 : 4), a.gate_bf16, d);

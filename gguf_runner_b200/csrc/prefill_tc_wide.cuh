@@ -245,6 +245,7 @@ prefill_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const float c = a.score_scale;
         const float thr = 8.0f / c;
         float m_used = -INFINITY, l = 0.0f;
+        bool odd = false;
         bool ok = true;
 #ifdef GGR_TC_TRACE
         long long ts_wait = 0, ts_ld = 0, ts_max = 0, ts_resc = 0, ts_exp = 0, ts_t0 = clock64(), tr_x;
@@ -305,13 +306,15 @@ prefill_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             for (int cidx = 0; cidx < 2; ++cidx)
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
-                    mxa = max3(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
-                    mxb = max3(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
-                    mxc = max3(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
-                    mxd = max3(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
+                    mxa = max3_nan(mxa, __uint_as_float(sr[cidx][i]), __uint_as_float(sr[cidx][i + 1]));
+                    mxb = max3_nan(mxb, __uint_as_float(sr[cidx][i + 2]), __uint_as_float(sr[cidx][i + 3]));
+                    mxc = max3_nan(mxc, __uint_as_float(sr[cidx][i + 4]), __uint_as_float(sr[cidx][i + 5]));
+                    mxd = max3_nan(mxd, __uint_as_float(sr[cidx][i + 6]), __uint_as_float(sr[cidx][i + 7]));
                 }
-            const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+            const float mx = max3_nan(max3_nan(mxa, mxb, mxc), mxd, mxd);
             TRACE_ADD(ts_max);
+            // (a NaN score: see prefill_tc.cuh)
+            odd |= mx != mx;
             const bool need = mx > m_used + thr;
             float alpha = 1.0f;
             if (need) {
@@ -398,7 +401,8 @@ prefill_tc_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         if (threadIdx.x == 0) TW_STAMP(5);
         if (ok && hi > lo) {
             fence_after_sync();
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            if (odd || m_used == INFINITY) l = NAN;
+            const float inv = l <= 0.0f ? 0.0f : 1.0f / l;  // (NaN stays one)
             float* orow_g = a.out + ((int64_t)qi * Hq + h) * D;
             const void* grow = nullptr;
             if (a.gate && valid)

@@ -153,13 +153,8 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return __all_sync(0xffffffffu, ok);
 }
 
-// three-input max and packed two-lane f32 arithmetic (one issue slot for two elements)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-// the same, NaN where one of the three is (max.f32 drops it)
+// three-input max (NaN where one of the three is: max.f32 drops it) and packed two-lane f32 arithmetic (one issue slot for two
+// elements)
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
