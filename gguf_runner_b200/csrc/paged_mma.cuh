@@ -63,7 +63,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 
 // Bounded waits (see mbar_wait) of kernels in which other warps of the CTA may meanwhile compute rows again, which takes as long as
 // the row's keys are many: flags[0] is raised by whoever gives up, flags[1] counts paged_row_again's steps, some microseconds each,
-// and the limit starts anew as long as it moves. (By the limit alone a CTA would give up its items while a warp has 32 rows of 150000 keys, at 0.25 us a row and key.)
+// and the limit starts anew as long as it moves. (By the limit alone a CTA would give up its items while a warp has 32 rows of
+// 150000 keys, at 0.25 us a row and key.)
 __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int* flags) {
     if (tc::mbar_test(bar, parity)) return true;
     int seen = 0;
